@@ -222,7 +222,8 @@ def prepare(case, seed):
         from malaga_b200 import ops
 
         state["cache"] = ops.PagedKV(state["k"], state["v"], state["k_scale"], state["v_scale"])
-        state["seqs"] = ops.Seqs(state["table"], state["q_start"], state["kv_len"], max_new=max(new), max_len=max(ctx))
+        state["seqs"] = ops.Seqs(state["table"], state["q_start"], state["kv_len"], max_new=max(new), max_len=max(ctx),
+                                 tokens=tokens)
     return state
 
 
