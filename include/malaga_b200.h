@@ -193,6 +193,112 @@ MGB_API mgb_status mgb_profile_step(mgb_ctx *ctx, const mgb_batch *batch, uint32
 MGB_API mgb_status mgb_argmax_noalloc(const float *logits, uint32_t rows, uint32_t vocab, uint32_t *ids, float *vals,
                                       void *stream);
 
+/* ------------------------------------------------------------------------
+ * Serving-step operators on device memory: a paged K/V cache that many
+ * sequences share, attention of new tokens over it, and rules on logits with
+ * the greedy choice. No counterpart in the reference (its caches are dense
+ * tensors per batch, graph.rs:58-63). They belong to no context: every pointer
+ * below is device memory of the current device, every call is asynchronous on
+ * `stream` (a cudaStream_t, NULL = the legacy default stream) and allocates
+ * nothing, and all may be captured into a CUDA graph after a first call of the
+ * same shape. Device data out of range (a page number outside the cache, a
+ * position past its table, a token id outside the vocabulary) is skipped, never
+ * followed.
+ */
+
+typedef enum { MGB_F32 = 0, MGB_F16 = 1, MGB_BF16 = 2 } mgb_type;
+
+/* How a cache holds a row (one position of one head): as f16 numbers, or as
+ * 8-bit codes with one f32 scale: scale = max|x| / 127 and code = x / scale to
+ * the nearest whole number (halves to even), both in f32 arithmetic; a row of
+ * zeros has scale 0 and codes 0, one with an infinity or NaN the scale NaN. */
+typedef enum { MGB_KV_F16 = 0, MGB_KV_Q8 = 1 } mgb_kv_format;
+
+/* A paged cache in the caller's memory. heads: 1..65535; dim: 16, 32, 64 or
+ * 128; page: positions of a page, a power of two from 16 to 1024. */
+typedef struct {
+    void *k, *v;              /* [pages][heads][page][dim], 16-byte aligned */
+    float *k_scale, *v_scale; /* [pages][heads][page]; only with MGB_KV_Q8 */
+    uint32_t pages, heads, page, dim;
+    int32_t format; /* mgb_kv_format */
+} mgb_kv;
+
+/* The sequences of a call. The new tokens of sequence b are rows q_start[b] ..
+ * q_start[b + 1] - 1 of the call's packed rows, and stand at the last positions
+ * of its kv_len[b]; position p is in page table[b][p / page]. max_new and
+ * max_len, bounds of a sequence's new tokens and positions, only size the launch
+ * (0: as large as the rows and the table allow): a value that is too small costs
+ * time, not correctness. */
+typedef struct {
+    const int32_t *table;   /* [seqs][table_stride] page numbers */
+    const int32_t *q_start; /* [seqs + 1] */
+    const int32_t *kv_len;  /* [seqs] */
+    uint32_t seqs, table_stride;
+    uint32_t max_new, max_len;
+} mgb_kv_seqs;
+
+/* Packed rows [tokens][heads][dim] of numbers; strides in elements, a row's
+ * dim numbers are contiguous. */
+typedef struct {
+    void *data;
+    int64_t token_stride, head_stride;
+    uint32_t tokens, heads;
+    int32_t type; /* mgb_type */
+} mgb_rows;
+
+/* Writes the new tokens' K and V rows (`heads` = the cache's) into the pages,
+ * cast or quantised to its format. Two tokens of one call must not share a
+ * place. f16 caches round to nearest, beyond their range to infinity. */
+MGB_API mgb_status mgb_kv_write(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, const mgb_rows *v,
+                                void *stream);
+
+/* The reverse: the values that the cache holds at each sequence's last
+ * q_start[b + 1] - q_start[b] positions, as packed rows. A row that has no
+ * place in the cache comes back as zeros. */
+MGB_API mgb_status mgb_kv_read(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, const mgb_rows *v,
+                               void *stream);
+
+/* out[t][h] = softmax over keys of (scale * q[t][h] . k) times v, for every new
+ * token t and query head h (a multiple of the cache's heads; query head h reads
+ * cache head h / (q heads / cache heads)). causal: a token sees the positions up
+ * to its own; otherwise all kv_len[b]. A token that sees no position gets zeros.
+ * q and out may have different types and strides, and are f32, f16 or bf16;
+ * sums, maxima and outputs are held in f32 and rounded once. scale: of the
+ * scores, commonly 1 / sqrt(dim). */
+MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *q, const mgb_rows *out,
+                                 float scale, int causal, void *stream);
+
+/* Rules on `rows` rows of logits x (NULL / 0 members are rules that are absent).
+ * With c the number of times that a token stands among the first
+ * history_len[r] ids of history[r], in this order:
+ *   c > 0:  y = x > 0 ? x / repetition[r] : x * repetition[r]
+ *           y = y - (frequency[r] * c + presence[r])
+ *   bias:   y = y + the sum of bias[r][i] with bias_ids[r][i] = token
+ *   grammar g = allow_row[r] >= 0:  y = -inf where bit (token % 32) of
+ *           allow[g][token / 32] is clear
+ * Ids outside the vocabulary (padding such as -1) are ignored, and so is a
+ * grammar number outside 0 .. allow_rows - 1. */
+typedef struct {
+    const int32_t *history;     /* [rows][history_stride] */
+    const int32_t *history_len; /* [rows], NULL = history_stride */
+    const float *repetition, *frequency, *presence; /* [rows] */
+    const int32_t *bias_ids;    /* [rows][bias_count] */
+    const float *bias;          /* [rows][bias_count] */
+    const uint32_t *allow;      /* [allow_rows][allow_stride] */
+    const int32_t *allow_row;   /* [rows], NULL = every row follows allow[0] */
+    uint32_t history_stride, bias_count, allow_rows, allow_stride;
+} mgb_logit_rules;
+
+/* Applies the rules to logits [rows][vocab] (row stride in elements), and per
+ * row chooses the token with the largest y (the lowest id on ties; NaN is never
+ * chosen) and its log-probability y - log(sum of exp(y)), NaN left out of the
+ * sum. ids, logp and adjusted may each be NULL; adjusted gets y in the logits'
+ * type and may be the logits themselves. A row without a choice gets id -1 and
+ * logp -inf. */
+MGB_API mgb_status mgb_logits_choose(const void *logits, int type, int64_t row_stride, uint32_t rows, uint32_t vocab,
+                                     const mgb_logit_rules *rules, int32_t *ids, float *logp, void *adjusted,
+                                     int64_t adjusted_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,27 @@ class ModelInfo(ctypes.Structure):
         ("lm_head_bytes", ctypes.c_uint64)]
 
 
+class Kv(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _u32), ("heads", _u32),
+                ("page", _u32), ("dim", _u32), ("format", ctypes.c_int32)]
+
+
+class KvSeqs(ctypes.Structure):
+    _fields_ = [("table", _vp), ("q_start", _vp), ("kv_len", _vp), ("seqs", _u32), ("table_stride", _u32),
+                ("max_new", _u32), ("max_len", _u32)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", _vp), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("tokens", _u32),
+                ("heads", _u32), ("type", ctypes.c_int32)]
+
+
+class LogitRules(ctypes.Structure):
+    _fields_ = [("history", _vp), ("history_len", _vp), ("repetition", _vp), ("frequency", _vp), ("presence", _vp),
+                ("bias_ids", _vp), ("bias", _vp), ("allow", _vp), ("allow_row", _vp), ("history_stride", _u32),
+                ("bias_count", _u32), ("allow_rows", _u32), ("allow_stride", _u32)]
+
+
 SIGNATURES = {
     "mgb_default_options": (None, [ctypes.POINTER(Options)]),
     "mgb_open": (_i, [ctypes.c_char_p, _i, ctypes.POINTER(Options), ctypes.POINTER(_vp)]),
@@ -51,6 +72,10 @@ SIGNATURES = {
     "mgb_kernel_launches": (_u64, [_vp]),
     "mgb_profile_step": (_i, [_vp, _vp, _u32, _u32, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_float)]),
     "mgb_argmax_noalloc": (_i, [_vp, _u32, _u32, _vp, _vp, _vp]),
+    "mgb_kv_write": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "mgb_kv_read": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "mgb_kv_attend": (_i, [_vp, _vp, _vp, _vp, ctypes.c_float, _i, _vp]),
+    "mgb_logits_choose": (_i, [_vp, _i, ctypes.c_int64, _u32, _u32, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp]),
 }
 
 

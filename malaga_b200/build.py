@@ -8,6 +8,7 @@
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 
@@ -28,7 +29,8 @@ NVCC_FLAGS = [
     # device code of the many kernel instantiations is optimized in parallel
     "--split-compile=0",
 ]
-ENGINE_SOURCES = ["engine.cu", "noalloc.cu"]
+ENGINE_SOURCES = ["engine.cu", "noalloc.cu", "kvcache.cu", "kvattend.cu", "logits.cu"]
+OBJ_DIR = os.path.join(HERE, "_build")
 
 
 def _newer(target: str, sources: list[str]) -> bool:
@@ -38,19 +40,37 @@ def _newer(target: str, sources: list[str]) -> bool:
     return any(os.path.getmtime(s) > t for s in sources)
 
 
-def _deps() -> list[str]:
-    out = []
-    for dirpath, _, files in os.walk(CSRC):
-        out += [os.path.join(dirpath, f) for f in files if f.endswith((".cu", ".cuh", ".h", ".cpp"))]
-    return out + [os.path.join(ROOT, "include", "malaga_b200.h")]
+def _includes(path: str, seen: set[str] | None = None) -> set[str]:
+    """`path` and every file that it includes by a quoted name, directly or not."""
+    seen = set() if seen is None else seen
+    path = os.path.realpath(path)
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#include\s+"([^"]+)"', f.read(), re.M):
+                _includes(os.path.join(os.path.dirname(path), name), seen)
+    return seen
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> str:
-    if force or _newer(LIB, _deps()):
-        cmd = ["nvcc", *NVCC_FLAGS, *(os.path.join(CSRC, s) for s in ENGINE_SOURCES), "-o", LIB]
-        if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        subprocess.check_call(cmd)
+    """Compiles the sources that are newer than their objects, side by side, and links them."""
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objects, running = [], []
+    flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas=-v"] if verbose else [])
+    for name in ENGINE_SOURCES:
+        src, obj = os.path.join(CSRC, name), os.path.join(OBJ_DIR, name + ".o")
+        objects.append(obj)
+        if force or _newer(obj, [*_includes(src), os.path.abspath(__file__)]):
+            cmd = ["nvcc", *flags, "-c", src, "-o", obj + ".part"]
+            running.append((cmd, obj, subprocess.Popen(cmd)))
+    for cmd, obj, p in running:
+        if p.wait() != 0:
+            for _, _, other in running:
+                other.wait()
+            raise subprocess.CalledProcessError(p.returncode, cmd)
+        os.replace(obj + ".part", obj)
+    if force or _newer(LIB, objects):
+        subprocess.check_call(["nvcc", *NVCC_FLAGS, *objects, "-o", LIB])
     return LIB
 
 

@@ -1,0 +1,414 @@
+// Rules on logits (repetition, frequency and presence penalties, biases,
+// grammar masks), the greedy choice and its log-probability, in one pass.
+//
+// Every logit is read once, and written once where the adjusted row is wanted:
+// HBM bounds a batch, the launch and the merge a single row. A row is cut over
+// the CTAs of a cluster, which merge their (maximum, sum of exponentials,
+// index) through shared memory, so one launch needs no scratch and no atomics
+// on global memory, and the merge order is fixed.
+//
+// The penalties and biases touch few tokens of a row. Each CTA marks those of
+// its tile in a bitmap (one bit a token), whose running popcount gives each
+// marked token a compact slot with its count and bias. The streaming pass
+// leaves marked tokens out; a second, short pass goes over the slots.
+#include <cooperative_groups.h>
+
+#include "serving.cuh"
+#include "sync.cuh"
+
+namespace mgb {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kUnroll = 4;            // 16-byte loads of a thread in flight
+constexpr uint32_t kMaxTile = 32768;  // tokens of one bitmap
+constexpr int kSlotBytes = 96 * 1024;  // shared memory for slots at most
+constexpr uint32_t kNone = 0xffffffffu;
+
+#define kPosInf __int_as_float(0x7f800000)
+#define kLowest __int_as_float(0xff800000)
+constexpr float kLog2e = 1.44269504088896341f;
+
+struct ChooseArgs {
+    const void *x;
+    long long stride;
+    uint32_t vocab, tile, cap;  // cap: slots of a tile
+    mgb_logit_rules rules;
+    int32_t *ids;
+    float *logp;
+    void *y;
+    long long y_stride;
+};
+
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Running maximum, sum of exp(y - maximum) and the maximum's lowest index.
+struct Best {
+    float m, l;
+    uint32_t i;
+};
+
+__device__ __forceinline__ float weight_of(float m, float top) {
+    return m == top ? 1.0f : m == kLowest ? 0.0f : exp2_of((m - top) * kLog2e);
+}
+
+__device__ __forceinline__ Best merge(const Best &a, const Best &b) {
+    Best r;
+    r.m = fmaxf(a.m, b.m);
+    r.i = a.m > b.m ? a.i : b.m > a.m ? b.i : min(a.i, b.i);
+    r.l = a.l * weight_of(a.m, r.m) + b.l * weight_of(b.m, r.m);
+    return r;
+}
+
+__device__ __forceinline__ Best shfl_xor(const Best &a, int o) {
+    return Best{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o),
+                __shfl_xor_sync(0xffffffffu, a.i, o)};
+}
+
+// N logits y at indices i0.. (-inf where they do not count) into b.
+template <int N>
+__device__ __forceinline__ void add(Best &b, const float (&y)[N], const uint32_t (&at)[N]) {
+    float top = y[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, y[e]);
+    if (top > b.m) {
+        b.l *= b.m == kLowest ? 0.0f : exp2_of((b.m - top) * kLog2e);
+        b.m = top;
+        b.i = kNone;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (y[e] == top) b.i = min(b.i, at[e]);
+    }
+    if (b.m == kPosInf) {  // exp(inf - inf) counts as one
+#pragma unroll
+        for (int e = 0; e < N; ++e) b.l += y[e] == kPosInf ? 1.0f : 0.0f;
+    } else if (b.m > kLowest) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += exp2_of((y[e] - b.m) * kLog2e);
+        b.l += s;
+    }
+}
+
+template <int TYPE>
+struct Num;  // logits of one type: 16-byte vectors of W numbers
+template <>
+struct Num<MGB_F32> {
+    using T = float;
+    static __device__ __forceinline__ float get(float x) { return x; }
+    static __device__ __forceinline__ float put(float x) { return x; }
+};
+template <>
+struct Num<MGB_F16> {
+    using T = uint16_t;
+    static __device__ __forceinline__ float get(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+    static __device__ __forceinline__ uint16_t put(float x) { return to_16(x, MGB_F16); }
+};
+template <>
+struct Num<MGB_BF16> {
+    using T = uint16_t;
+    static __device__ __forceinline__ float get(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+    static __device__ __forceinline__ uint16_t put(float x) { return to_16(x, MGB_BF16); }
+};
+
+// Bits off .. off + 31 of a bit row of `words` words.
+__device__ __forceinline__ uint32_t bits_at(const uint32_t *row, uint32_t words, uint32_t off) {
+    const uint32_t w = off >> 5;
+    const uint32_t lo = row[w], hi = w + 1 < words ? row[w + 1] : 0;
+    return __funnelshift_r(lo, hi, off & 31);
+}
+
+template <int TYPE, bool SLOTS>
+__global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
+    using N = Num<TYPE>;
+    using T = typename N::T;
+    constexpr int W = 16 / sizeof(T);
+    extern __shared__ uint32_t smem[];
+    __shared__ Best warp_best[kWarps];
+    __shared__ Best cta_best[16];
+    __shared__ uint32_t warp_sum[kWarps];
+    const uint32_t parts = gridDim.x, part = blockIdx.x, row = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+    const mgb_logit_rules &r = a.rules;
+    const T *x = reinterpret_cast<const T *>(a.x) + (size_t)row * a.stride;
+    T *y = a.y ? reinterpret_cast<T *>(a.y) + (size_t)row * a.y_stride : nullptr;
+    const uint32_t *allow = nullptr;
+    if (r.allow) {
+        const int g = r.allow_row ? r.allow_row[row] : 0;
+        if (g >= 0 && (uint32_t)g < r.allow_rows) allow = r.allow + (size_t)g * r.allow_stride;
+    }
+    // the row's share of this CTA, in whole 64s
+    const uint32_t share = ((a.vocab + parts - 1) / parts + 63) & ~63u;
+    const uint32_t c0 = min(a.vocab, part * share), c1 = min(a.vocab, c0 + share);
+
+    const uint32_t words = a.tile / 32;
+    uint32_t *mark = smem, *rank = mark + words, *count = rank + words, *token = count + a.cap;
+    float *bias = reinterpret_cast<float *>(token + a.cap);
+    uint32_t nh = 0;
+    const int32_t *hist = nullptr, *bias_ids = nullptr;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if constexpr (SLOTS) {
+        if (r.history) {
+            hist = r.history + (size_t)row * r.history_stride;
+            nh = r.history_len ? (uint32_t)min((long long)r.history_stride, (long long)max(0, r.history_len[row]))
+                               : r.history_stride;
+        }
+        if (r.bias_count) bias_ids = r.bias_ids + (size_t)row * r.bias_count;
+        if (r.repetition) rep = r.repetition[row];
+        if (r.frequency) freq = r.frequency[row];
+        if (r.presence) pres = r.presence[row];
+    }
+
+    Best best{kLowest, 0.0f, kNone};
+    for (uint32_t v0 = c0; v0 < c1; v0 += a.tile) {
+        const uint32_t v1 = min(c1, v0 + a.tile), width = v1 - v0;
+        uint32_t slots = 0;
+        if constexpr (SLOTS) {
+            for (uint32_t w = tid; w < words; w += kThreads) mark[w] = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < nh; i += kThreads) {
+                const uint32_t off = (uint32_t)hist[i] - v0;
+                if (off < width) atomicOr(&mark[off >> 5], 1u << (off & 31));
+            }
+            for (uint32_t i = tid; i < r.bias_count; i += kThreads) {
+                const uint32_t off = (uint32_t)bias_ids[i] - v0;
+                if (off < width) atomicOr(&mark[off >> 5], 1u << (off & 31));
+            }
+            __syncthreads();
+            // rank[w]: marked tokens before word w; a thread has two words
+            const uint32_t p0 = 2 * tid < words ? __popc(mark[2 * tid]) : 0;
+            const uint32_t p1 = 2 * tid + 1 < words ? __popc(mark[2 * tid + 1]) : 0;
+            uint32_t upto = p0 + p1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += u;
+            }
+            if (lane == 31) warp_sum[warp] = upto;
+            __syncthreads();
+            uint32_t before = 0;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                before += k < warp ? warp_sum[k] : 0;
+                slots += warp_sum[k];
+            }
+            before += upto - p0 - p1;
+            if (2 * tid < words) rank[2 * tid] = before;
+            if (2 * tid + 1 < words) rank[2 * tid + 1] = before + p0;
+            for (uint32_t k = tid; k < slots; k += kThreads) {
+                count[k] = 0;
+                bias[k] = 0.0f;
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < nh; i += kThreads) {
+                const uint32_t off = (uint32_t)hist[i] - v0;
+                if (off >= width) continue;
+                const uint32_t k = rank[off >> 5] + __popc(mark[off >> 5] & ((1u << (off & 31)) - 1));
+                atomicAdd(&count[k], 1u);
+                token[k] = off;
+            }
+            for (uint32_t i = tid; i < r.bias_count; i += kThreads) {
+                const int32_t id = bias_ids[i];
+                const uint32_t off = (uint32_t)id - v0;
+                if (off >= width) continue;
+                // the first entry of a token adds up all of them, in their order
+                float sum = 0.0f;
+                bool first = true;
+                for (uint32_t j = 0; j < r.bias_count && first; ++j) {
+                    if (bias_ids[j] != id) continue;
+                    first = j >= i;
+                    sum += r.bias[(size_t)row * r.bias_count + j];
+                }
+                if (!first) continue;
+                const uint32_t k = rank[off >> 5] + __popc(mark[off >> 5] & ((1u << (off & 31)) - 1));
+                bias[k] = sum;
+                token[k] = off;
+            }
+            __syncthreads();
+        }
+
+        // streaming pass: vectors from the 16-byte boundary at or before v0
+        const uint32_t shift = (uint32_t)(((uintptr_t)(x + v0) & 15) / sizeof(T));
+        const bool y_vec = y && (((uintptr_t)(y + v0) & 15) / sizeof(T)) == shift;
+        const uint32_t nvec = (width + shift + W - 1) / W;
+        for (uint32_t j0 = tid; j0 < nvec; j0 += kThreads * kUnroll) {
+            uint4 raw[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const uint32_t j = j0 + u * kThreads;
+                const bool whole = j * W >= shift && j * W + W <= width + shift;
+                if (whole) raw[u] = __ldcs(reinterpret_cast<const uint4 *>(x + v0 - shift) + j);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const uint32_t j = j0 + u * kThreads;
+                if (j >= nvec) break;
+                const uint32_t at = j * W - shift;  // of the tile; wraps in the first vector
+                const bool whole = j * W >= shift && j * W + W <= width + shift;
+                float f[W];
+                uint32_t idx[W];
+                uint32_t off_bits = 0, skip = 0;
+                if (whole) {
+                    const T *h = reinterpret_cast<const T *>(&raw[u]);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) f[e] = N::get(h[e]);
+                    if (allow) off_bits = ~bits_at(allow, r.allow_stride, v0 + at);
+                    if constexpr (SLOTS) skip = bits_at(mark, words, at);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const uint32_t o = at + e;
+                        f[e] = 0.0f;
+                        if (o >= width) {
+                            skip |= 1u << e;
+                            continue;
+                        }
+                        f[e] = N::get(x[v0 + o]);
+                        if (allow && !((allow[(v0 + o) >> 5] >> ((v0 + o) & 31)) & 1)) off_bits |= 1u << e;
+                        if constexpr (SLOTS) skip |= ((mark[o >> 5] >> (o & 31)) & 1) << e;
+                    }
+                }
+                if (y) {  // marked tokens keep their logit until the second pass
+                    T out[W];
+#pragma unroll
+                    for (int e = 0; e < W; ++e) out[e] = N::put(((off_bits & ~skip) >> e) & 1 ? kLowest : f[e]);
+                    if (whole && y_vec) {
+                        *(reinterpret_cast<uint4 *>(y + v0 - shift) + j) = *reinterpret_cast<const uint4 *>(out);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < W; ++e)
+                            if (at + e < width) y[v0 + at + e] = out[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    if (((off_bits | skip) >> e) & 1 || !(f[e] == f[e])) f[e] = kLowest;
+                    idx[e] = v0 + at + e;
+                }
+                add<W>(best, f, idx);
+            }
+        }
+        if constexpr (SLOTS) {
+            __syncthreads();
+            for (uint32_t k = tid; k < slots; k += kThreads) {
+                const uint32_t id = v0 + token[k], c = count[k];
+                float f = N::get(x[id]);
+                if (c) {
+                    f = f > 0.0f ? __fdiv_rn(f, rep) : f * rep;
+                    f = f - (freq * (float)c + pres);
+                }
+                if (bias_ids) f = f + bias[k];
+                if (allow && !((allow[id >> 5] >> (id & 31)) & 1)) f = kLowest;
+                if (y) y[id] = N::put(f);
+                const float one[1] = {f == f ? f : kLowest};
+                const uint32_t at[1] = {id};
+                Best b{kLowest, 0.0f, kNone};
+                add<1>(b, one, at);
+                best = merge(best, b);
+            }
+            __syncthreads();
+        }
+    }
+
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+    if (lane == 0) warp_best[warp] = best;
+    __syncthreads();
+    if (warp == 0) {
+        best = lane < kWarps ? warp_best[lane] : Best{kLowest, 0.0f, kNone};
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+    }
+    if (parts > 1) {
+        namespace cg = cooperative_groups;
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the cluster runs
+        if (tid == 0) *cg::this_cluster().map_shared_rank(&cta_best[part], 0) = best;
+        cluster_sync();
+        if (part != 0) return;
+        if (warp == 0) {
+            best = lane < parts ? cta_best[lane] : Best{kLowest, 0.0f, kNone};
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+        }
+    }
+    if (tid == 0) {
+        const bool found = best.i != kNone;
+        if (a.ids) a.ids[row] = found ? (int32_t)best.i : -1;
+        if (a.logp) a.logp[row] = found ? -logf(best.l) : kLowest;
+    }
+}
+
+template <int TYPE, bool SLOTS>
+cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem, cudaStream_t s) {
+    static std::atomic<bool> done[kMaxDevices];
+    cudaError_t e = op_allow(choose_kernel<TYPE, SLOTS>, kSlotBytes + (int)(kMaxTile / 4), true, done);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(parts, rows);
+    c.blockDim = dim3(kThreads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, SLOTS>, a);
+}
+
+}  // namespace
+}  // namespace mgb
+
+extern "C" MGB_API mgb_status mgb_logits_choose(const void *logits, int type, int64_t row_stride, uint32_t rows,
+                                                uint32_t vocab, const mgb_logit_rules *rules, int32_t *ids, float *logp,
+                                                void *adjusted, int64_t adjusted_stride, void *stream) {
+    using namespace mgb;
+    static const char *op = "mgb_logits_choose";
+    if (type < MGB_F32 || type > MGB_BF16) return op_fail(MGB_ERR_INVALID, op, "unknown number type");
+    if (rows == 0) return MGB_OK;
+    if (!logits) return op_fail(MGB_ERR_INVALID, op, "null logits");
+    if (vocab == 0 || vocab > 0x7fffffffu) return op_fail(MGB_ERR_INVALID, op, "vocab out of range");
+    if (rows > 65535) return op_fail(MGB_ERR_INVALID, op, "more than 65535 rows");
+    const uintptr_t unit = type_size(type) - 1;
+    if (((uintptr_t)logits | (uintptr_t)adjusted) & unit)
+        return op_fail(MGB_ERR_INVALID, op, "logits are not aligned to their type");
+    if (row_stride < 0 || (rows > 1 && row_stride < (int64_t)vocab) ||
+        (adjusted && rows > 1 && adjusted_stride < (int64_t)vocab))
+        return op_fail(MGB_ERR_INVALID, op, "rows overlap");
+    ChooseArgs a{logits, row_stride, vocab, 0, 0, {}, ids, logp, adjusted, adjusted_stride};
+    if (rules) a.rules = *rules;
+    mgb_logit_rules &r = a.rules;
+    if (r.bias_count && (!r.bias_ids || !r.bias)) return op_fail(MGB_ERR_INVALID, op, "null bias");
+    if (r.allow && (uint64_t)r.allow_stride * 32 < vocab) return op_fail(MGB_ERR_INVALID, op, "grammar rows are too short");
+    if (!r.repetition && !r.frequency && !r.presence) r.history = nullptr;
+    if (!r.history) r.history_stride = 0;
+    const bool slots = r.history_stride || r.bias_count;
+
+    // A row is cut over 16 CTAs (the largest cluster) while that many do not
+    // yet fill the GPU's 148 SMs twice, over fewer for more rows, and never
+    // into shares below 2048 tokens.
+    uint32_t parts = 16;
+    while (parts > 1 && (rows * parts > 4 * 148 || (uint64_t)parts * 2048 > vocab + 2047ull)) parts /= 2;
+    const uint32_t share = ((vocab + parts - 1) / parts + 63) & ~63u;
+    a.tile = share < kMaxTile ? share : kMaxTile;
+    const uint64_t entries = (uint64_t)r.history_stride + r.bias_count;
+    auto cap = [&] { return (uint32_t)(entries < a.tile ? entries : a.tile); };
+    while ((uint64_t)cap() * 12 > (uint64_t)kSlotBytes) a.tile = (a.tile / 2 + 63) & ~63u;
+    a.cap = cap();
+    const int smem = slots ? (int)(a.tile / 32 * 8 + a.cap * 12) : 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    switch (type) {
+        case MGB_F32: e = slots ? launch<MGB_F32, true>(a, rows, parts, smem, s) : launch<MGB_F32, false>(a, rows, parts, smem, s); break;
+        case MGB_F16: e = slots ? launch<MGB_F16, true>(a, rows, parts, smem, s) : launch<MGB_F16, false>(a, rows, parts, smem, s); break;
+        default: e = slots ? launch<MGB_BF16, true>(a, rows, parts, smem, s) : launch<MGB_BF16, false>(a, rows, parts, smem, s); break;
+    }
+    return op_launch_status(e, op);
+}
