@@ -46,7 +46,9 @@ __device__ __forceinline__ float exp2_of(float x) {
     return y;
 }
 
-// Running maximum, sum of exp(y - maximum) and the maximum's lowest index.
+// Running maximum m, its lowest index i, and the sum l of exp(y - m) over all
+// logits but that one, whose own term is 1: the log-probability -log1p(l) keeps
+// its relative precision where one token has nearly all of the weight.
 struct Best {
     float m, l;
     uint32_t i;
@@ -57,11 +59,11 @@ __device__ __forceinline__ float weight_of(float m, float top) {
 }
 
 __device__ __forceinline__ Best merge(const Best &a, const Best &b) {
-    Best r;
-    r.m = fmaxf(a.m, b.m);
-    r.i = a.m > b.m ? a.i : b.m > a.m ? b.i : min(a.i, b.i);
-    r.l = a.l * weight_of(a.m, r.m) + b.l * weight_of(b.m, r.m);
-    return r;
+    const bool first = a.m > b.m || (a.m == b.m && a.i <= b.i);
+    const float m = first ? a.m : b.m, w = weight_of(first ? b.m : a.m, m);
+    // the loser's own term joins the sum, unless it has none
+    const float own = (first ? b.i : a.i) == kNone ? 0.0f : 1.0f;
+    return Best{m, first ? a.l + (own + b.l) * w : b.l + (own + a.l) * w, first ? a.i : b.i};
 }
 
 __device__ __forceinline__ Best shfl_xor(const Best &a, int o) {
@@ -76,14 +78,16 @@ __device__ __forceinline__ void add(Best &b, const float (&y)[N], const uint32_t
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, y[e]);
     if (top > b.m) {
-        b.l *= b.m == kLowest ? 0.0f : exp2_of((b.m - top) * kLog2e);
+        b.l = b.m == kLowest ? 0.0f : (1.0f + b.l) * exp2_of((b.m - top) * kLog2e);
         b.m = top;
         b.i = kNone;
 #pragma unroll
+        for (int e = N - 1; e >= 0; --e)
+            if (y[e] == top) b.i = at[e];
+#pragma unroll
         for (int e = 0; e < N; ++e)
-            if (y[e] == top) b.i = min(b.i, at[e]);
-    }
-    if (b.m == kPosInf) {  // exp(inf - inf) counts as one
+            if (at[e] != b.i) b.l += weight_of(y[e], top);
+    } else if (b.m == kPosInf) {  // exp(inf - inf) counts as one
 #pragma unroll
         for (int e = 0; e < N; ++e) b.l += y[e] == kPosInf ? 1.0f : 0.0f;
     } else if (b.m > kLowest) {
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
     if (tid == 0) {
         const bool found = best.i != kNone;
         if (a.ids) a.ids[row] = found ? (int32_t)best.i : -1;
-        if (a.logp) a.logp[row] = found ? -logf(best.l) : kLowest;
+        if (a.logp) a.logp[row] = found ? -log1pf(best.l) : kLowest;
     }
 }
 
