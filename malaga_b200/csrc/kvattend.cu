@@ -11,7 +11,7 @@
 // Roundings to fewer than 32 bits, besides the output's:
 //  * p d_v goes into its product as f16: 2^-11 relative, the size of one
 //    rounding of a 16-bit output, and averaged over the keys. It is formed as
-//    2^14 p (d_v 2^-E), E a running exponent of the largest d_v, so that f16's
+//    2^7 p (d_v 2^-E), E a running exponent of the largest d_v, so that f16's
 //    narrow range costs nothing.
 //  * q goes in as f16: exact for f16 q; bf16 q is first scaled by a power of
 //    two per row, and then exact but for numbers 2^-38 of the row's largest.
@@ -27,7 +27,6 @@ namespace {
 
 #define kLowest __int_as_float(0xff800000)
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kRaise = 14.0f;  // p is held as 2^14 p
 
 struct AttendArgs {
     KvView kv;
@@ -89,16 +88,23 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: 16 rows (token, head of the group) of one cache head a CTA.
+// Few rows: tiles of 8 or 16 rows (token, head of the group) of one cache head.
 //
-// K and V go from global memory straight into the registers in which
-// mma.m16n8k16 wants them, with 16-byte loads: the order of the head dimension
-// inside q . k is free (Q is permuted the same way), and so is the order of the
-// output's columns. For K, four lanes share a key and take every fourth vector
-// of its row; for V, eight lanes share a key, and a byte permute pairs two keys.
-// A warp takes blocks of BLOCK keys in turn and keeps its own maximum, sum and
-// output; warps join in shared memory, the CTAs of a cluster (which cut the
-// keys among them) through distributed shared memory, in a fixed order.
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
+// the rows are the 8-wide side of mma.m16n8k16 and a single query wastes as
+// little as it can. K and V go from global memory straight into the registers
+// in which the mma wants them as its A operand, with 16-byte loads: the order
+// of the head dimension inside q . k is free (Q is permuted the same way), and
+// so is the order of the rows of O^T. For K, four lanes share a key and take
+// every fourth vector of its row; for V, eight lanes share a key, and a byte
+// permute pairs two keys. movmatrix turns P^T, as it leaves the first product,
+// into the B operand of the second.
+//
+// A warp takes blocks of 16 keys in turn and keeps its own maximum, sum and
+// output. The maximum only has to be near: it is raised when a score passes it
+// by 2^8, so most blocks need one vote and no reduction across lanes. Warps
+// join in shared memory, the CTAs of a cluster (which cut the keys among them)
+// through distributed shared memory, in a fixed order.
 
 template <int D, bool Q8>
 struct Frag {
@@ -108,7 +114,7 @@ struct Frag {
     static constexpr int VB = D * ESZ / 8 < 16 ? D * ESZ / 8 : 16;
     static constexpr int VN = D * ESZ / 8 / VB;
     static constexpr int KW = D * ESZ / 16, VW = D * ESZ / 32 ? D * ESZ / 32 : 1;  // words of a key and lane
-    static constexpr int STEPS = D / 16, TILES = D / 8;
+    static constexpr int STEPS = D / 16;
     // dim of element e of lane t's part of a K row, of lane g's part of a V row
     static __device__ __forceinline__ int k_dim(int t, int e) {
         constexpr int VE = KB / ESZ;
@@ -120,63 +126,227 @@ struct Frag {
     }
 };
 
-template <int D, bool Q8>
-struct Block {  // 16 keys of a warp in registers
-    uint32_t k[2][Frag<D, Q8>::KW];
-    uint32_t v[4][Frag<D, Q8>::VW];
-    float ks[4], vs[4];  // scales of keys 2t, 2t+1, 2t+8, 2t+9
-    bool hole;           // the table names no page of the cache
+constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
+constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
+constexpr float kRaise = 7.0f;  // p is held as 2^7 p, up to 2^15
+
+// Where a block of 16 keys lies. left: how many of its keys exist (0 where the
+// table names no page of the cache); the others are read as zeros.
+struct Place {
+    size_t row;
+    int left;
+    bool hole;
 };
 
-constexpr int kRowWarps = 8;
+__device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t head, uint32_t page, int key0, int end) {
+    Place p;
+    p.hole = page >= a.kv.pages;
+    p.row = a.kv.row(p.hole ? 0 : page, head, (uint32_t)key0 & ((1u << a.kv.page_log2) - 1));
+    p.left = p.hole ? 0 : end - key0;
+    return p;
+}
 
 template <int D, bool Q8>
-__device__ __forceinline__ void load_block(const AttendArgs &a, uint32_t head, uint32_t page, int key0, int end, int g,
-                                           int t, Block<D, Q8> &blk) {
-    using F = Frag<D, Q8>;
-    const bool mapped = page < a.kv.pages;
-    const size_t row = a.kv.row(mapped ? page : 0, head, (uint32_t)key0 & ((1u << a.kv.page_log2) - 1));
-    const uint8_t *k = static_cast<const uint8_t *>(a.kv.k) + row * (D * F::ESZ);
-    const uint8_t *v = static_cast<const uint8_t *>(a.kv.v) + row * (D * F::ESZ);
-    const int left = mapped ? end - key0 : 0;  // keys of the block that exist; the others are read as zeros
+struct KBlock {
+    uint32_t w[2][Frag<D, Q8>::KW];  // keys g, g + 8
+    float scale[2];
+    Place at;
+    __device__ __forceinline__ void load(const AttendArgs &a, const Place &p, int g, int t) {
+        using F = Frag<D, Q8>;
+        at = p;
+        const uint8_t *k = static_cast<const uint8_t *>(a.kv.k) + p.row * (D * F::ESZ);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int key = g + 8 * u;
+        for (int u = 0; u < 2; ++u) {
+            const int key = g + 8 * u;
 #pragma unroll
-        for (int w = 0; w < F::KW; ++w) blk.k[u][w] = 0;
-        if (key < left) {
+            for (int i = 0; i < F::KW; ++i) w[u][i] = 0;
+            scale[u] = 0.0f;
+            if (key < p.left) {
 #pragma unroll
-            for (int c = 0; c < F::KN; ++c)
-                load_words<F::KB>(k + (size_t)key * (D * F::ESZ) + (t + 4 * c) * F::KB, &blk.k[u][c * (F::KB / 4)]);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int key = 2 * t + (u & 1) + 8 * (u >> 1);
-#pragma unroll
-        for (int w = 0; w < F::VW; ++w) blk.v[u][w] = 0;
-        blk.ks[u] = blk.vs[u] = 0.0f;
-        if (key < left) {
-#pragma unroll
-            for (int c = 0; c < F::VN; ++c)
-                load_words<F::VB>(v + (size_t)key * (D * F::ESZ) + (g + 8 * c) * F::VB, &blk.v[u][c * (F::VB / 4)]);
-            if constexpr (Q8) {
-                blk.ks[u] = __ldg(a.kv.ks + row + key);
-                blk.vs[u] = __ldg(a.kv.vs + row + key);
+                for (int c = 0; c < F::KN; ++c)
+                    load_words<F::KB>(k + key * (D * F::ESZ) + (t + 4 * c) * F::KB, &w[u][c * (F::KB / 4)]);
+                if constexpr (Q8) scale[u] = __ldg(a.kv.ks + p.row + key);
             }
         }
     }
-    blk.hole = !mapped;
+};
+
+template <int D, bool Q8>
+struct VBlock {
+    uint32_t w[4][Frag<D, Q8>::VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+    float scale[2];                  // of keys g, g + 8
+    __device__ __forceinline__ void load(const AttendArgs &a, const Place &p, int g, int t) {
+        using F = Frag<D, Q8>;
+        const uint8_t *v = static_cast<const uint8_t *>(a.kv.v) + p.row * (D * F::ESZ);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int key = 2 * t + (u & 1) + 8 * (u >> 1);
+#pragma unroll
+            for (int i = 0; i < F::VW; ++i) w[u][i] = 0;
+            if (key < p.left) {
+#pragma unroll
+                for (int c = 0; c < F::VN; ++c)
+                    load_words<F::VB>(v + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &w[u][c * (F::VB / 4)]);
+            }
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) scale[u] = g + 8 * u < p.left ? __ldg(a.kv.vs + p.row + g + 8 * u) : 0.0f;
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
-template <int D, bool Q8, bool SPLIT>
-__global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const AttendArgs a) {
+// Over the eight lanes that share t (the keys of a block).
+__device__ __forceinline__ float max_keys(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+__device__ __forceinline__ float sum_keys(float x) {
+    x += __shfl_xor_sync(0xffffffffu, x, 4);
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+
+// NT: tiles of 8 rows. State of a warp: per row (2t and 2t + 1 of each tile,
+// the same in all lanes of equal t) the near maximum m; l is this lane's share.
+template <int D, bool Q8, bool SPLIT, int NT>
+struct Rows {
     using F = Frag<D, Q8>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    float *so = reinterpret_cast<float *>(smem);                 // [warps][16][D]
-    __half *sq = reinterpret_cast<__half *>(smem);               // [SPLIT + 1][16][D], before so is used
-    __shared__ float row_scale[16], wm[kRowWarps][16], wl[kRowWarps][16];
-    __shared__ float cm[16], cl[16];
+    uint32_t q[SPLIT ? 2 : 1][NT][F::STEPS][2];
+    float scale[NT][2];
+    int limit[NT][2];
+    int all;  // keys below are seen by every row
+    float o[NT][F::STEPS][4];
+    float m[NT][2], l[NT][2];
+    int exp_v;  // V's scales so far are below 2^exp_v
+
+    __device__ __forceinline__ void step(const KBlock<D, Q8> &k, const VBlock<D, Q8> &v, int key0, int g) {
+        float s[NT][4];  // key g: rows 2t, 2t + 1; key g + 8: the same
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < F::STEPS; ++st) {
+            uint32_t x[4];
+            if constexpr (Q8) {
+                const uint32_t lo = k.w[0][st] ^ 0x80808080u, hi = k.w[1][st] ^ 0x80808080u;
+                x[0] = codes2(lo, 0x4140), x[1] = codes2(hi, 0x4140);
+                x[2] = codes2(lo, 0x4342), x[3] = codes2(hi, 0x4342);
+            } else {
+                x[0] = k.w[0][2 * st], x[1] = k.w[1][2 * st];
+                x[2] = k.w[0][2 * st + 1], x[3] = k.w[1][2 * st + 1];
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16(s[n], x, q[0][n][st][0], q[0][n][st][1]);
+                if constexpr (SPLIT) mma16(s[n], x, q[1][n][st][0], q[1][n][st][1]);
+            }
+        }
+        const bool whole = key0 + 16 <= all && !k.at.hole;
+        bool see[NT][4], past = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                see[n][e] = whole || (key0 + g + 8 * (e >> 1) < limit[n][e & 1] && !k.at.hole);
+                s[n][e] = see[n][e] ? s[n][e] * (Q8 ? scale[n][e & 1] * k.scale[e >> 1] : scale[n][e & 1]) : kLowest;
+                past |= s[n][e] > m[n][e & 1] + kSlack;
+            }
+        if constexpr (Q8) {
+            const float d = fmaxf(fabsf(v.scale[0]), fabsf(v.scale[1]));
+            past |= (__float_as_int(d) >> 23) - 126 > exp_v;
+        }
+        if (__any_sync(0xffffffffu, past)) {
+            float f = 1.0f;
+            if constexpr (Q8) {
+                const float d = max_keys(fmaxf(fabsf(v.scale[0]), fabsf(v.scale[1])));
+                const int e = max(exp_v, min(126, (__float_as_int(d) >> 23) - 126));
+                f = power_of_2(exp_v - e);
+                exp_v = e;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float top = fmaxf(m[n][r], max_keys(fmaxf(s[n][r], s[n][2 + r])));
+                    const float w = m[n][r] == kLowest ? 0.0f : exp2_of(m[n][r] - top);
+                    m[n][r] = top;
+                    l[n][r] *= w;
+#pragma unroll
+                    for (int j = 0; j < F::STEPS; ++j) {
+                        o[n][j][r] *= w * f;
+                        o[n][j][2 + r] *= w * f;
+                    }
+                }
+        }
+        uint32_t p[SPLIT ? 2 : 1][NT][2];
+        const float back = Q8 ? __int_as_float((127 - exp_v) << 23) : 1.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            // where nothing was seen yet s is -inf, and any finite maximum gives p = 0
+            const float z[2] = {(m[n][0] == kLowest ? 0.0f : m[n][0]) - kRaise, (m[n][1] == kLowest ? 0.0f : m[n][1]) - kRaise};
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = exp2_of(s[n][e] - z[e & 1]);
+                l[n][e & 1] += w[e];
+                if constexpr (Q8) w[e] = see[n][e] ? w[e] * (v.scale[e >> 1] * back) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t hi = pack(w[2 * u], w[2 * u + 1]);
+                p[0][n][u] = transpose8(hi);
+                if constexpr (SPLIT) {
+                    const float2 h = unpack(hi);
+                    p[1][n][u] = transpose8(pack(w[2 * u] - h.x, w[2 * u + 1] - h.y));
+                }
+            }
+        }
+        auto pair = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            const uint32_t x[4] = {a0, a1, a2, a3};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16(o[n][j], x, p[0][n][0], p[0][n][1]);
+                if constexpr (SPLIT) mma16(o[n][j], x, p[1][n][0], p[1][n][1]);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < F::VW; ++i) {
+            if constexpr (Q8) {
+                const uint32_t x0 = v.w[0][i] ^ 0x80808080u, x1 = v.w[1][i] ^ 0x80808080u;
+                const uint32_t x2 = v.w[2][i] ^ 0x80808080u, x3 = v.w[3][i] ^ 0x80808080u;
+                const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
+                constexpr int PER = F::STEPS < 2 ? 1 : 2;
+                pair(PER * i, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
+                if constexpr (PER == 2) {
+                    const uint32_t hi0 = __byte_perm(x0, x1, 0x7362), hi1 = __byte_perm(x2, x3, 0x7362);
+                    pair(PER * i + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
+                }
+            } else {
+                pair(i, __byte_perm(v.w[0][i], v.w[1][i], 0x5410), __byte_perm(v.w[0][i], v.w[1][i], 0x7632),
+                     __byte_perm(v.w[2][i], v.w[3][i], 0x5410), __byte_perm(v.w[2][i], v.w[3][i], 0x7632));
+            }
+        }
+    }
+};
+
+template <int D, bool Q8, bool SPLIT, int NT>
+__global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs a) {
+    using F = Frag<D, Q8>;
+    constexpr int R = 8 * NT, PER_ROW = kRowThreads / R, E = D / PER_ROW;
+    static_assert(E >= 1, "at most one thread a number");
+    __shared__ __align__(16) float so[kRowWarps][R][D];
+    __shared__ __align__(16) __half sq[SPLIT ? 2 : 1][R][D];
+    __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R];
+    __shared__ int row_limit[R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
@@ -188,12 +358,22 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const Atten
     // keys that token i sees
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 
-    for (long long r0 = (long long)(blockIdx.y / heads) * 16; r0 < rows; r0 += (long long)(gridDim.y / heads) * 16) {
-        // Q: 16 threads a row; the row's largest number to just below 2^14 (f16 q stays as it is)
+    for (long long r0 = (long long)(blockIdx.y / heads) * R; r0 < rows; r0 += (long long)(gridDim.y / heads) * R) {
+        const int end = limit((int)((min(r0 + R, rows) - 1) / a.group));  // no row of the tile sees further
+        const int blocks = (end + 15) / 16;
+        const int first = (int)((long long)blocks * part / parts), stop = (int)((long long)blocks * (part + 1) / parts);
+        // the first keys are on their way while the queries are prepared
+        auto page_of = [&](int blk) { return blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u; };
+        int blk = first + warp;
+        KBlock<D, Q8> k0, k1;
+        VBlock<D, Q8> v;
+        uint32_t page = page_of(blk), next = page_of(blk + kRowWarps);
+        if (blk < stop) k0.load(a, place_of(a, head, page, blk * 16, end), g, t);
+
+        // Q: the row's largest number to just below 2^14 (f16 q stays as it is)
         {
-            const int r = tid >> 4, c = tid & 15;
+            const int r = tid / PER_ROW, c = tid % PER_ROW;
             const long long rr = r0 + r;
-            constexpr int E = D / 16;
             float x[E], m = 0.0f;
             const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
 #pragma unroll
@@ -204,7 +384,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const Atten
                 m = fmaxf(m, fabsf(x[e]));
             }
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             int shift = 0;
             if (a.q_type != MGB_F16 && m > 0.0f && m < __int_as_float(0x7f800000)) shift = 13 - ilogbf(m);
             // 2^shift in two factors, since either may leave the range of f32 alone
@@ -214,210 +394,84 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const Atten
             for (int e = 0; e < E; ++e) {
                 const float y = x[e] * f1 * f2;
                 const __half hi = __float2half_rn(y);
-                sq[r * D + c * E + e] = hi;
-                if constexpr (SPLIT) sq[16 * D + r * D + c * E + e] = __float2half_rn(y - __half2float(hi));
+                sq[0][r][c * E + e] = hi;
+                if constexpr (SPLIT) sq[1][r][c * E + e] = __float2half_rn(y - __half2float(hi));
             }
-            if (c == 0) row_scale[r] = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+            if (c == 0) {
+                row_scale[r] = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+                row_limit[r] = rr < rows ? limit(i) : 0;
+            }
         }
         __syncthreads();
-        uint32_t q[SPLIT ? 2 : 1][F::STEPS][4];
+        Rows<D, Q8, SPLIT, NT> st;
+        st.exp_v = -126;
+        st.all = limit((int)(r0 / a.group));
+        if (r0 + R > rows) st.all = 0;
 #pragma unroll
-        for (int z = 0; z < (SPLIT ? 2 : 1); ++z)
+        for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int s = 0; s < F::STEPS; ++s) {
-                const int d0 = F::k_dim(t, 4 * s);
-                const uint2 lo = *reinterpret_cast<const uint2 *>(sq + (z * 16 + g) * D + d0);
-                const uint2 hi = *reinterpret_cast<const uint2 *>(sq + (z * 16 + g + 8) * D + d0);
-                q[z][s][0] = lo.x, q[z][s][1] = hi.x, q[z][s][2] = lo.y, q[z][s][3] = hi.y;
+            for (int z = 0; z < (SPLIT ? 2 : 1); ++z)
+#pragma unroll
+                for (int s = 0; s < F::STEPS; ++s) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(&sq[z][8 * j + g][F::k_dim(t, 4 * s)]);
+                    st.q[z][j][s][0] = x.x, st.q[z][j][s][1] = x.y;
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                st.scale[j][r] = row_scale[8 * j + 2 * t + r];
+                st.limit[j][r] = row_limit[8 * j + 2 * t + r];
+                st.m[j][r] = kLowest;
+                st.l[j][r] = 0.0f;
             }
-        const float scale0 = row_scale[g], scale1 = row_scale[g + 8];
-        const int lim0 = r0 + g < rows ? limit((int)((r0 + g) / a.group)) : 0;
-        const int lim1 = r0 + g + 8 < rows ? limit((int)((r0 + g + 8) / a.group)) : 0;
-        const long long last = r0 + 15 < rows ? r0 + 15 : rows - 1;
-        const int end = limit((int)(last / a.group));  // no row of the tile sees further
-        const int blocks = (end + 15) / 16;
-        const int first = (int)((long long)blocks * part / parts), stop = (int)((long long)blocks * (part + 1) / parts);
+#pragma unroll
+            for (int s = 0; s < F::STEPS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[j][s][e] = 0.0f;
+        }
 
-        float o[F::TILES][4];
-#pragma unroll
-        for (int j = 0; j < F::TILES; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-        float m0 = kLowest, m1 = kLowest, l0 = 0.0f, l1 = 0.0f;
-        int exp_v = -126;  // of the largest V scale so far
-
-        auto page_of = [&](int blk) { return blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u; };
-        auto step = [&](const Block<D, Q8> &x, int key0) {
-            float s[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
-#pragma unroll
-                for (int st = 0; st < F::STEPS; ++st) {
-                    uint32_t b0, b1;
-                    if constexpr (Q8) {
-                        const uint32_t w = x.k[u][st] ^ 0x80808080u;
-                        b0 = codes2(w, 0x4140);
-                        b1 = codes2(w, 0x4342);
-                    } else {
-                        b0 = x.k[u][2 * st];
-                        b1 = x.k[u][2 * st + 1];
-                    }
-                    mma16(s[u], q[0][st], b0, b1);
-                    if constexpr (SPLIT) mma16(s[u], q[1][st], b0, b1);
-                }
-            }
-            float top0 = kLowest, top1 = kLowest;
-            bool see0[4], see1[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int key = key0 + 2 * t + (u & 1) + 8 * (u >> 1);
-                float &a0 = s[u >> 1][u & 1], &a1 = s[u >> 1][2 + (u & 1)];
-                see0[u] = key < lim0 && !x.hole;
-                see1[u] = key < lim1 && !x.hole;
-                a0 = see0[u] ? a0 * (Q8 ? scale0 * x.ks[u] : scale0) : kLowest;
-                a1 = see1[u] ? a1 * (Q8 ? scale1 * x.ks[u] : scale1) : kLowest;
-                top0 = fmaxf(top0, a0);
-                top1 = fmaxf(top1, a1);
-            }
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
-            int exp_new = exp_v;
-            if constexpr (Q8) {
-                float d = fmaxf(fmaxf(fabsf(x.vs[0]), fabsf(x.vs[1])), fmaxf(fabsf(x.vs[2]), fabsf(x.vs[3])));
-                d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 1));
-                d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
-                exp_new = max(exp_v, min(126, (__float_as_int(d) >> 23) - 126));  // d < 2^exp_new
-            }
-            const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
-            if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1 || exp_new > exp_v)) {
-                const float f = Q8 ? power_of_2(exp_v - exp_new) : 1.0f;
-                const float a0 = m0 == kLowest ? 0.0f : exp2_of(m0 - n0), a1 = m1 == kLowest ? 0.0f : exp2_of(m1 - n1);
-                l0 *= a0;
-                l1 *= a1;
-#pragma unroll
-                for (int j = 0; j < F::TILES; ++j) {
-                    o[j][0] *= a0 * f;
-                    o[j][1] *= a0 * f;
-                    o[j][2] *= a1 * f;
-                    o[j][3] *= a1 * f;
-                }
-                m0 = n0;
-                m1 = n1;
-                exp_v = exp_new;
-            }
-            // rows that have seen nothing: s is -inf everywhere, any finite maximum gives p = 0
-            const float z0 = (m0 == kLowest ? 0.0f : m0) - kRaise, z1 = (m1 == kLowest ? 0.0f : m1) - kRaise;
-            float w0[4], w1[4];
-            const float back = Q8 ? __int_as_float((127 - exp_v) << 23) : 1.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                w0[u] = exp2_of(s[u >> 1][u & 1] - z0);
-                w1[u] = exp2_of(s[u >> 1][2 + (u & 1)] - z1);
-                l0 += w0[u];
-                l1 += w1[u];
-                if constexpr (Q8) {
-                    const float d = x.vs[u] * back;
-                    w0[u] = see0[u] ? w0[u] * d : 0.0f;
-                    w1[u] = see1[u] ? w1[u] * d : 0.0f;
-                }
-            }
-            uint32_t p[SPLIT ? 2 : 1][4];
-            p[0][0] = pack(w0[0], w0[1]);
-            p[0][1] = pack(w1[0], w1[1]);
-            p[0][2] = pack(w0[2], w0[3]);
-            p[0][3] = pack(w1[2], w1[3]);
-            if constexpr (SPLIT) {
-                float2 h = unpack(p[0][0]);
-                p[1][0] = pack(w0[0] - h.x, w0[1] - h.y);
-                h = unpack(p[0][1]);
-                p[1][1] = pack(w1[0] - h.x, w1[1] - h.y);
-                h = unpack(p[0][2]);
-                p[1][2] = pack(w0[2] - h.x, w0[3] - h.y);
-                h = unpack(p[0][3]);
-                p[1][3] = pack(w1[2] - h.x, w1[3] - h.y);
-            }
-            auto tile = [&](int j, uint32_t b0, uint32_t b1) {
-                mma16(o[j], p[0], b0, b1);
-                if constexpr (SPLIT) mma16(o[j], p[1], b0, b1);
-            };
-            if constexpr (Q8) {
-                constexpr int PER = F::TILES < 4 ? F::TILES : 4;
-#pragma unroll
-                for (int w = 0; w < F::VW; ++w) {
-                    const uint32_t x0 = x.v[0][w] ^ 0x80808080u, x1 = x.v[1][w] ^ 0x80808080u;
-                    const uint32_t x2 = x.v[2][w] ^ 0x80808080u, x3 = x.v[3][w] ^ 0x80808080u;
-                    const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), hi0 = __byte_perm(x0, x1, 0x7362);
-                    const uint32_t lo1 = __byte_perm(x2, x3, 0x5140), hi1 = __byte_perm(x2, x3, 0x7362);
-                    tile(PER * w, codes2(lo0, 0x4140), codes2(lo1, 0x4140));
-                    tile(PER * w + 1, codes2(lo0, 0x4342), codes2(lo1, 0x4342));
-                    if constexpr (PER == 4) {
-                        tile(PER * w + 2, codes2(hi0, 0x4140), codes2(hi1, 0x4140));
-                        tile(PER * w + 3, codes2(hi0, 0x4342), codes2(hi1, 0x4342));
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int w = 0; w < F::VW; ++w) {
-                    tile(2 * w, __byte_perm(x.v[0][w], x.v[1][w], 0x5410), __byte_perm(x.v[2][w], x.v[3][w], 0x5410));
-                    tile(2 * w + 1, __byte_perm(x.v[0][w], x.v[1][w], 0x7632), __byte_perm(x.v[2][w], x.v[3][w], 0x7632));
-                }
-            }
-        };
-
-        // one block is computed while the next is on its way, and the page after that is looked up
-        {
-            int blk = first + warp;
-            Block<D, Q8> x0, x1;
-            uint32_t page = page_of(blk);
-            if (blk < stop) load_block<D, Q8>(a, head, page, blk * 16, end, g, t, x0);
-            page = page_of(blk + kRowWarps);
-            while (blk < stop) {
-                const int n1b = blk + kRowWarps, n2b = n1b + kRowWarps;
-                if (n1b < stop) load_block<D, Q8>(a, head, page, n1b * 16, end, g, t, x1);
-                page = page_of(n2b);
-                step(x0, blk * 16);
-                if (n1b >= stop) break;
-                if (n2b < stop) load_block<D, Q8>(a, head, page, n2b * 16, end, g, t, x0);
-                page = page_of(n2b + kRowWarps);
-                step(x1, n1b * 16);
-                blk = n2b;
-            }
+        // V of a block and K of the next are on their way while the block's scores are formed
+        while (blk < stop) {
+            const int b1 = blk + kRowWarps, b2 = b1 + kRowWarps;
+            v.load(a, k0.at, g, t);
+            if (b1 < stop) k1.load(a, place_of(a, head, next, b1 * 16, end), g, t);
+            next = page_of(b2);
+            st.step(k0, v, blk * 16, g);
+            if (b1 >= stop) break;
+            v.load(a, k1.at, g, t);
+            if (b2 < stop) k0.load(a, place_of(a, head, next, b2 * 16, end), g, t);
+            next = page_of(b2 + kRowWarps);
+            st.step(k1, v, b1 * 16, g);
+            blk = b2;
         }
 
         // the CTA's warps
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (t == 0) {
-            wm[warp][g] = m0, wm[warp][g + 8] = m1;
-            wl[warp][g] = l0, wl[warp][g + 8] = l1;
-        }
-        __syncthreads();
-        {
-            float top0 = kLowest, top1 = kLowest;
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) {
-                top0 = fmaxf(top0, wm[w][g]);
-                top1 = fmaxf(top1, wm[w][g + 8]);
-            }
-            const float f = Q8 ? power_of_2(exp_v) : 1.0f;
-            const float a0 = m0 == kLowest ? 0.0f : exp2_of(m0 - top0) * f, a1 = m1 == kLowest ? 0.0f : exp2_of(m1 - top1) * f;
-            float *mine = so + warp * 16 * D;
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < F::TILES; ++j)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int d = F::v_dim(2 * t + c, j);
-                    mine[g * D + d] = o[j][c] * a0;
-                    mine[(g + 8) * D + d] = o[j][2 + c] * a1;
+            for (int r = 0; r < 2; ++r) {
+                const float l = sum_keys(st.l[j][r]);
+                if (g == 0) {
+                    wm[warp][8 * j + 2 * t + r] = st.m[j][r];
+                    wl[warp][8 * j + 2 * t + r] = l;
                 }
-        }
-        if (tid < 16) {
+            }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 8 * j + 2 * t + r;
+                float top = wm[0][row];
+#pragma unroll
+                for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, wm[w][row]);
+                const float f = st.m[j][r] == kLowest ? 0.0f : exp2_of(st.m[j][r] - top) * (Q8 ? power_of_2(st.exp_v) : 1.0f);
+#pragma unroll
+                for (int s = 0; s < F::STEPS; ++s) {
+                    so[warp][row][F::v_dim(g, 2 * s)] = st.o[j][s][r] * f;
+                    so[warp][row][F::v_dim(g, 2 * s + 1)] = st.o[j][s][2 + r] * f;
+                }
+            }
+        if (tid < R) {
             float top = kLowest, sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, wm[w][tid]);
@@ -430,24 +484,24 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const Atten
         __syncthreads();
         namespace cg = cooperative_groups;
         auto cluster = cg::this_cluster();
+        const int live = (int)min((long long)R, rows - r0);
         if (parts > 1) {
-            for (int u = tid; u < 16 * D; u += kRowWarps * 32) {
+            for (int u = tid; u < live * D; u += kRowThreads) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kRowWarps; ++w) sum += so[w * 16 * D + u];
-                so[u] = sum;
+                for (int w = 0; w < kRowWarps; ++w) sum += (&so[w][0][0])[u];
+                (&so[0][0][0])[u] = sum;
             }
             cluster_sync();
         }
         // outputs; with several CTAs each takes its share of the tile
-        for (int u = (int)part * (kRowWarps * 32) + tid; u < 16 * D; u += (int)parts * (kRowWarps * 32)) {
+        for (int u = (int)part * kRowThreads + tid; u < live * D; u += (int)parts * kRowThreads) {
             const int r = u / D, d = u % D;
-            const long long rr = r0 + r;
             float sum = 0.0f, l = 0.0f;
             if (parts == 1) {
                 l = cl[r];
 #pragma unroll
-                for (int w = 0; w < kRowWarps; ++w) sum += so[w * 16 * D + u];
+                for (int w = 0; w < kRowWarps; ++w) sum += (&so[w][0][0])[u];
             } else {
                 float top = kLowest;
                 for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, *cluster.map_shared_rank(&cm[r], c));
@@ -455,30 +509,27 @@ __global__ void __launch_bounds__(kRowWarps * 32) attend_rows_kernel(const Atten
                     const float m = *cluster.map_shared_rank(&cm[r], c);
                     const float f = m == kLowest ? 0.0f : exp2_of(m - top);
                     l += f * *cluster.map_shared_rank(&cl[r], c);
-                    sum += f * *cluster.map_shared_rank(&so[u], c);
+                    sum += f * *cluster.map_shared_rank(&so[0][0][0] + u, c);
                 }
             }
-            if (rr < rows) {
-                const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
-                store1(a.out, (size_t)((t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head) + d, a.o_type,
-                       l == 0.0f ? 0.0f : sum / l);
-            }
+            const long long rr = r0 + r;
+            const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
+            store1(a.out, (size_t)((t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head) + d, a.o_type,
+                   l == 0.0f ? 0.0f : sum / l);
         }
         if (parts > 1) cluster_sync();
         else __syncthreads();
     }
 }
 
-template <int D, bool Q8, bool SPLIT>
+template <int D, bool Q8, bool SPLIT, int NT>
 cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
-    constexpr int SMEM = kRowWarps * 16 * D * 4;
     static std::atomic<bool> done[kMaxDevices];
-    cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT>, SMEM, true, done);
+    cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT, NT>, 0, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
-    c.blockDim = dim3(kRowWarps * 32);
-    c.dynamicSmemBytes = SMEM;
+    c.blockDim = dim3(kRowThreads);
     c.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -486,14 +537,30 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = grid.x > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, attend_rows_kernel<D, Q8, SPLIT>, a);
+    return cudaLaunchKernelEx(&c, attend_rows_kernel<D, Q8, SPLIT, NT>, a);
+}
+
+// 8-row tiles where a call has no more rows a cache head than that, else 16.
+// Keys are cut over more CTAs of a cluster while the GPU (148 SMs, about three
+// CTAs each) is not full and every CTA keeps two blocks a warp.
+template <int D, bool Q8, bool SPLIT>
+cudaError_t launch_rows(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+    const uint64_t rows = most_new * a.group;
+    const int r = rows <= 8 ? 8 : 16;
+    uint64_t tiles = (rows + r - 1) / r;
+    if (tiles * a.kv.heads > 65535) tiles = 65535 / a.kv.heads;
+    const uint64_t base = tiles * a.kv.heads * a.seq.seqs;
+    uint32_t parts = 1;
+    while (parts < 16 && base * parts < 3 * 148 && most_len / (parts * 2) >= kRowWarps * 32) parts *= 2;
+    const dim3 grid(parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs);
+    return r == 8 ? launch_rows<D, Q8, SPLIT, 1>(a, grid, s) : launch_rows<D, Q8, SPLIT, 2>(a, grid, s);
 }
 
 template <int D>
-cudaError_t launch_rows(const AttendArgs &a, bool q8, dim3 grid, cudaStream_t s) {
-    const bool split = a.q_type == MGB_F32;
-    if (q8) return split ? launch_rows<D, true, true>(a, grid, s) : launch_rows<D, true, false>(a, grid, s);
-    return split ? launch_rows<D, false, true>(a, grid, s) : launch_rows<D, false, false>(a, grid, s);
+cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+    if (a.q_type == MGB_F32)
+        return q8 ? launch_rows<D, true, true>(a, most_new, most_len, s) : launch_rows<D, false, true>(a, most_new, most_len, s);
+    return q8 ? launch_rows<D, true, false>(a, most_new, most_len, s) : launch_rows<D, false, false>(a, most_new, most_len, s);
 }
 
 }  // namespace
@@ -514,22 +581,15 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, q->heads / kv->heads,
                  scale * kLog2e};
-    uint64_t tiles = ((uint64_t)bound_new(*seqs, q->tokens) * a.group + 15) / 16;
-    if (tiles * kv->heads > 65535) tiles = 65535 / kv->heads;
-    // Keys are cut over more CTAs while that adds parallelism (two CTAs an SM)
-    // and leaves each at least a block a warp.
-    const uint64_t base = tiles * kv->heads * seqs->seqs;
-    uint32_t parts = 1;
-    while (parts < 16 && base * parts * 2 <= 2 * 148 && bound_len(*seqs, kv->page) / (parts * 2) >= kRowWarps * 16) parts *= 2;
-    const dim3 grid(parts, (unsigned)(tiles * kv->heads), seqs->seqs);
+    const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
     cudaError_t e;
     switch (kv->dim) {
-        case 16: e = launch_rows<16>(a, q8, grid, s); break;
-        case 32: e = launch_rows<32>(a, q8, grid, s); break;
-        case 64: e = launch_rows<64>(a, q8, grid, s); break;
-        default: e = launch_rows<128>(a, q8, grid, s); break;
+        case 16: e = launch_rows<16>(a, q8, most_new, most_len, s); break;
+        case 32: e = launch_rows<32>(a, q8, most_new, most_len, s); break;
+        case 64: e = launch_rows<64>(a, q8, most_new, most_len, s); break;
+        default: e = launch_rows<128>(a, q8, most_new, most_len, s); break;
     }
     return op_launch_status(e, op);
 }

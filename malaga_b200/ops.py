@@ -43,12 +43,14 @@ def _cuda(x: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = 
 def _rows(x: torch.Tensor, name: str, device: torch.device, dim: int) -> _lib.Rows:
     """Packed rows [tokens, heads, dim] as the library takes them: any strides of tokens and heads."""
     kind = _TYPES.get(x.dtype)
-    _need(kind is not None, f"{name} must be float32, float16 or bfloat16")
-    _need(x.dim() == 3 and x.size(2) == dim, f"{name} must be [tokens, heads, {dim}]")
-    _need(x.device == device, f"{name} is on {x.device}, the cache on {device}")
-    ts, hs, ds = x.stride()
-    _need(ds == 1, f"the numbers of a row of {name} must be contiguous")
-    return _lib.Rows(x.data_ptr(), ts, hs, x.size(0), x.size(1), kind)
+    if kind is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, the cache on {device}")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != dim or strides[2] != 1:
+        raise ValueError(f"{name} must be [tokens, heads, {dim}] with contiguous rows")
+    return _lib.Rows(x.data_ptr(), strides[0], strides[1], shape[0], shape[1], kind)
 
 
 def _call(device: torch.device, fn, *args) -> None:
@@ -142,7 +144,8 @@ class PagedKV:
         return cls(*data, *scales)
 
     def _check(self, seqs: Seqs) -> None:
-        _need(seqs.device == self.device, f"the sequences are on {seqs.device}, the cache on {self.device}")
+        if seqs.device != self.device:
+            raise ValueError(f"the sequences are on {seqs.device}, the cache on {self.device}")
 
     def write(self, seqs: Seqs, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes the new tokens' rows k, v [tokens, heads, dim] into their pages."""
@@ -175,7 +178,7 @@ class PagedKV:
         self._check(seqs)
         cq = _rows(q, "q", self.device, self.dim)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         co = _rows(out, "out", self.device, self.dim)
         _call(self.device, self._lib.mgb_kv_attend, self._ref, seqs._ref, ctypes.byref(cq), ctypes.byref(co),
               self.dim ** -0.5 if scale is None else scale, causal)
@@ -239,20 +242,24 @@ class LogitRules:
         the token with the largest result (the lowest on ties; int32, -1 where nothing may be chosen)
         and its log-probability (float32) among the results. adjusted, of the logits' type and shape,
         gets the results themselves and comes back as a third value; it may be the logits."""
-        kind = _TYPES.get(logits.dtype)
-        _need(kind is not None, "logits must be float32, float16 or bfloat16")
-        _need(logits.dim() == 2 and logits.is_cuda and logits.stride(1) == 1,
-              "logits must be [rows, vocab] on a GPU with contiguous rows")
-        device, (rows, vocab) = logits.device, logits.shape
-        _need(self.rows in (None, rows), f"the rules are for {self.rows} rows, the logits have {rows}")
-        _need(self.device in (None, device), f"the rules are on {self.device}, the logits on {device}")
+        kind, shape, strides = _TYPES.get(logits.dtype), logits.shape, logits.stride()
+        if kind is None:
+            raise ValueError("logits must be float32, float16 or bfloat16")
+        if len(shape) != 2 or not logits.is_cuda or strides[1] != 1:
+            raise ValueError("logits must be [rows, vocab] on a GPU with contiguous rows")
+        device, (rows, vocab) = logits.device, shape
+        if self.rows is not None and self.rows != rows:
+            raise ValueError(f"the rules are for {self.rows} rows, the logits have {rows}")
+        if self.device is not None and self.device != device:
+            raise ValueError(f"the rules are on {self.device}, the logits on {device}")
         y, y_stride = None, 0
         if adjusted is not None:
-            _need(adjusted.dtype == logits.dtype and adjusted.shape == logits.shape and adjusted.device == device
-                  and adjusted.stride(1) == 1, "adjusted must be like the logits")
+            if (adjusted.dtype != logits.dtype or adjusted.shape != shape or adjusted.device != device
+                    or adjusted.stride(1) != 1):
+                raise ValueError("adjusted must be like the logits")
             y, y_stride = adjusted.data_ptr(), adjusted.stride(0)
         ids = torch.empty(rows, dtype=torch.int32, device=device)
         logp = torch.empty(rows, dtype=torch.float32, device=device)
-        _call(device, self._lib.mgb_logits_choose, logits.data_ptr(), kind, logits.stride(0), rows, vocab, self._ref,
+        _call(device, self._lib.mgb_logits_choose, logits.data_ptr(), kind, strides[0], rows, vocab, self._ref,
               ids.data_ptr(), logp.data_ptr(), y, y_stride)
         return (ids, logp) if adjusted is None else (ids, logp, adjusted)
