@@ -71,19 +71,19 @@ __device__ __forceinline__ uint32_t codes2(uint32_t biased, uint32_t sel) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// BYTES bytes at p (aligned to their size, at most 16) into words.
+// BYTES bytes of shared memory at p (aligned to their size, at most 16) into words.
 template <int BYTES>
 __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
     if constexpr (BYTES == 16) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint4 x = *reinterpret_cast<const uint4 *>(p);
         w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else if constexpr (BYTES == 8) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
         w[0] = x.x, w[1] = x.y;
     } else if constexpr (BYTES == 4) {
-        w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
     } else {
-        w[0] = __ldg(reinterpret_cast<const uint16_t *>(p));
+        w[0] = *reinterpret_cast<const uint16_t *>(p);
     }
 }
 
@@ -92,16 +92,18 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
 // the rows are the 8-wide side of mma.m16n8k16 and a single query wastes as
-// little as it can. K and V go from global memory straight into the registers
-// in which the mma wants them as its A operand, with 16-byte loads: the order
-// of the head dimension inside q . k is free (Q is permuted the same way), and
-// so is the order of the rows of O^T. For K, four lanes share a key and take
-// every fourth vector of its row; for V, eight lanes share a key, and a byte
-// permute pairs two keys. movmatrix turns P^T, as it leaves the first product,
-// into the B operand of the second.
+// little as it can. A lane reads K and V from shared memory in 16-byte pieces
+// that are its parts of the mma's A operand: the order of the head dimension
+// inside q . k is free (Q is permuted the same way), and so is the order of the
+// rows of O^T. For K, four lanes share a key and take every fourth vector of
+// its row; for V, eight lanes share a key, and a byte permute pairs two keys.
+// movmatrix turns P^T, as it leaves the first product, into the B operand of
+// the second.
 //
-// A warp takes blocks of 16 keys in turn and keeps its own maximum, sum and
-// output. The maximum only has to be near: it is raised when a score passes it
+// A warp takes blocks of 16 keys in turn. Each block of K, V and their scales
+// is one contiguous run of its page, which a bulk copy brings into the warp's
+// own ring of stages, so the loads in flight do not depend on registers or on
+// the page table's latency. A warp keeps its own maximum, sum and output. The maximum only has to be near: it is raised when a score passes it
 // by 2^8, so most blocks need one vote and no reduction across lanes. Warps
 // join in shared memory, the CTAs of a cluster (which cut the keys among them)
 // through distributed shared memory, in a fixed order.
@@ -130,68 +132,58 @@ constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
 constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
 constexpr float kRaise = 7.0f;  // p is held as 2^7 p, up to 2^15
 
-// Where a block of 16 keys lies. left: how many of its keys exist (0 where the
-// table names no page of the cache); the others are read as zeros.
-struct Place {
-    size_t row;
-    int left;
-    bool hole;
+// A stage: 16 keys of K and of V, then their scales (8-bit caches).
+template <int D, bool Q8>
+struct Ring {
+    static constexpr int ROWS = 16 * D * (Q8 ? 1 : 2), SCALES = Q8 ? 64 : 0;
+    static constexpr int STAGE = 2 * ROWS + 2 * SCALES;
+    static constexpr int FIT = 16384 / STAGE;  // about 16 KB a warp in flight, at most 8 stages
+    static constexpr int N = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;
+    static constexpr int BYTES = kRowWarps * N * STAGE;
 };
 
-__device__ __forceinline__ Place place_of(const AttendArgs &a, uint32_t head, uint32_t page, int key0, int end) {
-    Place p;
-    p.hole = page >= a.kv.pages;
-    p.row = a.kv.row(p.hole ? 0 : page, head, (uint32_t)key0 & ((1u << a.kv.page_log2) - 1));
-    p.left = p.hole ? 0 : end - key0;
-    return p;
-}
-
 template <int D, bool Q8>
-struct KBlock {
-    uint32_t w[2][Frag<D, Q8>::KW];  // keys g, g + 8
-    float scale[2];
-    Place at;
-    __device__ __forceinline__ void load(const AttendArgs &a, const Place &p, int g, int t) {
+struct Block {  // a lane's share of 16 keys
+    uint32_t k[2][Frag<D, Q8>::KW];  // keys g, g + 8
+    uint32_t v[4][Frag<D, Q8>::VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+    float ks[2], vs[2];              // scales of keys g, g + 8
+    // left: keys that exist; the places of the others hold anything
+    __device__ __forceinline__ void load_k(const uint8_t *stage, int g, int t) {
         using F = Frag<D, Q8>;
-        at = p;
-        const uint8_t *k = static_cast<const uint8_t *>(a.kv.k) + p.row * (D * F::ESZ);
+        using R = Ring<D, Q8>;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int key = g + 8 * u;
 #pragma unroll
-            for (int i = 0; i < F::KW; ++i) w[u][i] = 0;
-            scale[u] = 0.0f;
-            if (key < p.left) {
-#pragma unroll
-                for (int c = 0; c < F::KN; ++c)
-                    load_words<F::KB>(k + key * (D * F::ESZ) + (t + 4 * c) * F::KB, &w[u][c * (F::KB / 4)]);
-                if constexpr (Q8) scale[u] = __ldg(a.kv.ks + p.row + key);
-            }
+            for (int c = 0; c < F::KN; ++c)
+                load_words<F::KB>(stage + (g + 8 * u) * (D * F::ESZ) + (t + 4 * c) * F::KB, &k[u][c * (F::KB / 4)]);
+            if constexpr (Q8) ks[u] = reinterpret_cast<const float *>(stage + 2 * R::ROWS)[g + 8 * u];
         }
     }
-};
-
-template <int D, bool Q8>
-struct VBlock {
-    uint32_t w[4][Frag<D, Q8>::VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
-    float scale[2];                  // of keys g, g + 8
-    __device__ __forceinline__ void load(const AttendArgs &a, const Place &p, int g, int t) {
+    __device__ __forceinline__ void load_v(const uint8_t *stage, int left, int g, int t) {
         using F = Frag<D, Q8>;
-        const uint8_t *v = static_cast<const uint8_t *>(a.kv.v) + p.row * (D * F::ESZ);
+        using R = Ring<D, Q8>;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int key = 2 * t + (u & 1) + 8 * (u >> 1);
 #pragma unroll
-            for (int i = 0; i < F::VW; ++i) w[u][i] = 0;
-            if (key < p.left) {
-#pragma unroll
-                for (int c = 0; c < F::VN; ++c)
-                    load_words<F::VB>(v + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &w[u][c * (F::VB / 4)]);
-            }
+            for (int c = 0; c < F::VN; ++c)
+                load_words<F::VB>(stage + R::ROWS + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &v[u][c * (F::VB / 4)]);
         }
         if constexpr (Q8) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) scale[u] = g + 8 * u < p.left ? __ldg(a.kv.vs + p.row + g + 8 * u) : 0.0f;
+            for (int u = 0; u < 2; ++u)
+                vs[u] = reinterpret_cast<const float *>(stage + 2 * R::ROWS + R::SCALES)[g + 8 * u];
+        }
+        if (left < 16) {  // 0 times what a stale place holds must stay 0
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (2 * t + (u & 1) + 8 * (u >> 1) >= left) {
+#pragma unroll
+                    for (int i = 0; i < F::VW; ++i) v[u][i] = 0;
+                }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (Q8 && g + 8 * u >= left) vs[u] = 0.0f;
         }
     }
 };
@@ -227,7 +219,8 @@ struct Rows {
     float m[NT][2], l[NT][2];
     int exp_v;  // V's scales so far are below 2^exp_v
 
-    __device__ __forceinline__ void step(const KBlock<D, Q8> &k, const VBlock<D, Q8> &v, int key0, int g) {
+    __device__ __forceinline__ void step(Block<D, Q8> &x, const uint8_t *stage, int key0, int end, int g, int t) {
+        x.load_k(stage, g, t);
         float s[NT][4];  // key g: rows 2t, 2t + 1; key g + 8: the same
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -235,39 +228,40 @@ struct Rows {
             for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
 #pragma unroll
         for (int st = 0; st < F::STEPS; ++st) {
-            uint32_t x[4];
+            uint32_t a[4];
             if constexpr (Q8) {
-                const uint32_t lo = k.w[0][st] ^ 0x80808080u, hi = k.w[1][st] ^ 0x80808080u;
-                x[0] = codes2(lo, 0x4140), x[1] = codes2(hi, 0x4140);
-                x[2] = codes2(lo, 0x4342), x[3] = codes2(hi, 0x4342);
+                const uint32_t lo = x.k[0][st] ^ 0x80808080u, hi = x.k[1][st] ^ 0x80808080u;
+                a[0] = codes2(lo, 0x4140), a[1] = codes2(hi, 0x4140);
+                a[2] = codes2(lo, 0x4342), a[3] = codes2(hi, 0x4342);
             } else {
-                x[0] = k.w[0][2 * st], x[1] = k.w[1][2 * st];
-                x[2] = k.w[0][2 * st + 1], x[3] = k.w[1][2 * st + 1];
+                a[0] = x.k[0][2 * st], a[1] = x.k[1][2 * st];
+                a[2] = x.k[0][2 * st + 1], a[3] = x.k[1][2 * st + 1];
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma16(s[n], x, q[0][n][st][0], q[0][n][st][1]);
-                if constexpr (SPLIT) mma16(s[n], x, q[1][n][st][0], q[1][n][st][1]);
+                mma16(s[n], a, q[0][n][st][0], q[0][n][st][1]);
+                if constexpr (SPLIT) mma16(s[n], a, q[1][n][st][0], q[1][n][st][1]);
             }
         }
-        const bool whole = key0 + 16 <= all && !k.at.hole;
+        x.load_v(stage, end - key0, g, t);
+        const bool whole = key0 + 16 <= all;
         bool see[NT][4], past = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                see[n][e] = whole || (key0 + g + 8 * (e >> 1) < limit[n][e & 1] && !k.at.hole);
-                s[n][e] = see[n][e] ? s[n][e] * (Q8 ? scale[n][e & 1] * k.scale[e >> 1] : scale[n][e & 1]) : kLowest;
+                see[n][e] = whole || key0 + g + 8 * (e >> 1) < limit[n][e & 1];
+                s[n][e] = see[n][e] ? s[n][e] * (Q8 ? scale[n][e & 1] * x.ks[e >> 1] : scale[n][e & 1]) : kLowest;
                 past |= s[n][e] > m[n][e & 1] + kSlack;
             }
         if constexpr (Q8) {
-            const float d = fmaxf(fabsf(v.scale[0]), fabsf(v.scale[1]));
+            const float d = fmaxf(fabsf(x.vs[0]), fabsf(x.vs[1]));
             past |= (__float_as_int(d) >> 23) - 126 > exp_v;
         }
         if (__any_sync(0xffffffffu, past)) {
             float f = 1.0f;
             if constexpr (Q8) {
-                const float d = max_keys(fmaxf(fabsf(v.scale[0]), fabsf(v.scale[1])));
+                const float d = max_keys(fmaxf(fabsf(x.vs[0]), fabsf(x.vs[1])));
                 const int e = max(exp_v, min(126, (__float_as_int(d) >> 23) - 126));
                 f = power_of_2(exp_v - e);
                 exp_v = e;
@@ -298,7 +292,7 @@ struct Rows {
             for (int e = 0; e < 4; ++e) {
                 w[e] = exp2_of(s[n][e] - z[e & 1]);
                 l[n][e & 1] += w[e];
-                if constexpr (Q8) w[e] = see[n][e] ? w[e] * (v.scale[e >> 1] * back) : 0.0f;
+                if constexpr (Q8) w[e] = see[n][e] ? w[e] * (x.vs[e >> 1] * back) : 0.0f;
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -311,18 +305,18 @@ struct Rows {
             }
         }
         auto pair = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-            const uint32_t x[4] = {a0, a1, a2, a3};
+            const uint32_t f[4] = {a0, a1, a2, a3};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma16(o[n][j], x, p[0][n][0], p[0][n][1]);
-                if constexpr (SPLIT) mma16(o[n][j], x, p[1][n][0], p[1][n][1]);
+                mma16(o[n][j], f, p[0][n][0], p[0][n][1]);
+                if constexpr (SPLIT) mma16(o[n][j], f, p[1][n][0], p[1][n][1]);
             }
         };
 #pragma unroll
         for (int i = 0; i < F::VW; ++i) {
             if constexpr (Q8) {
-                const uint32_t x0 = v.w[0][i] ^ 0x80808080u, x1 = v.w[1][i] ^ 0x80808080u;
-                const uint32_t x2 = v.w[2][i] ^ 0x80808080u, x3 = v.w[3][i] ^ 0x80808080u;
+                const uint32_t x0 = x.v[0][i] ^ 0x80808080u, x1 = x.v[1][i] ^ 0x80808080u;
+                const uint32_t x2 = x.v[2][i] ^ 0x80808080u, x3 = x.v[3][i] ^ 0x80808080u;
                 const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
                 constexpr int PER = F::STEPS < 2 ? 1 : 2;
                 pair(PER * i, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
@@ -331,8 +325,8 @@ struct Rows {
                     pair(PER * i + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
                 }
             } else {
-                pair(i, __byte_perm(v.w[0][i], v.w[1][i], 0x5410), __byte_perm(v.w[0][i], v.w[1][i], 0x7632),
-                     __byte_perm(v.w[2][i], v.w[3][i], 0x5410), __byte_perm(v.w[2][i], v.w[3][i], 0x7632));
+                pair(i, __byte_perm(x.v[0][i], x.v[1][i], 0x5410), __byte_perm(x.v[0][i], x.v[1][i], 0x7632),
+                     __byte_perm(x.v[2][i], x.v[3][i], 0x5410), __byte_perm(x.v[2][i], x.v[3][i], 0x7632));
             }
         }
     }
@@ -343,7 +337,12 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     using F = Frag<D, Q8>;
     constexpr int R = 8 * NT, PER_ROW = kRowThreads / R, E = D / PER_ROW;
     static_assert(E >= 1, "at most one thread a number");
-    __shared__ __align__(16) float so[kRowWarps][R][D];
+    using RG = Ring<D, Q8>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    static_assert(RG::BYTES >= kRowWarps * R * D * 4, "the warps' outputs take the rings' place");
+    float(*so)[R][D] = reinterpret_cast<float(*)[R][D]>(smem);
+    __shared__ uint64_t full[kRowWarps][RG::N];
+    __shared__ int have[kRowWarps][RG::N];  // whether the stage's block is in the cache
     __shared__ __align__(16) __half sq[SPLIT ? 2 : 1][R][D];
     __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R];
     __shared__ int row_limit[R];
@@ -355,6 +354,10 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const long long rows = (long long)n * a.group;
+    if (lane < RG::N) mbar_init(&full[warp][lane], 1);
+    __syncwarp();
+    uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
+    uint32_t taken = 0;  // blocks of this warp so far, over all tiles
     // keys that token i sees
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 
@@ -362,13 +365,36 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         const int end = limit((int)((min(r0 + R, rows) - 1) / a.group));  // no row of the tile sees further
         const int blocks = (end + 15) / 16;
         const int first = (int)((long long)blocks * part / parts), stop = (int)((long long)blocks * (part + 1) / parts);
-        // the first keys are on their way while the queries are prepared
-        auto page_of = [&](int blk) { return blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u; };
-        int blk = first + warp;
-        KBlock<D, Q8> k0, k1;
-        VBlock<D, Q8> v;
-        uint32_t page = page_of(blk), next = page_of(blk + kRowWarps);
-        if (blk < stop) k0.load(a, place_of(a, head, page, blk * 16, end), g, t);
+        const int mine = first + warp < stop ? (stop - first - warp + kRowWarps - 1) / kRowWarps : 0;
+        // block i of the warp is number first + warp + i * kRowWarps; the lanes hold the pages of 32 of them
+        uint32_t pages = 0;
+        auto issue = [&](int i) {
+            if ((i & 31) == 0) {
+                const int blk = first + warp + (i + lane) * kRowWarps;
+                pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u;
+            }
+            const uint32_t page = __shfl_sync(0xffffffffu, pages, i & 31);
+            if (lane == 0) {
+                const uint32_t st = (taken + i) % RG::N;
+                uint8_t *at = ring + st * RG::STAGE;
+                const int key0 = (first + warp + i * kRowWarps) * 16;
+                const bool there = page < a.kv.pages;
+                have[warp][st] = there;
+                if (there) {
+                    const size_t row = a.kv.row(page, head, (uint32_t)key0 & ((1u << a.kv.page_log2) - 1));
+                    mbar_expect_tx(&full[warp][st], RG::STAGE);
+                    bulk_g2s(at, static_cast<const uint8_t *>(a.kv.k) + row * (D * F::ESZ), RG::ROWS, &full[warp][st]);
+                    bulk_g2s(at + RG::ROWS, static_cast<const uint8_t *>(a.kv.v) + row * (D * F::ESZ), RG::ROWS, &full[warp][st]);
+                    if constexpr (Q8) {
+                        bulk_g2s(at + 2 * RG::ROWS, a.kv.ks + row, RG::SCALES, &full[warp][st]);
+                        bulk_g2s(at + 2 * RG::ROWS + RG::SCALES, a.kv.vs + row, RG::SCALES, &full[warp][st]);
+                    }
+                } else {
+                    mbar_arrive_cta(&full[warp][st]);
+                }
+            }
+        };
+        for (int i = 0; i < min(mine, RG::N); ++i) issue(i);
 
         // Q: the row's largest number to just below 2^14 (f16 q stays as it is)
         {
@@ -429,20 +455,19 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                 for (int e = 0; e < 4; ++e) st.o[j][s][e] = 0.0f;
         }
 
-        // V of a block and K of the next are on their way while the block's scores are formed
-        while (blk < stop) {
-            const int b1 = blk + kRowWarps, b2 = b1 + kRowWarps;
-            v.load(a, k0.at, g, t);
-            if (b1 < stop) k1.load(a, place_of(a, head, next, b1 * 16, end), g, t);
-            next = page_of(b2);
-            st.step(k0, v, blk * 16, g);
-            if (b1 >= stop) break;
-            v.load(a, k1.at, g, t);
-            if (b2 < stop) k0.load(a, place_of(a, head, next, b2 * 16, end), g, t);
-            next = page_of(b2 + kRowWarps);
-            st.step(k1, v, b1 * 16, g);
-            blk = b2;
+        bool lost = false;  // a copy did not arrive in time: the rows become NaN
+        for (int i = 0; i < mine; ++i) {
+            const uint32_t st_no = (taken + i) % RG::N;
+            lost |= !mbar_wait(&full[warp][st_no], ((taken + i) / RG::N) & 1);
+            if (have[warp][st_no]) {
+                Block<D, Q8> x;
+                st.step(x, ring + st_no * RG::STAGE, (first + warp + i * kRowWarps) * 16, end, g, t);
+            }
+            __syncwarp();  // every lane has read the stage
+            if (i + RG::N < mine) issue(i + RG::N);
         }
+        taken += mine;
+        if (lost) st.l[0][0] = st.l[0][1] = st.l[NT - 1][0] = st.l[NT - 1][1] = __int_as_float(0x7fffffff);
 
         // the CTA's warps
 #pragma unroll
@@ -517,6 +542,8 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             store1(a.out, (size_t)((t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head) + d, a.o_type,
                    l == 0.0f ? 0.0f : sum / l);
         }
+        // the next tile's copies go where this one's outputs stood
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (parts > 1) cluster_sync();
         else __syncthreads();
     }
@@ -524,12 +551,14 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
 
 template <int D, bool Q8, bool SPLIT, int NT>
 cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
+    constexpr int SMEM = Ring<D, Q8>::BYTES;
     static std::atomic<bool> done[kMaxDevices];
-    cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT, NT>, 0, true, done);
+    cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT, NT>, SMEM, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
     c.blockDim = dim3(kRowThreads);
+    c.dynamicSmemBytes = SMEM;
     c.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;

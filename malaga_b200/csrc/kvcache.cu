@@ -1,19 +1,20 @@
 // Writing rows into a paged K/V cache, and reading them back.
 //
 // Both move each number once and compute next to nothing, so HBM bounds them.
-// A row (one position of one head of K or V) is spread over dim / 8 lanes of 8
-// numbers each: one 16-byte access of 16-bit numbers a lane, and the maximum
-// over the row is a shuffle over at most 16 lanes. Rows run over heads first,
-// as the packed rows lie; in the cache each row is its own contiguous run of
-// dim to 2 * dim bytes. A row with an infinity or NaN has no 8-bit form: its
-// scale is NaN, so all of it reads back as NaN.
+// A CTA takes a run of the call's tokens: its threads first look up each
+// token's place (a search for its sequence, then the page table), then move the
+// rows of all heads, K and V. A row is spread over dim / 8 lanes of 8 numbers;
+// the lanes' pieces are laid out so that a warp's accesses to the packed rows
+// are contiguous for 32-bit and for 16-bit numbers. Tokens are cut evenly over
+// the CTAs whatever the sequences' lengths.
 #include "serving.cuh"
 
 namespace mgb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;  // rows of a thread in flight
+constexpr int kBatch = 4;       // rows of a thread in flight
+constexpr int kMaxTokens = 16;  // tokens of a CTA
 
 #define kInf __int_as_float(0x7f800000)
 #define kNan __int_as_float(0x7fffffff)
@@ -25,100 +26,133 @@ struct MoveArgs {
     long long k_token, k_head, v_token, v_head;  // strides in numbers
     int k_type, v_type;
     bool k_vec, v_vec;
+    uint32_t per_cta;  // tokens of a CTA
 };
 
-// grid (row groups, sequences, K or V). A row group takes rows of its sequence
-// in steps of the grid, so any number of new tokens is handled whatever the
-// grid was sized for.
+// Code bytes of x / d for four numbers. x * (1 / d) is within 2^-15 of the f32
+// quotient (|x / d| <= 127), so it rounds to the same whole number unless it
+// lies that near a half; then the quotient itself is taken. Adding 1.5 * 2^23
+// rounds to a whole number, halves to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t codes_of(const float *x, float d, float inv, bool tiny) {
+    constexpr float kWhole = 12582912.0f;
+    uint32_t r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float q = x[e] * inv, w = q + kWhole;
+        r[e] = __float_as_uint(w);
+        if (tiny || fabsf(q - (w - kWhole)) > 0.4999f)
+            r[e] = d > 0.0f ? __float_as_uint(fminf(fmaxf(__fdiv_rn(x[e], d), -127.0f), 127.0f) + kWhole) : 0u;
+    }
+    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+
+// Four code bytes as f32: the bytes 00 00 4b above u are the number 2^23 + u.
+__device__ __forceinline__ void values_of(uint32_t codes, float d, float *x) {
+    const uint32_t u = codes ^ 0x80808080u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = d * (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + e)) - 8388736.0f);
+}
+
 template <int DIM, bool Q8, bool WRITE>
 __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     constexpr int LANES = DIM / 8, ROWS = kThreads / LANES;
-    const uint32_t b = blockIdx.y;
-    const bool is_v = blockIdx.z;
-    int n;
-    const int t0 = a.seq.first(b, n);
-    const int base = a.seq.length(b, a.kv.page_log2), len = a.seq.kv_len[b];
-    const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
+    __shared__ int64_t place[kMaxTokens];  // row of head 0 in the cache, -1 where there is none
+    const uint32_t first = blockIdx.x * a.per_cta, tokens = min(a.per_cta, a.seq.tokens - first);
+    if (threadIdx.x < tokens) {
+        const int token = (int)(first + threadIdx.x);
+        // the last sequence that starts at or before the token
+        uint32_t lo = 0, hi = a.seq.seqs;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (a.seq.q_start[mid] <= token) lo = mid;
+            else hi = mid;
+        }
+        int64_t row = -1;
+        const int start = a.seq.q_start[lo], stop = a.seq.q_start[lo + 1];
+        if (token >= start && token < stop) {
+            const long long pos = (long long)a.seq.kv_len[lo] - (stop - token);
+            if (pos >= 0 && (pos >> a.kv.page_log2) < a.seq.table_stride) {
+                const uint32_t page = (uint32_t)a.seq.table[(size_t)lo * a.seq.table_stride + (pos >> a.kv.page_log2)];
+                if (page < a.kv.pages) row = (int64_t)a.kv.row(page, 0, (uint32_t)pos & ((1u << a.kv.page_log2) - 1));
+            }
+        }
+        place[threadIdx.x] = row;
+    }
+    __syncthreads();
+
+    const bool is_v = blockIdx.y;
     void *rows = is_v ? a.v : a.k;
-    const long long token = is_v ? a.v_token : a.k_token, head = is_v ? a.v_head : a.k_head;
+    const long long token_stride = is_v ? a.v_token : a.k_token, head_stride = is_v ? a.v_head : a.k_head;
     const int type = is_v ? a.v_type : a.k_type;
     const bool vec = is_v ? a.v_vec : a.k_vec;
-    void *data = is_v ? a.kv.v : a.kv.k;
+    uint8_t *data = static_cast<uint8_t *>(is_v ? a.kv.v : a.kv.k);
     float *scale = is_v ? a.kv.vs : a.kv.ks;
-    const int lane = threadIdx.x % LANES, part = lane * 8;
-    const uint32_t heads = a.kv.heads;
-    const uint64_t total = (uint64_t)n * heads;
+    // a lane's two pieces of four numbers: apart for 32-bit rows, side by side for 16-bit ones
+    const int lane = threadIdx.x % LANES;
+    const int p0 = type == MGB_F32 ? 4 * lane : 8 * lane, p1 = type == MGB_F32 ? DIM / 2 + 4 * lane : 8 * lane + 4;
+    const uint32_t heads = a.kv.heads, total = tokens * heads;
 
-    for (uint64_t r0 = (uint64_t)blockIdx.x * (ROWS * kBatch); r0 < total; r0 += (uint64_t)gridDim.x * (ROWS * kBatch)) {
-        const uint32_t i0 = (uint32_t)(r0 / heads), h0 = (uint32_t)(r0 - (uint64_t)i0 * heads) + threadIdx.x / LANES;
+    for (uint32_t r0 = 0; r0 < total; r0 += ROWS * kBatch) {
         float x[kBatch][8];
-        size_t at[kBatch], row[kBatch];
-        bool live[kBatch], placed[kBatch];
+        int64_t at[kBatch], row[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const uint32_t hu = h0 + u * ROWS, i = i0 + hu / heads, h = hu % heads;
-            live[u] = i < (uint32_t)n;
-            const long long pos = (long long)len - n + i;
-            placed[u] = live[u] && pos >= 0 && pos < base;
-            uint32_t page = 0;
-            if (placed[u]) {
-                page = (uint32_t)table[pos >> a.kv.page_log2];
-                placed[u] = page < a.kv.pages;
-            }
-            at[u] = (size_t)((long long)(t0 + i) * token + h * head + part);
-            row[u] = placed[u] ? a.kv.row(page, h, (uint32_t)pos & ((1u << a.kv.page_log2) - 1)) : 0;
+            const uint32_t r = r0 + u * ROWS + threadIdx.x / LANES, i = r / heads, h = r - i * heads;
+            row[u] = r < total ? place[i] : -2;  // -2: no such row
+            if (row[u] >= 0) row[u] += (int64_t)h << a.kv.page_log2;
+            at[u] = (int64_t)(first + i) * token_stride + (int64_t)h * head_stride;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
+            if (row[u] < 0) continue;
             if constexpr (WRITE) {
-                if (placed[u]) load8(rows, at[u], type, vec, x[u]);
-            } else if (placed[u]) {
-                if constexpr (Q8) {
-                    const uint2 c = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(data) + row[u] * DIM + part);
-                    const float d = scale[row[u]];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        x[u][e] = d * (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3)));
-                } else {
-                    load8(data, row[u] * DIM + part, MGB_F16, true, x[u]);
-                }
+                load4(rows, at[u] + p0, type, vec, &x[u][0]);
+                load4(rows, at[u] + p1, type, vec, &x[u][4]);
+            } else if constexpr (Q8) {
+                const uint8_t *c = data + row[u] * DIM;
+                const float d = scale[row[u]];
+                values_of(*reinterpret_cast<const uint32_t *>(c + p0), d, &x[u][0]);
+                values_of(*reinterpret_cast<const uint32_t *>(c + p1), d, &x[u][4]);
+            } else {
+                load4(data, row[u] * DIM + p0, MGB_F16, true, &x[u][0]);
+                load4(data, row[u] * DIM + p1, MGB_F16, true, &x[u][4]);
             }
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if constexpr (!WRITE) {
-                if (live[u]) store8(rows, at[u], type, vec, x[u]);
+                if (row[u] == -2) continue;
+                store4(rows, at[u] + p0, type, vec, &x[u][0]);
+                store4(rows, at[u] + p1, type, vec, &x[u][4]);
             } else if constexpr (Q8) {
                 float m = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m = fabsf(x[u][e]) <= 3.402823466e38f ? fmaxf(m, fabsf(x[u][e])) : kInf;
+                for (int e = 0; e < 8; ++e) m = fabsf(x[u][e]) < kInf ? fmaxf(m, fabsf(x[u][e])) : kInf;
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float d = m == kInf ? kNan : __fdiv_rn(m, 127.0f);
-                uint32_t c[2] = {0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    // the quotient is at most 127 in magnitude but for the rounding of d in the subnormal range
-                    const float q = d > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(x[u][e], d)), -127.0f), 127.0f) : 0.0f;
-                    c[e >> 2] |= ((uint32_t)(int)q & 255u) << (8 * (e & 3));
-                }
-                if (placed[u]) {
-                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(data) + row[u] * DIM + part) = make_uint2(c[0], c[1]);
+                const bool tiny = !(d > 1e-30f);  // 1 / d would leave f32's range, or there is no d
+                const float inv = tiny ? 0.0f : __frcp_rn(d);
+                const uint32_t c0 = codes_of(&x[u][0], d, inv, tiny), c1 = codes_of(&x[u][4], d, inv, tiny);
+                if (row[u] >= 0) {
+                    uint8_t *c = data + row[u] * DIM;
+                    *reinterpret_cast<uint32_t *>(c + p0) = c0;
+                    *reinterpret_cast<uint32_t *>(c + p1) = c1;
                     if (lane == 0) scale[row[u]] = d;
                 }
-            } else if (placed[u]) {
-                store8(data, row[u] * DIM + part, MGB_F16, true, x[u]);
+            } else if (row[u] >= 0) {
+                store4(data, row[u] * DIM + p0, MGB_F16, true, &x[u][0]);
+                store4(data, row[u] * DIM + p1, MGB_F16, true, &x[u][4]);
             }
         }
     }
 }
 
+// As many tokens a CTA as leave four CTAs an SM (148 SMs), at most kMaxTokens.
 template <int DIM, bool Q8, bool WRITE>
-cudaError_t launch(const MoveArgs &a, uint32_t max_new, cudaStream_t s) {
-    constexpr int ROWS = kThreads / (DIM / 8);
-    const uint64_t rows = (uint64_t)max_new * a.kv.heads;
-    uint64_t groups = (rows + ROWS * kBatch - 1) / (ROWS * kBatch);
-    if (groups > 65536) groups = 65536;
-    kv_move_kernel<DIM, Q8, WRITE><<<dim3((unsigned)groups, a.seq.seqs, 2), kThreads, 0, s>>>(a);
+cudaError_t launch(MoveArgs a, cudaStream_t s) {
+    const uint32_t n = a.seq.tokens / (2 * 148);
+    a.per_cta = n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n;
+    kv_move_kernel<DIM, Q8, WRITE><<<dim3((a.seq.tokens + a.per_cta - 1) / a.per_cta, 2), kThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -134,16 +168,15 @@ mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, co
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
     if (seqs->seqs == 0 || k->tokens == 0) return MGB_OK;
     MoveArgs a{view(*kv), view(*seqs, k->tokens), k->data, v->data, k->token_stride, k->head_stride,
-               v->token_stride, v->head_stride, k->type, v->type, rows_vec(*k), rows_vec(*v)};
+               v->token_stride, v->head_stride, k->type, v->type, rows_vec(*k), rows_vec(*v), 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
-    const uint32_t most_new = bound_new(*seqs, k->tokens);
     cudaError_t e;
     switch (kv->dim) {
-        case 16: e = q8 ? launch<16, true, WRITE>(a, most_new, s) : launch<16, false, WRITE>(a, most_new, s); break;
-        case 32: e = q8 ? launch<32, true, WRITE>(a, most_new, s) : launch<32, false, WRITE>(a, most_new, s); break;
-        case 64: e = q8 ? launch<64, true, WRITE>(a, most_new, s) : launch<64, false, WRITE>(a, most_new, s); break;
-        default: e = q8 ? launch<128, true, WRITE>(a, most_new, s) : launch<128, false, WRITE>(a, most_new, s); break;
+        case 16: e = q8 ? launch<16, true, WRITE>(a, s) : launch<16, false, WRITE>(a, s); break;
+        case 32: e = q8 ? launch<32, true, WRITE>(a, s) : launch<32, false, WRITE>(a, s); break;
+        case 64: e = q8 ? launch<64, true, WRITE>(a, s) : launch<64, false, WRITE>(a, s); break;
+        default: e = q8 ? launch<128, true, WRITE>(a, s) : launch<128, false, WRITE>(a, s); break;
     }
     return op_launch_status(e, op);
 }

@@ -3,7 +3,7 @@
 //
 // Every logit is read once, and written once where the adjusted row is wanted:
 // HBM bounds a batch, the launch and the merge a single row. A row is cut over
-// the CTAs of a cluster, which merge their (maximum, sum of exponentials,
+// the CTAs of a cluster, which join their (maximum, sum of exponentials,
 // index) through shared memory, so one launch needs no scratch and no atomics
 // on global memory, and the merge order is fixed.
 //
@@ -20,7 +20,6 @@ namespace mgb {
 namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kUnroll = 4;            // 16-byte loads of a thread in flight
 constexpr uint32_t kMaxTile = 32768;  // tokens of one bitmap
 constexpr int kSlotBytes = 96 * 1024;  // shared memory for slots at most
 constexpr uint32_t kNone = 0xffffffffu;
@@ -71,30 +70,33 @@ __device__ __forceinline__ Best shfl_xor(const Best &a, int o) {
                 __shfl_xor_sync(0xffffffffu, a.i, o)};
 }
 
-// N logits y at indices i0.. (-inf where they do not count) into b.
-template <int N>
-__device__ __forceinline__ void add(Best &b, const float (&y)[N], const uint32_t (&at)[N]) {
+// N logits y (-inf where they do not count) at tokens `first` + place(e) into b.
+template <int N, typename Place>
+__device__ __forceinline__ void add(Best &b, const float (&y)[N], uint32_t first, Place place) {
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, y[e]);
+    float own = 0.0f;  // the new maximum's own term, which the sum below would add
     if (top > b.m) {
         b.l = b.m == kLowest ? 0.0f : (1.0f + b.l) * exp2_of((b.m - top) * kLog2e);
         b.m = top;
-        b.i = kNone;
 #pragma unroll
         for (int e = N - 1; e >= 0; --e)
-            if (y[e] == top) b.i = at[e];
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (at[e] != b.i) b.l += weight_of(y[e], top);
-    } else if (b.m == kPosInf) {  // exp(inf - inf) counts as one
+            if (y[e] == top) b.i = first + place(e);
+        own = 1.0f;
+    }
+    if (b.m == kPosInf) {  // exp(inf - inf) counts as one
 #pragma unroll
         for (int e = 0; e < N; ++e) b.l += y[e] == kPosInf ? 1.0f : 0.0f;
+        b.l -= own;
     } else if (b.m > kLowest) {
-        float s = 0.0f;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += exp2_of((y[e] - b.m) * kLog2e);
-        b.l += s;
+        for (int e = 0; e < N; ++e) {
+            const float w = exp2_of((y[e] - b.m) * kLog2e);
+            s[e & 3] += own != 0.0f && b.i == first + place(e) ? 0.0f : w;
+        }
+        b.l += (s[0] + s[1]) + (s[2] + s[3]);
     }
 }
 
@@ -119,18 +121,18 @@ struct Num<MGB_BF16> {
     static __device__ __forceinline__ uint16_t put(float x) { return to_16(x, MGB_BF16); }
 };
 
-// Bits off .. off + 31 of a bit row of `words` words.
-__device__ __forceinline__ uint32_t bits_at(const uint32_t *row, uint32_t words, uint32_t off) {
-    const uint32_t w = off >> 5;
-    const uint32_t lo = row[w], hi = w + 1 < words ? row[w + 1] : 0;
-    return __funnelshift_r(lo, hi, off & 31);
+// Bits off .. off + 31 of a bit row of `words` words (off may be below 0).
+__device__ __forceinline__ uint32_t bits_at(const uint32_t *row, uint32_t words, int64_t off) {
+    const int64_t w = off >> 5;
+    const uint32_t lo = w >= 0 && w < words ? row[w] : 0, hi = w + 1 >= 0 && w + 1 < words ? row[w + 1] : 0;
+    return __funnelshift_r(lo, hi, (uint32_t)off & 31);
 }
 
-template <int TYPE, bool SLOTS>
-__global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
+template <int TYPE, bool RULES>
+__global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a) {
     using N = Num<TYPE>;
     using T = typename N::T;
-    constexpr int W = 16 / sizeof(T);
+    constexpr int W = 16 / sizeof(T), UNROLL = 16 / W;
     extern __shared__ uint32_t smem[];
     __shared__ Best warp_best[kWarps];
     __shared__ Best cta_best[16];
@@ -142,22 +144,21 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
     const mgb_logit_rules &r = a.rules;
     const T *x = reinterpret_cast<const T *>(a.x) + (size_t)row * a.stride;
     T *y = a.y ? reinterpret_cast<T *>(a.y) + (size_t)row * a.y_stride : nullptr;
-    const uint32_t *allow = nullptr;
-    if (r.allow) {
-        const int g = r.allow_row ? r.allow_row[row] : 0;
-        if (g >= 0 && (uint32_t)g < r.allow_rows) allow = r.allow + (size_t)g * r.allow_stride;
-    }
     // the row's share of this CTA, in whole 64s
     const uint32_t share = ((a.vocab + parts - 1) / parts + 63) & ~63u;
     const uint32_t c0 = min(a.vocab, part * share), c1 = min(a.vocab, c0 + share);
 
-    const uint32_t words = a.tile / 32;
-    uint32_t *mark = smem, *rank = mark + words, *count = rank + words, *token = count + a.cap;
+    // Bit maps of the tile, bit i for the token at the tile's first 16-byte
+    // boundary plus i, so that a vector's bits lie in one word.
+    const uint32_t words = a.tile / 32 + 1;
+    uint32_t *mark = smem, *off = mark + words, *rank = off + words;  // touched by a rule; ruled out by the grammar
+    uint32_t *count = rank + words, *token = count + a.cap;
     float *bias = reinterpret_cast<float *>(token + a.cap);
     uint32_t nh = 0;
     const int32_t *hist = nullptr, *bias_ids = nullptr;
+    const uint32_t *allow = nullptr;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if constexpr (SLOTS) {
+    if constexpr (RULES) {
         if (r.history) {
             hist = r.history + (size_t)row * r.history_stride;
             nh = r.history_len ? (uint32_t)min((long long)r.history_stride, (long long)max(0, r.history_len[row]))
@@ -167,138 +168,149 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
         if (r.repetition) rep = r.repetition[row];
         if (r.frequency) freq = r.frequency[row];
         if (r.presence) pres = r.presence[row];
+        if (r.allow) {
+            const int g = r.allow_row ? r.allow_row[row] : 0;
+            if (g >= 0 && (uint32_t)g < r.allow_rows) allow = r.allow + (size_t)g * r.allow_stride;
+        }
     }
+    const bool slotted = nh || bias_ids;
 
     Best best{kLowest, 0.0f, kNone};
     for (uint32_t v0 = c0; v0 < c1; v0 += a.tile) {
         const uint32_t v1 = min(c1, v0 + a.tile), width = v1 - v0;
+        const uint32_t shift = (uint32_t)(((uintptr_t)(x + v0) & 15) / sizeof(T));
         uint32_t slots = 0;
-        if constexpr (SLOTS) {
-            for (uint32_t w = tid; w < words; w += kThreads) mark[w] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < nh; i += kThreads) {
-                const uint32_t off = (uint32_t)hist[i] - v0;
-                if (off < width) atomicOr(&mark[off >> 5], 1u << (off & 31));
-            }
-            for (uint32_t i = tid; i < r.bias_count; i += kThreads) {
-                const uint32_t off = (uint32_t)bias_ids[i] - v0;
-                if (off < width) atomicOr(&mark[off >> 5], 1u << (off & 31));
+        if constexpr (RULES) {
+            for (uint32_t w = tid; w < words; w += kThreads) {
+                mark[w] = 0;
+                off[w] = allow ? ~bits_at(allow, r.allow_stride, (int64_t)v0 + 32 * w - shift) : 0u;
             }
             __syncthreads();
-            // rank[w]: marked tokens before word w; a thread has two words
-            const uint32_t p0 = 2 * tid < words ? __popc(mark[2 * tid]) : 0;
-            const uint32_t p1 = 2 * tid + 1 < words ? __popc(mark[2 * tid + 1]) : 0;
-            uint32_t upto = p0 + p1;
+            if (slotted) {
+                auto touch = [&](int32_t id) {
+                    const uint32_t i = (uint32_t)id - v0;
+                    if (i < width) atomicOr(&mark[(i + shift) >> 5], 1u << ((i + shift) & 31));
+                };
+                for (uint32_t i = tid; i < nh; i += kThreads) touch(hist[i]);
+                for (uint32_t i = tid; i < r.bias_count; i += kThreads) touch(bias_ids[i]);
+                __syncthreads();
+                // rank[w]: touched tokens before word w; a thread has four words
+                uint32_t pop[4], upto = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += u;
-            }
-            if (lane == 31) warp_sum[warp] = upto;
-            __syncthreads();
-            uint32_t before = 0;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) {
-                before += k < warp ? warp_sum[k] : 0;
-                slots += warp_sum[k];
-            }
-            before += upto - p0 - p1;
-            if (2 * tid < words) rank[2 * tid] = before;
-            if (2 * tid + 1 < words) rank[2 * tid + 1] = before + p0;
-            for (uint32_t k = tid; k < slots; k += kThreads) {
-                count[k] = 0;
-                bias[k] = 0.0f;
-            }
-            __syncthreads();
-            for (uint32_t i = tid; i < nh; i += kThreads) {
-                const uint32_t off = (uint32_t)hist[i] - v0;
-                if (off >= width) continue;
-                const uint32_t k = rank[off >> 5] + __popc(mark[off >> 5] & ((1u << (off & 31)) - 1));
-                atomicAdd(&count[k], 1u);
-                token[k] = off;
-            }
-            for (uint32_t i = tid; i < r.bias_count; i += kThreads) {
-                const int32_t id = bias_ids[i];
-                const uint32_t off = (uint32_t)id - v0;
-                if (off >= width) continue;
-                // the first entry of a token adds up all of them, in their order
-                float sum = 0.0f;
-                bool first = true;
-                for (uint32_t j = 0; j < r.bias_count && first; ++j) {
-                    if (bias_ids[j] != id) continue;
-                    first = j >= i;
-                    sum += r.bias[(size_t)row * r.bias_count + j];
+                for (int e = 0; e < 4; ++e) {
+                    pop[e] = 4 * tid + e < words ? __popc(mark[4 * tid + e]) : 0;
+                    upto += pop[e];
                 }
-                if (!first) continue;
-                const uint32_t k = rank[off >> 5] + __popc(mark[off >> 5] & ((1u << (off & 31)) - 1));
-                bias[k] = sum;
-                token[k] = off;
+                const uint32_t mine = upto;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += u;
+                }
+                if (lane == 31) warp_sum[warp] = upto;
+                __syncthreads();
+                uint32_t before = upto - mine;
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    before += k < warp ? warp_sum[k] : 0;
+                    slots += warp_sum[k];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (4 * tid + e < words) rank[4 * tid + e] = before;
+                    before += pop[e];
+                }
+                for (uint32_t k = tid; k < slots; k += kThreads) {
+                    count[k] = 0;
+                    bias[k] = 0.0f;
+                }
+                __syncthreads();
+                auto slot_of = [&](uint32_t i) {
+                    const uint32_t bit = i + shift, k = rank[bit >> 5] + __popc(mark[bit >> 5] & ((1u << (bit & 31)) - 1));
+                    token[k] = i;
+                    return k;
+                };
+                for (uint32_t i = tid; i < nh; i += kThreads) {
+                    const uint32_t at = (uint32_t)hist[i] - v0;
+                    if (at < width) atomicAdd(&count[slot_of(at)], 1u);
+                }
+                for (uint32_t i = tid; i < r.bias_count; i += kThreads) {
+                    const int32_t id = bias_ids[i];
+                    const uint32_t at = (uint32_t)id - v0;
+                    if (at >= width) continue;
+                    // the first entry of a token adds up all of them, in their order
+                    float sum = 0.0f;
+                    bool first = true;
+                    for (uint32_t j = 0; j < r.bias_count && first; ++j) {
+                        if (bias_ids[j] != id) continue;
+                        first = j >= i;
+                        sum += r.bias[(size_t)row * r.bias_count + j];
+                    }
+                    if (first) bias[slot_of(at)] = sum;
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
 
-        // streaming pass: vectors from the 16-byte boundary at or before v0
-        const uint32_t shift = (uint32_t)(((uintptr_t)(x + v0) & 15) / sizeof(T));
+        // streaming pass: vectors from the 16-byte boundary at or before v0; all but the first and last are whole
+        const uint4 *vectors = reinterpret_cast<const uint4 *>(x + v0 - shift);
         const bool y_vec = y && (((uintptr_t)(y + v0) & 15) / sizeof(T)) == shift;
         const uint32_t nvec = (width + shift + W - 1) / W;
-        for (uint32_t j0 = tid; j0 < nvec; j0 += kThreads * kUnroll) {
-            uint4 raw[kUnroll];
+        const uint32_t whole0 = shift ? 1 : 0, whole1 = (width + shift) / W;
+        for (uint32_t j0 = tid; j0 < nvec; j0 += kThreads * UNROLL) {
+            uint4 raw[UNROLL];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
+            for (int u = 0; u < UNROLL; ++u) {
                 const uint32_t j = j0 + u * kThreads;
-                const bool whole = j * W >= shift && j * W + W <= width + shift;
-                if (whole) raw[u] = __ldcs(reinterpret_cast<const uint4 *>(x + v0 - shift) + j);
+                if (j >= whole0 && j < whole1) raw[u] = __ldcs(vectors + j);
             }
+            float f[UNROLL * W];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
+            for (int u = 0; u < UNROLL; ++u) {
                 const uint32_t j = j0 + u * kThreads;
-                if (j >= nvec) break;
-                const uint32_t at = j * W - shift;  // of the tile; wraps in the first vector
-                const bool whole = j * W >= shift && j * W + W <= width + shift;
-                float f[W];
-                uint32_t idx[W];
-                uint32_t off_bits = 0, skip = 0;
-                if (whole) {
-                    const T *h = reinterpret_cast<const T *>(&raw[u]);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) f[e] = N::get(h[e]);
-                    if (allow) off_bits = ~bits_at(allow, r.allow_stride, v0 + at);
-                    if constexpr (SLOTS) skip = bits_at(mark, words, at);
+                uint32_t out_of = 0, touched = 0;  // bits of the vector
+                if constexpr (RULES) {
+                    const uint32_t w = (j * W) >> 5, s = (j * W) & 31;
+                    if (j < nvec) {
+                        touched = mark[w] >> s;
+                        out_of = off[w] >> s;
+                    }
+                }
+                T h[W];
+                if (j >= whole0 && j < whole1) {
+                    *reinterpret_cast<uint4 *>(h) = raw[u];
                 } else {
 #pragma unroll
                     for (int e = 0; e < W; ++e) {
-                        const uint32_t o = at + e;
-                        f[e] = 0.0f;
-                        if (o >= width) {
-                            skip |= 1u << e;
-                            continue;
-                        }
-                        f[e] = N::get(x[v0 + o]);
-                        if (allow && !((allow[(v0 + o) >> 5] >> ((v0 + o) & 31)) & 1)) off_bits |= 1u << e;
-                        if constexpr (SLOTS) skip |= ((mark[o >> 5] >> (o & 31)) & 1) << e;
+                        const uint32_t o = j * W + e - shift;
+                        h[e] = N::put(kLowest);
+                        if (j < nvec && o < width) h[e] = x[v0 + o];
                     }
                 }
-                if (y) {  // marked tokens keep their logit until the second pass
-                    T out[W];
+                // touched tokens keep their logit until the second pass
+                const uint32_t cut = out_of & ~touched;
 #pragma unroll
-                    for (int e = 0; e < W; ++e) out[e] = N::put(((off_bits & ~skip) >> e) & 1 ? kLowest : f[e]);
-                    if (whole && y_vec) {
-                        *(reinterpret_cast<uint4 *>(y + v0 - shift) + j) = *reinterpret_cast<const uint4 *>(out);
+                for (int e = 0; e < W; ++e)
+                    if ((cut >> e) & 1) h[e] = N::put(kLowest);
+                if (y && j < nvec) {
+                    if (y_vec && j >= whole0 && j < whole1) {
+                        reinterpret_cast<uint4 *>(y + v0 - shift)[j] = *reinterpret_cast<const uint4 *>(h);
                     } else {
 #pragma unroll
                         for (int e = 0; e < W; ++e)
-                            if (at + e < width) y[v0 + at + e] = out[e];
+                            if (j * W + e - shift < width) y[v0 + j * W + e - shift] = h[e];
                     }
                 }
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    if (((off_bits | skip) >> e) & 1 || !(f[e] == f[e])) f[e] = kLowest;
-                    idx[e] = v0 + at + e;
+                    // fmax drops NaN
+                    const float g = fmaxf(N::get(h[e]), kLowest);
+                    f[u * W + e] = RULES && ((touched >> e) & 1) ? kLowest : g;
                 }
-                add<W>(best, f, idx);
             }
+            add(best, f, v0 - shift + j0 * W, [](int e) { return (uint32_t)((e / W) * kThreads * W + e % W); });
         }
-        if constexpr (SLOTS) {
+        if constexpr (RULES) {
             __syncthreads();
             for (uint32_t k = tid; k < slots; k += kThreads) {
                 const uint32_t id = v0 + token[k], c = count[k];
@@ -310,11 +322,8 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
                 if (bias_ids) f = f + bias[k];
                 if (allow && !((allow[id >> 5] >> (id & 31)) & 1)) f = kLowest;
                 if (y) y[id] = N::put(f);
-                const float one[1] = {f == f ? f : kLowest};
-                const uint32_t at[1] = {id};
-                Best b{kLowest, 0.0f, kNone};
-                add<1>(b, one, at);
-                best = merge(best, b);
+                const Best one{fmaxf(f, kLowest), 0.0f, id};
+                if (one.m > kLowest) best = merge(best, one);
             }
             __syncthreads();
         }
@@ -348,10 +357,10 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseArgs a) {
     }
 }
 
-template <int TYPE, bool SLOTS>
+template <int TYPE, bool RULES>
 cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
-    cudaError_t e = op_allow(choose_kernel<TYPE, SLOTS>, kSlotBytes + (int)(kMaxTile / 4), true, done);
+    cudaError_t e = op_allow(choose_kernel<TYPE, RULES>, kSlotBytes + (int)(kMaxTile / 32 + 1) * 12, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(parts, rows);
@@ -364,7 +373,7 @@ cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem,
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, SLOTS>, a);
+    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, RULES>, a);
 }
 
 }  // namespace
@@ -393,7 +402,7 @@ extern "C" MGB_API mgb_status mgb_logits_choose(const void *logits, int type, in
     if (r.allow && (uint64_t)r.allow_stride * 32 < vocab) return op_fail(MGB_ERR_INVALID, op, "grammar rows are too short");
     if (!r.repetition && !r.frequency && !r.presence) r.history = nullptr;
     if (!r.history) r.history_stride = 0;
-    const bool slots = r.history_stride || r.bias_count;
+    const bool ruled = r.history_stride || r.bias_count || r.allow;
 
     // A row is cut over 16 CTAs (the largest cluster) while that many do not
     // yet fill the GPU's 148 SMs twice, over fewer for more rows, and never
@@ -406,13 +415,13 @@ extern "C" MGB_API mgb_status mgb_logits_choose(const void *logits, int type, in
     auto cap = [&] { return (uint32_t)(entries < a.tile ? entries : a.tile); };
     while ((uint64_t)cap() * 12 > (uint64_t)kSlotBytes) a.tile = (a.tile / 2 + 63) & ~63u;
     a.cap = cap();
-    const int smem = slots ? (int)(a.tile / 32 * 8 + a.cap * 12) : 0;
+    const int smem = ruled ? (int)((a.tile / 32 + 1) * 12 + a.cap * 12) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     switch (type) {
-        case MGB_F32: e = slots ? launch<MGB_F32, true>(a, rows, parts, smem, s) : launch<MGB_F32, false>(a, rows, parts, smem, s); break;
-        case MGB_F16: e = slots ? launch<MGB_F16, true>(a, rows, parts, smem, s) : launch<MGB_F16, false>(a, rows, parts, smem, s); break;
-        default: e = slots ? launch<MGB_BF16, true>(a, rows, parts, smem, s) : launch<MGB_BF16, false>(a, rows, parts, smem, s); break;
+        case MGB_F32: e = ruled ? launch<MGB_F32, true>(a, rows, parts, smem, s) : launch<MGB_F32, false>(a, rows, parts, smem, s); break;
+        case MGB_F16: e = ruled ? launch<MGB_F16, true>(a, rows, parts, smem, s) : launch<MGB_F16, false>(a, rows, parts, smem, s); break;
+        default: e = ruled ? launch<MGB_BF16, true>(a, rows, parts, smem, s) : launch<MGB_BF16, false>(a, rows, parts, smem, s); break;
     }
     return op_launch_status(e, op);
 }

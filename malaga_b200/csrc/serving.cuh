@@ -92,6 +92,8 @@ inline const char *check_kv(const mgb_kv *kv) {
     if (kv->format != MGB_KV_F16 && kv->format != MGB_KV_Q8) return "unknown cache format";
     if (kv->format == MGB_KV_Q8 && (!kv->k_scale || !kv->v_scale)) return "an 8-bit cache needs its scales";
     if (((uintptr_t)kv->k | (uintptr_t)kv->v) & 15) return "the cache must be 16-byte aligned";
+    if (kv->format == MGB_KV_Q8 && (((uintptr_t)kv->k_scale | (uintptr_t)kv->v_scale) & 15))
+        return "the cache's scales must be 16-byte aligned";
     if (kv->dim != 16 && kv->dim != 32 && kv->dim != 64 && kv->dim != 128) return "head dim must be 16, 32, 64 or 128";
     if (!power_of_two(kv->page) || kv->page < 16 || kv->page > 1024) return "page must be a power of two from 16 to 1024";
     if (kv->heads == 0 || kv->heads > 65535 || kv->pages == 0 || kv->pages > 0x7fffffffu) return "heads or pages out of range";
@@ -129,33 +131,7 @@ inline uint64_t bound_len(const mgb_kv_seqs &s, uint32_t page) {
 }
 
 // ---------------------------------------------------------------------------
-// Eight numbers of a row as f32, and back
-
-// `vec`: the address is a multiple of the vector's size.
-__device__ __forceinline__ void load8(const void *base, size_t at, int type, bool vec, float (&x)[8]) {
-    if (type == MGB_F32) {
-        const float *p = reinterpret_cast<const float *>(base) + at;
-        if (vec) {
-            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p[i];
-        }
-        return;
-    }
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + at;
-    uint16_t h[8];
-    if (vec) {
-        *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = type == MGB_F16 ? __half2float(__ushort_as_half(h[i])) : __uint_as_float((uint32_t)h[i] << 16);
-}
+// Numbers of a row as f32, and back
 
 __device__ __forceinline__ uint16_t to_16(float x, int type) {
     return type == MGB_F16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
@@ -172,36 +148,49 @@ __device__ __forceinline__ void store1(void *base, size_t at, int type, float x)
     else reinterpret_cast<uint16_t *>(base)[at] = to_16(x, type);
 }
 
-__device__ __forceinline__ void store8(void *base, size_t at, int type, bool vec, const float (&x)[8]) {
-    if (type == MGB_F32) {
-        float *p = reinterpret_cast<float *>(base) + at;
-        if (vec) {
-            *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
+// Four numbers; `vec`: their address is a multiple of their size.
+__device__ __forceinline__ void load4(const void *base, int64_t at, int type, bool vec, float *x) {
+    if (!vec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = x[i];
-        }
-        return;
-    }
-    uint16_t *p = reinterpret_cast<uint16_t *>(base) + at;
-    uint16_t h[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = to_16(x[i], type);
-    if (vec) {
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
+        for (int i = 0; i < 4; ++i) x[i] = load1(base, (size_t)(at + i), type);
+    } else if (type == MGB_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
     } else {
+        const uint2 a = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(base) + at);
+        const uint32_t w[2] = {a.x, a.y};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = h[i];
+        for (int i = 0; i < 2; ++i) {
+            if (type == MGB_F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store4(void *base, int64_t at, int type, bool vec, const float *x) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store1(base, (size_t)(at + i), type, x[i]);
+    } else if (type == MGB_F32) {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(base) + at) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        uint16_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = to_16(x[i], type);
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(base) + at) =
+            make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
     }
 }
 
 inline size_t type_size(int type) { return type == MGB_F32 ? 4 : 2; }
 
-// Whether every eighth number of the rows is a 16-byte boundary.
+// Whether every fourth number of the rows stands at a multiple of four numbers' size.
 inline bool rows_vec(const mgb_rows &r) {
-    const int64_t unit = 16 / (int64_t)type_size(r.type);
-    return ((uintptr_t)r.data & 15) == 0 && r.token_stride % unit == 0 && r.head_stride % unit == 0;
+    return ((uintptr_t)r.data & (4 * type_size(r.type) - 1)) == 0 && r.token_stride % 4 == 0 && r.head_stride % 4 == 0;
 }
 
 }  // namespace mgb
