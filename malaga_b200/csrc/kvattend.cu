@@ -19,6 +19,7 @@
 //    products each, which keeps 22 bits.
 #include <cooperative_groups.h>
 
+#include "numerics.cuh"
 #include "serving.cuh"
 #include "sync.cuh"
 
@@ -35,7 +36,9 @@ struct AttendArgs {
     void *out;
     long long q_token, q_head, o_token, o_head;
     int q_type, o_type, causal;
+    bool o_vec;
     uint32_t group;  // query heads of a cache head
+    uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
 };
 
@@ -117,6 +120,8 @@ struct Frag {
     static constexpr int VN = D * ESZ / 8 / VB;
     static constexpr int KW = D * ESZ / 16, VW = D * ESZ / 32 ? D * ESZ / 32 : 1;  // words of a key and lane
     static constexpr int STEPS = D / 16;
+    static constexpr int CTAS = D == 128 ? 4 : 5;  // of an SM, with tiles of 8 rows
+    static constexpr int STATIC = 32 * D + 512;  // static shared memory of a CTA a tile of 8 rows, at most
     // dim of element e of lane t's part of a K row, of lane g's part of a V row
     static __device__ __forceinline__ int k_dim(int t, int e) {
         constexpr int VE = KB / ESZ;
@@ -128,6 +133,7 @@ struct Frag {
     }
 };
 
+constexpr int kFewRows = 64;
 constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
 constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
 constexpr float kRaise = 7.0f;  // p is held as 2^7 p, up to 2^15
@@ -137,8 +143,9 @@ template <int D, bool Q8>
 struct Ring {
     static constexpr int ROWS = 16 * D * (Q8 ? 1 : 2), SCALES = Q8 ? 64 : 0;
     static constexpr int STAGE = 2 * ROWS + 2 * SCALES;
-    static constexpr int FIT = 16384 / STAGE;  // about 16 KB a warp in flight, at most 8 stages
-    static constexpr int N = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;
+    // about 12 KB a warp, 2 to 4 stages: more would cost CTAs of an SM
+    static constexpr int FIT = 12800 / STAGE;
+    static constexpr int N = FIT < 2 ? 2 : FIT > 4 ? 4 : FIT;
     static constexpr int BYTES = kRowWarps * N * STAGE;
 };
 
@@ -333,7 +340,7 @@ struct Rows {
 };
 
 template <int D, bool Q8, bool SPLIT, int NT>
-__global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)) attend_rows_kernel(const AttendArgs a) {
     using F = Frag<D, Q8>;
     constexpr int R = 8 * NT, PER_ROW = kRowThreads / R, E = D / PER_ROW;
     static_assert(E >= 1, "at most one thread a number");
@@ -354,10 +361,17 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const long long rows = (long long)n * a.group;
+    if (rows > a.few) return;
     if (lane < RG::N) mbar_init(&full[warp][lane], 1);
     __syncwarp();
     uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
-    uint32_t taken = 0;  // blocks of this warp so far, over all tiles
+    uint32_t put = 0, get = 0, phase = 0;  // next stage to fill and to read, and its barrier's parity
+    const uint32_t page_mask = (1u << a.kv.page_log2) - 1;
+    const bool scales = lane & 2;
+    const uint8_t *my_base = static_cast<const uint8_t *>(scales ? (lane & 1 ? (void *)a.kv.vs : (void *)a.kv.ks)
+                                                                 : (lane & 1 ? a.kv.v : a.kv.k));
+    const uint32_t my_row = scales ? 4 : D * F::ESZ, my_bytes = scales ? RG::SCALES : RG::ROWS;
+    const uint32_t my_offset = (scales ? 2 * RG::ROWS : 0) + (lane & 1) * my_bytes;
     // keys that token i sees
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 
@@ -374,25 +388,19 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                 pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u;
             }
             const uint32_t page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const bool there = page < a.kv.pages;
+            uint64_t *bar = &full[warp][put];
             if (lane == 0) {
-                const uint32_t st = (taken + i) % RG::N;
-                uint8_t *at = ring + st * RG::STAGE;
-                const int key0 = (first + warp + i * kRowWarps) * 16;
-                const bool there = page < a.kv.pages;
-                have[warp][st] = there;
-                if (there) {
-                    const size_t row = a.kv.row(page, head, (uint32_t)key0 & ((1u << a.kv.page_log2) - 1));
-                    mbar_expect_tx(&full[warp][st], RG::STAGE);
-                    bulk_g2s(at, static_cast<const uint8_t *>(a.kv.k) + row * (D * F::ESZ), RG::ROWS, &full[warp][st]);
-                    bulk_g2s(at + RG::ROWS, static_cast<const uint8_t *>(a.kv.v) + row * (D * F::ESZ), RG::ROWS, &full[warp][st]);
-                    if constexpr (Q8) {
-                        bulk_g2s(at + 2 * RG::ROWS, a.kv.ks + row, RG::SCALES, &full[warp][st]);
-                        bulk_g2s(at + 2 * RG::ROWS + RG::SCALES, a.kv.vs + row, RG::SCALES, &full[warp][st]);
-                    }
-                } else {
-                    mbar_arrive_cta(&full[warp][st]);
-                }
+                have[warp][put] = there;
+                if (there) mbar_expect_tx(bar, RG::STAGE);
+                else mbar_arrive_cta(bar);
             }
+            __syncwarp();
+            if (lane < (Q8 ? 4 : 2) && there) {  // lane 0 copies K, 1 V, 2 and 3 their scales
+                const size_t row = a.kv.row(page, head, (uint32_t)((first + warp + i * kRowWarps) * 16) & page_mask);
+                bulk_g2s(ring + put * RG::STAGE + my_offset, my_base + row * my_row, my_bytes, bar);
+            }
+            put = put + 1 == RG::N ? 0 : put + 1;
         };
         for (int i = 0; i < min(mine, RG::N); ++i) issue(i);
 
@@ -457,16 +465,15 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
 
         bool lost = false;  // a copy did not arrive in time: the rows become NaN
         for (int i = 0; i < mine; ++i) {
-            const uint32_t st_no = (taken + i) % RG::N;
-            lost |= !mbar_wait(&full[warp][st_no], ((taken + i) / RG::N) & 1);
-            if (have[warp][st_no]) {
+            lost |= !mbar_wait(&full[warp][get], phase);
+            if (have[warp][get]) {
                 Block<D, Q8> x;
-                st.step(x, ring + st_no * RG::STAGE, (first + warp + i * kRowWarps) * 16, end, g, t);
+                st.step(x, ring + get * RG::STAGE, (first + warp + i * kRowWarps) * 16, end, g, t);
             }
             __syncwarp();  // every lane has read the stage
             if (i + RG::N < mine) issue(i + RG::N);
+            if (++get == RG::N) get = 0, phase ^= 1;
         }
-        taken += mine;
         if (lost) st.l[0][0] = st.l[0][1] = st.l[NT - 1][0] = st.l[NT - 1][1] = __int_as_float(0x7fffffff);
 
         // the CTA's warps
@@ -569,20 +576,28 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
     return cudaLaunchKernelEx(&c, attend_rows_kernel<D, Q8, SPLIT, NT>, a);
 }
 
-// 8-row tiles where a call has no more rows a cache head than that, else 16.
-// Keys are cut over more CTAs of a cluster while the GPU (148 SMs, about three
-// CTAs each) is not full and every CTA keeps two blocks a warp.
-template <int D, bool Q8, bool SPLIT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
-    const uint64_t rows = most_new * a.group;
-    const int r = rows <= 8 ? 8 : 16;
-    uint64_t tiles = (rows + r - 1) / r;
+// Keys are cut over the CTAs of a cluster (at most 16) while all CTAs still run
+// at once and every warp keeps two blocks, and further while a CTA would have
+// more than 2048 keys: sequences of unlike lengths then even out.
+template <int D, bool Q8, bool SPLIT, int NT>
+cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
+    constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, PER_SM = 227 * 1024 / SMEM;
+    constexpr int SLOTS = 148 * (PER_SM < 4 ? PER_SM : 4);
+    uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
     if (tiles * a.kv.heads > 65535) tiles = 65535 / a.kv.heads;
     const uint64_t base = tiles * a.kv.heads * a.seq.seqs;
     uint32_t parts = 1;
-    while (parts < 16 && base * parts < 3 * 148 && most_len / (parts * 2) >= kRowWarps * 32) parts *= 2;
-    const dim3 grid(parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs);
-    return r == 8 ? launch_rows<D, Q8, SPLIT, 1>(a, grid, s) : launch_rows<D, Q8, SPLIT, 2>(a, grid, s);
+    while (parts < 16 && most_len / (parts * 2) >= kRowWarps * 32 &&
+           (base * parts * 2 <= SLOTS || most_len / parts > 2048))
+        parts *= 2;
+    return launch_rows<D, Q8, SPLIT, NT>(a, dim3(parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
+}
+
+// 8-row tiles where a call has no more rows a cache head than that, else 16.
+template <int D, bool Q8, bool SPLIT>
+cudaError_t launch_rows(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+    const uint64_t rows = most_new * a.group;
+    return rows <= 8 ? launch_rows<D, Q8, SPLIT, 1>(a, rows, most_len, s) : launch_rows<D, Q8, SPLIT, 2>(a, rows, most_len, s);
 }
 
 template <int D>
@@ -590,6 +605,48 @@ cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t most_new, uint64_
     if (a.q_type == MGB_F32)
         return q8 ? launch_rows<D, true, true>(a, most_new, most_len, s) : launch_rows<D, false, true>(a, most_new, most_len, s);
     return q8 ? launch_rows<D, true, false>(a, most_new, most_len, s) : launch_rows<D, false, false>(a, most_new, most_len, s);
+}
+
+#include "attend_tiles.cuh"
+
+// A row tile's keys are cut over the CTAs of a cluster (at most 8) while that
+// fills SMs that would stay idle (one CTA an SM, 148 SMs) and leaves each CTA
+// four key tiles.
+template <int D, bool Q8>
+cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+    static std::atomic<bool> done[kMaxDevices];
+    cudaError_t e = op_allow(tiles::attend_tiles_kernel<D, Q8>, tiles::Smem<D>::ASKED, false, done);
+    if (e != cudaSuccess) return e;
+    uint64_t row_tiles = (most_new * a.group + 255) / 256;
+    if (row_tiles * a.kv.heads > 65535) row_tiles = 65535 / a.kv.heads;
+    const uint64_t base = row_tiles * a.kv.heads * a.seq.seqs;
+    uint32_t parts = 1;
+    while (parts < 8 && base * parts * 2 <= 148 && most_len / (parts * 2) >= 4 * tiles::kKeys) parts *= 2;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(parts, (unsigned)(row_tiles * a.kv.heads), a.seq.seqs);
+    c.blockDim = dim3(tiles::kThreads);
+    c.dynamicSmemBytes = tiles::Smem<D>::ASKED;
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, tiles::attend_tiles_kernel<D, Q8>, a);
+}
+
+template <int D>
+cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+    // Sequences of more than 64 rows a cache head go to the tensor-core tiles, but
+    // for f32 queries, whose two f16 parts only the other kernel takes.
+    if (a.q_type == MGB_F32 || most_new * a.group <= kFewRows) return launch_rows<D>(a, q8, most_new, most_len, s);
+    a.few = kFewRows;
+    cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
+    // sequences of unlike lengths: there may be some of few rows
+    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs)
+        e = launch_rows<D>(a, q8, (kFewRows + a.group - 1) / a.group, most_len, s);
+    return e;
 }
 
 }  // namespace
@@ -608,17 +665,17 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
     if (seqs->seqs == 0 || q->tokens == 0) return MGB_OK;
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
-                 out->token_stride, out->head_stride, q->type, out->type, causal != 0, q->heads / kv->heads,
-                 scale * kLog2e};
+                 out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), q->heads / kv->heads,
+                 0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
     cudaError_t e;
     switch (kv->dim) {
-        case 16: e = launch_rows<16>(a, q8, most_new, most_len, s); break;
-        case 32: e = launch_rows<32>(a, q8, most_new, most_len, s); break;
-        case 64: e = launch_rows<64>(a, q8, most_new, most_len, s); break;
-        default: e = launch_rows<128>(a, q8, most_new, most_len, s); break;
+        case 16: e = launch<16>(a, q8, most_new, most_len, s); break;
+        case 32: e = launch<32>(a, q8, most_new, most_len, s); break;
+        case 64: e = launch<64>(a, q8, most_new, most_len, s); break;
+        default: e = launch<128>(a, q8, most_new, most_len, s); break;
     }
     return op_launch_status(e, op);
 }

@@ -19,31 +19,44 @@ constexpr int kMaxTokens = 16;  // tokens of a CTA
 #define kInf __int_as_float(0x7f800000)
 #define kNan __int_as_float(0x7fffffff)
 
+struct Side {  // K or V: its packed rows and its half of the cache
+    void *rows;
+    long long token_stride, head_stride;  // in numbers
+    uint8_t *data;
+    float *scale;
+};
+
 struct MoveArgs {
     KvView kv;
     SeqView seq;
-    void *k, *v;
-    long long k_token, k_head, v_token, v_head;  // strides in numbers
-    int k_type, v_type;
-    bool k_vec, v_vec;
+    Side side[2];
     uint32_t per_cta;  // tokens of a CTA
 };
 
-// Code bytes of x / d for four numbers. x * (1 / d) is within 2^-15 of the f32
+// Code bytes of x / d for eight numbers. x * (1 / d) is within 2^-15 of the f32
 // quotient (|x / d| <= 127), so it rounds to the same whole number unless it
-// lies that near a half; then the quotient itself is taken. Adding 1.5 * 2^23
-// rounds to a whole number, halves to even, and leaves it in the low bits.
-__device__ __forceinline__ uint32_t codes_of(const float *x, float d, float inv, bool tiny) {
+// lies that near a half; then the quotients themselves are taken. Adding
+// 1.5 * 2^23 rounds to a whole number, halves to even, and leaves it in the low
+// bits.
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float d) {
     constexpr float kWhole = 12582912.0f;
-    uint32_t r[4];
+    const bool tiny = !(d > 1e-30f);  // 1 / d would leave f32's range, or there is no d
+    const float inv = __frcp_rn(d);
+    uint32_t r[8];
+    float far = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
         const float q = x[e] * inv, w = q + kWhole;
         r[e] = __float_as_uint(w);
-        if (tiny || fabsf(q - (w - kWhole)) > 0.4999f)
+        far = fmaxf(far, fabsf(q - (w - kWhole)));
+    }
+    if (tiny || far > 0.4999f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
             r[e] = d > 0.0f ? __float_as_uint(fminf(fmaxf(__fdiv_rn(x[e], d), -127.0f), 127.0f) + kWhole) : 0u;
     }
-    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    return make_uint2(__byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410));
 }
 
 // Four code bytes as f32: the bytes 00 00 4b above u are the number 2^23 + u.
@@ -53,7 +66,7 @@ __device__ __forceinline__ void values_of(uint32_t codes, float d, float *x) {
     for (int e = 0; e < 4; ++e) x[e] = d * (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + e)) - 8388736.0f);
 }
 
-template <int DIM, bool Q8, bool WRITE>
+template <int DIM, bool Q8, bool WRITE, int TYPE, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     constexpr int LANES = DIM / 8, ROWS = kThreads / LANES;
     __shared__ int64_t place[kMaxTokens];  // row of head 0 in the cache, -1 where there is none
@@ -80,16 +93,13 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     }
     __syncthreads();
 
-    const bool is_v = blockIdx.y;
-    void *rows = is_v ? a.v : a.k;
-    const long long token_stride = is_v ? a.v_token : a.k_token, head_stride = is_v ? a.v_head : a.k_head;
-    const int type = is_v ? a.v_type : a.k_type;
-    const bool vec = is_v ? a.v_vec : a.k_vec;
-    uint8_t *data = static_cast<uint8_t *>(is_v ? a.kv.v : a.kv.k);
-    float *scale = is_v ? a.kv.vs : a.kv.ks;
+    const Side &side = a.side[blockIdx.y];
+    void *rows = side.rows;
+    uint8_t *data = side.data;
+    float *scale = side.scale;
     // a lane's two pieces of four numbers: apart for 32-bit rows, side by side for 16-bit ones
     const int lane = threadIdx.x % LANES;
-    const int p0 = type == MGB_F32 ? 4 * lane : 8 * lane, p1 = type == MGB_F32 ? DIM / 2 + 4 * lane : 8 * lane + 4;
+    const int p0 = TYPE == MGB_F32 ? 4 * lane : 8 * lane, p1 = TYPE == MGB_F32 ? DIM / 2 + 4 * lane : 8 * lane + 4;
     const uint32_t heads = a.kv.heads, total = tokens * heads;
 
     for (uint32_t r0 = 0; r0 < total; r0 += ROWS * kBatch) {
@@ -100,13 +110,13 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
             const uint32_t r = r0 + u * ROWS + threadIdx.x / LANES, i = r / heads, h = r - i * heads;
             row[u] = r < total ? place[i] : -2;  // -2: no such row
             if (row[u] >= 0) row[u] += (int64_t)h << a.kv.page_log2;
-            at[u] = (int64_t)(first + i) * token_stride + (int64_t)h * head_stride;
+            at[u] = (int64_t)(first + i) * side.token_stride + (int64_t)h * side.head_stride;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
             if (row[u] < 0) continue;
             if constexpr (WRITE) {
-                load4(rows, at[u] + p0, type, vec, &x[u][0]);
-                load4(rows, at[u] + p1, type, vec, &x[u][4]);
+                load4(rows, at[u] + p0, TYPE, VEC, &x[u][0]);
+                load4(rows, at[u] + p1, TYPE, VEC, &x[u][4]);
             } else if constexpr (Q8) {
                 const uint8_t *c = data + row[u] * DIM;
                 const float d = scale[row[u]];
@@ -121,8 +131,8 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
         for (int u = 0; u < kBatch; ++u) {
             if constexpr (!WRITE) {
                 if (row[u] == -2) continue;
-                store4(rows, at[u] + p0, type, vec, &x[u][0]);
-                store4(rows, at[u] + p1, type, vec, &x[u][4]);
+                store4(rows, at[u] + p0, TYPE, VEC, &x[u][0]);
+                store4(rows, at[u] + p1, TYPE, VEC, &x[u][4]);
             } else if constexpr (Q8) {
                 float m = 0.0f;
 #pragma unroll
@@ -130,13 +140,11 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                 const float d = m == kInf ? kNan : __fdiv_rn(m, 127.0f);
-                const bool tiny = !(d > 1e-30f);  // 1 / d would leave f32's range, or there is no d
-                const float inv = tiny ? 0.0f : __frcp_rn(d);
-                const uint32_t c0 = codes_of(&x[u][0], d, inv, tiny), c1 = codes_of(&x[u][4], d, inv, tiny);
+                const uint2 code = codes_of(x[u], d);
                 if (row[u] >= 0) {
                     uint8_t *c = data + row[u] * DIM;
-                    *reinterpret_cast<uint32_t *>(c + p0) = c0;
-                    *reinterpret_cast<uint32_t *>(c + p1) = c1;
+                    *reinterpret_cast<uint32_t *>(c + p0) = code.x;
+                    *reinterpret_cast<uint32_t *>(c + p1) = code.y;
                     if (lane == 0) scale[row[u]] = d;
                 }
             } else if (row[u] >= 0) {
@@ -147,13 +155,28 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     }
 }
 
-// As many tokens a CTA as leave four CTAs an SM (148 SMs), at most kMaxTokens.
+// As many tokens a CTA as leave two CTAs an SM (148 SMs) on either side, at
+// most kMaxTokens.
 template <int DIM, bool Q8, bool WRITE>
-cudaError_t launch(MoveArgs a, cudaStream_t s) {
+cudaError_t launch(MoveArgs a, int sides, int type, bool vec, cudaStream_t s) {
     const uint32_t n = a.seq.tokens / (2 * 148);
     a.per_cta = n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n;
-    kv_move_kernel<DIM, Q8, WRITE><<<dim3((a.seq.tokens + a.per_cta - 1) / a.per_cta, 2), kThreads, 0, s>>>(a);
+    const dim3 grid((a.seq.tokens + a.per_cta - 1) / a.per_cta, sides);
+    auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a); };
+    if (type == MGB_F32) vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, false>);
+    else if (type == MGB_F16) vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, false>);
+    else vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, false>);
     return cudaGetLastError();
+}
+
+template <bool WRITE>
+cudaError_t launch(const MoveArgs &a, int sides, bool q8, int type, bool vec, cudaStream_t s) {
+    switch (a.kv.dim) {
+        case 16: return q8 ? launch<16, true, WRITE>(a, sides, type, vec, s) : launch<16, false, WRITE>(a, sides, type, vec, s);
+        case 32: return q8 ? launch<32, true, WRITE>(a, sides, type, vec, s) : launch<32, false, WRITE>(a, sides, type, vec, s);
+        case 64: return q8 ? launch<64, true, WRITE>(a, sides, type, vec, s) : launch<64, false, WRITE>(a, sides, type, vec, s);
+        default: return q8 ? launch<128, true, WRITE>(a, sides, type, vec, s) : launch<128, false, WRITE>(a, sides, type, vec, s);
+    }
 }
 
 template <bool WRITE>
@@ -167,17 +190,17 @@ mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, co
     if (!bad && (k->heads != kv->heads || v->heads != kv->heads)) bad = "the rows' heads are not the cache's";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
     if (seqs->seqs == 0 || k->tokens == 0) return MGB_OK;
-    MoveArgs a{view(*kv), view(*seqs, k->tokens), k->data, v->data, k->token_stride, k->head_stride,
-               v->token_stride, v->head_stride, k->type, v->type, rows_vec(*k), rows_vec(*v), 0};
+    MoveArgs a{view(*kv), view(*seqs, k->tokens),
+               {{k->data, k->token_stride, k->head_stride, static_cast<uint8_t *>(kv->k), kv->k_scale},
+                {v->data, v->token_stride, v->head_stride, static_cast<uint8_t *>(kv->v), kv->v_scale}},
+               0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
-    cudaError_t e;
-    switch (kv->dim) {
-        case 16: e = q8 ? launch<16, true, WRITE>(a, s) : launch<16, false, WRITE>(a, s); break;
-        case 32: e = q8 ? launch<32, true, WRITE>(a, s) : launch<32, false, WRITE>(a, s); break;
-        case 64: e = q8 ? launch<64, true, WRITE>(a, s) : launch<64, false, WRITE>(a, s); break;
-        default: e = q8 ? launch<128, true, WRITE>(a, s) : launch<128, false, WRITE>(a, s); break;
-    }
+    if (k->type == v->type) return op_launch_status(launch<WRITE>(a, 2, q8, k->type, rows_vec(*k) && rows_vec(*v), s), op);
+    // rows of two types: a launch each
+    cudaError_t e = launch<WRITE>(a, 1, q8, k->type, rows_vec(*k), s);
+    a.side[0] = a.side[1];
+    if (e == cudaSuccess) e = launch<WRITE>(a, 1, q8, v->type, rows_vec(*v), s);
     return op_launch_status(e, op);
 }
 

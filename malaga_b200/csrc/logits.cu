@@ -19,9 +19,10 @@
 namespace mgb {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxTile = 32768;  // tokens of one bitmap
 constexpr int kSlotBytes = 96 * 1024;  // shared memory for slots at most
+constexpr int kPer = (kMaxTile / 32 + kThreads) / kThreads;  // words of a bit map a thread
 constexpr uint32_t kNone = 0xffffffffu;
 
 #define kPosInf __int_as_float(0x7f800000)
@@ -129,7 +130,7 @@ __device__ __forceinline__ uint32_t bits_at(const uint32_t *row, uint32_t words,
 }
 
 template <int TYPE, bool RULES>
-__global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a) {
     using N = Num<TYPE>;
     using T = typename N::T;
     constexpr int W = 16 / sizeof(T), UNROLL = 16 / W;
@@ -179,6 +180,19 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a)
     for (uint32_t v0 = c0; v0 < c1; v0 += a.tile) {
         const uint32_t v1 = min(c1, v0 + a.tile), width = v1 - v0;
         const uint32_t shift = (uint32_t)(((uintptr_t)(x + v0) & 15) / sizeof(T));
+        // vectors from the 16-byte boundary at or before v0; all but the first and last are whole
+        const uint4 *vectors = reinterpret_cast<const uint4 *>(x + v0 - shift);
+        const uint32_t nvec = (width + shift + W - 1) / W;
+        const uint32_t whole0 = shift ? 1 : 0, whole1 = (width + shift) / W;
+        uint4 raw[UNROLL];
+        auto fetch = [&](uint32_t j0) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t j = j0 + u * kThreads;
+                if (j >= whole0 && j < whole1) raw[u] = __ldcs(vectors + j);
+            }
+        };
+        fetch(tid);  // on their way while the bit maps are built
         uint32_t slots = 0;
         if constexpr (RULES) {
             for (uint32_t w = tid; w < words; w += kThreads) {
@@ -194,11 +208,11 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a)
                 for (uint32_t i = tid; i < nh; i += kThreads) touch(hist[i]);
                 for (uint32_t i = tid; i < r.bias_count; i += kThreads) touch(bias_ids[i]);
                 __syncthreads();
-                // rank[w]: touched tokens before word w; a thread has four words
-                uint32_t pop[4], upto = 0;
+                // rank[w]: touched tokens before word w; a thread has kPer words
+                uint32_t pop[kPer], upto = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    pop[e] = 4 * tid + e < words ? __popc(mark[4 * tid + e]) : 0;
+                for (int e = 0; e < kPer; ++e) {
+                    pop[e] = kPer * tid + e < words ? __popc(mark[kPer * tid + e]) : 0;
                     upto += pop[e];
                 }
                 const uint32_t mine = upto;
@@ -216,8 +230,8 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a)
                     slots += warp_sum[k];
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (4 * tid + e < words) rank[4 * tid + e] = before;
+                for (int e = 0; e < kPer; ++e) {
+                    if (kPer * tid + e < words) rank[kPer * tid + e] = before;
                     before += pop[e];
                 }
                 for (uint32_t k = tid; k < slots; k += kThreads) {
@@ -252,18 +266,10 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a)
             }
         }
 
-        // streaming pass: vectors from the 16-byte boundary at or before v0; all but the first and last are whole
-        const uint4 *vectors = reinterpret_cast<const uint4 *>(x + v0 - shift);
+        // streaming pass
         const bool y_vec = y && (((uintptr_t)(y + v0) & 15) / sizeof(T)) == shift;
-        const uint32_t nvec = (width + shift + W - 1) / W;
-        const uint32_t whole0 = shift ? 1 : 0, whole1 = (width + shift) / W;
         for (uint32_t j0 = tid; j0 < nvec; j0 += kThreads * UNROLL) {
-            uint4 raw[UNROLL];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                const uint32_t j = j0 + u * kThreads;
-                if (j >= whole0 && j < whole1) raw[u] = __ldcs(vectors + j);
-            }
+            if (j0 != tid) fetch(j0);
             float f[UNROLL * W];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
@@ -353,7 +359,8 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(const ChooseArgs a)
     if (tid == 0) {
         const bool found = best.i != kNone;
         if (a.ids) a.ids[row] = found ? (int32_t)best.i : -1;
-        if (a.logp) a.logp[row] = found ? -log1pf(best.l) : kLowest;
+        // a sum below 2^-53 does not move 1 even in 64 bits
+        if (a.logp) a.logp[row] = found ? (best.l < 1.1102230246251565e-16f ? 0.0f : -log1pf(best.l)) : kLowest;
     }
 }
 
@@ -404,11 +411,11 @@ extern "C" MGB_API mgb_status mgb_logits_choose(const void *logits, int type, in
     if (!r.history) r.history_stride = 0;
     const bool ruled = r.history_stride || r.bias_count || r.allow;
 
-    // A row is cut over 16 CTAs (the largest cluster) while that many do not
-    // yet fill the GPU's 148 SMs twice, over fewer for more rows, and never
-    // into shares below 2048 tokens.
+    // A row is cut over 16 CTAs (the largest cluster), over fewer where they
+    // would not all run at once (four an SM, 148 SMs), and never into shares
+    // below 2048 tokens.
     uint32_t parts = 16;
-    while (parts > 1 && (rows * parts > 4 * 148 || (uint64_t)parts * 2048 > vocab + 2047ull)) parts /= 2;
+    while (parts > 1 && ((uint64_t)rows * parts > 4 * 148 || (uint64_t)parts * 2048 > vocab + 2047ull)) parts /= 2;
     const uint32_t share = ((vocab + parts - 1) / parts + 63) & ~63u;
     a.tile = share < kMaxTile ? share : kMaxTile;
     const uint64_t entries = (uint64_t)r.history_stride + r.bias_count;
