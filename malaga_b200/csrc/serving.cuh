@@ -193,4 +193,9 @@ inline bool rows_vec(const mgb_rows &r) {
     return ((uintptr_t)r.data & (4 * type_size(r.type) - 1)) == 0 && r.token_stride % 4 == 0 && r.head_stride % 4 == 0;
 }
 
+// Whether they are 16-bit numbers, and every eighth stands at a multiple of 16 bytes.
+inline bool rows_vec16(const mgb_rows &r) {
+    return r.type != MGB_F32 && ((uintptr_t)r.data & 15) == 0 && r.token_stride % 8 == 0 && r.head_stride % 8 == 0;
+}
+
 }  // namespace mgb
