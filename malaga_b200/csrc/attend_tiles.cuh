@@ -7,15 +7,20 @@
 // stay in tensor memory: P (f16) takes the place of the S it came from and is
 // the A operand of O += P V, O is only rescaled when a row's maximum passes the
 // one in use by 2^8. Warps 8-11 bring keys and values of the pages into shared
-// memory as f16, up to two tiles of 128 keys ahead; warp 12 issues the products.
+// memory as f16, up to two tiles of 128 keys ahead. Warp 12 issues the products of whichever row tile
+// is ready first, all of a step's at once: the tiles then settle half a step
+// apart (with a warp each they ran in step and shared every unit at the same
+// time).
 // Registers go where a whole row of scores is held (setmaxnreg). Operands lie
 // in the K-major layout without swizzle: 8 rows x 16 bytes are one 128-byte
 // block, so a warp's 16-byte stores cover whole blocks; V is read from the same
 // layout as the transposed operand.
 //
-// 8-bit caches: K's codes are exact in f16 and their scales multiply S; V's
-// scales (over the running exponent) multiply its codes as they are unpacked,
-// one rounding of the product to f16.
+// 8-bit caches: K's codes are exact in f16 and their scales multiply S (folding
+// them into K as it is unpacked was 4 % faster and made the error of f16
+// outputs 3.2e-4 -> 6.8e-4); V's scales, over the running exponent, multiply its
+// codes as they are unpacked, one rounding of the product to f16 (the scale
+// enters as a high and a low part).
 #pragma once
 
 namespace tiles {
@@ -129,10 +134,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Whether phase `parity` of the mbarrier is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+
 // What all roles of a CTA know of its row tile.
 struct Span {
-    long long r0;
-    int live, groups;  // rows of the tile; 128-row groups that have some
+    int r0, live, groups;  // its first row; rows of the tile; 128-row groups that have some
     int end, all;      // keys that its last row sees; keys that every row sees
     int first, count;  // its part's key tiles
 };
@@ -147,8 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
     int n;
     const int t0 = a.seq.first(b, n);
-    const long long rows = (long long)n * a.group;
-    if (rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
+    const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
+    if ((uint32_t)rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
@@ -162,8 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.k_full[i], kLoadWarps);
             mbar_init(&sh.v_full[i], kLoadWarps);
-            mbar_init(&sh.k_free[i], 1);
-            mbar_init(&sh.v_free[i], 1);
+            mbar_init(&sh.k_free[i], 2);
+            mbar_init(&sh.v_free[i], 2);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_full[i], kSoftWarps / 2);
         }
@@ -179,14 +193,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     // the row tiles with the most keys first
     auto span_of = [&](uint32_t rt) {
         Span s;
-        s.r0 = (long long)(row_tiles - 1 - rt) * 256;
-        s.live = (int)min(256ll, rows - s.r0);
+        s.r0 = (int)(row_tiles - 1 - rt) * 256;
+        s.live = min(256, rows - s.r0);
         s.groups = s.live > 128 ? 2 : 1;
-        s.end = limit((int)((s.r0 + s.live - 1) / a.group));
-        s.all = limit((int)(s.r0 / a.group));
+        s.end = limit((s.r0 + s.live - 1) / (int)a.group);
+        s.all = limit(s.r0 / (int)a.group);
         const int total = (s.end + kKeys - 1) / kKeys;
-        s.first = (int)((long long)total * part / parts);
-        s.count = (int)((long long)total * (part + 1) / parts) - s.first;
+        // parts is at most 8 and a tile 128 keys, so the products stay below 2^31
+        s.first = (int)((uint32_t)total * part / parts);
+        s.count = (int)((uint32_t)total * (part + 1) / parts) - s.first;
         if (*reinterpret_cast<volatile int *>(&sh.lost)) s.count = 0;  // every barrier is still met
         return s;
     };
@@ -219,32 +234,48 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             float scale = 0.0f;
             {
                 constexpr int PIECES = D / 8, PER = PIECES < 4 ? 1 : PIECES / 4;
-                float x[4][PER][8];
+                // all loads before any use, as the numbers' bits
+                uint4 raw[4][PER];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const long long rr = sp.r0 + 32 * warp + 8 * q + (lane & 7);
-                    const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
-                    const int64_t at = (t0 + i) * a.q_token + (long long)(head * a.group + h) * a.q_head;
+                    const int rr = sp.r0 + 32 * warp + 8 * q + (lane & 7);
+                    const int i = rr / (int)a.group, h = rr - i * (int)a.group;
+                    const uint16_t *from = static_cast<const uint16_t *>(a.q) + (t0 + i) * a.q_token + (long long)(head * a.group + h) * a.q_head;
 #pragma unroll
                     for (int u = 0; u < PER; ++u) {
                         const int c = (lane >> 3) + 4 * u;
+                        raw[q][u] = make_uint4(0, 0, 0, 0);
+                        if (rr >= rows || c >= PIECES) continue;
+                        if (a.q_vec16) {
+                            raw[q][u] = __ldg(reinterpret_cast<const uint4 *>(from + 8 * c));
+                        } else {
+                            uint16_t y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[q][u][e] = 0.0f;
-                        if (rr < rows && c < PIECES) {
-                            load4(a.q, at + 8 * c, a.q_type, a.q_vec, &x[q][u][0]);
-                            load4(a.q, at + 8 * c + 4, a.q_type, a.q_vec, &x[q][u][4]);
+                            for (int e = 0; e < 8; ++e) y[e] = from[8 * c + e];
+                            raw[q][u] = *reinterpret_cast<const uint4 *>(y);
                         }
                     }
                 }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
+                    float x[PER][8];
+#pragma unroll
+                    for (int u = 0; u < PER; ++u) {
+                        const uint32_t w[4] = {raw[q][u].x, raw[q][u].y, raw[q][u].z, raw[q][u].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = unpack(w[e]);
+                            x[u][2 * e] = a.q_type == MGB_F16 ? f.x : __uint_as_float(w[e] << 16);
+                            x[u][2 * e + 1] = a.q_type == MGB_F16 ? f.y : __uint_as_float(w[e] & 0xffff0000u);
+                        }
+                    }
                     int shift = 0;
                     if (a.q_type != MGB_F16) {
                         float m = 0.0f;
 #pragma unroll
                         for (int u = 0; u < PER; ++u)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[q][u][e]));
+                            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[u][e]));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                         if (m > 0.0f && m < __int_as_float(0x7f800000)) shift = 13 - ilogbf(m);
@@ -261,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         const int c = (lane >> 3) + 4 * u;
                         uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack(x[q][u][2 * e] * f1 * f2, x[q][u][2 * e + 1] * f1 * f2);
+                        for (int e = 0; e < 4; ++e) w[e] = pack(x[u][2 * e] * f1 * f2, x[u][2 * e + 1] * f1 * f2);
                         if (c < PIECES) *reinterpret_cast<uint4 *>(mine + piece<D>(8 * q + (lane & 7), c)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
@@ -270,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             __syncwarp();
             if (lane == 0) mbar_arrive_cta(&sh.q_full);
 
-            const int lim = row < sp.live ? limit((int)((sp.r0 + row) / a.group)) : 0;
+            const int lim = row < sp.live ? limit((sp.r0 + row) / (int)a.group) : 0;
             float m = kLowest, l = 0.0f;
             int exp_v = -126;
             bool ok = !sh.lost;
@@ -353,7 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             const float back = Q8 ? power_of_2(exp_v) : 1.0f;
             const bool has = count > 0;
             if (parts == 1) {
-                const float f = l == 0.0f ? 0.0f : back / l;
+                const bool some = has && !(l < 1e-30f);  // a row that sees nothing has at most 128 times 2^-126 a tile
+                const float f = some ? back / l : 0.0f;
                 if (a.o_vec16) {
                     // through the warp's rows of Q, which no product reads any more, to whole rows of 16-bit numbers
                     constexpr int PIECES = D / 8;
@@ -364,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         tmem_wait_load();
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
-                            const float u = has && l != 0.0f ? __uint_as_float(raw[2 * c]) * f : 0.0f;
-                            const float v = has && l != 0.0f ? __uint_as_float(raw[2 * c + 1]) * f : 0.0f;
+                            const float u = some ? __uint_as_float(raw[2 * c]) * f : 0.0f;
+                            const float v = some ? __uint_as_float(raw[2 * c + 1]) * f : 0.0f;
                             w[c] = to_16(ok ? u : l, a.o_type) | (uint32_t)to_16(ok ? v : l, a.o_type) << 16;
                         }
 #pragma unroll
@@ -376,16 +408,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 4
                     for (int u = lane; u < 32 * PIECES; u += 32) {
                         const int r = u / PIECES, c = u % PIECES;
-                        const long long rr = sp.r0 + 32 * warp + r;
+                        const int rr = sp.r0 + 32 * warp + r;
                         if (32 * warp + r >= sp.live) break;
-                        const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
+                        const int i = rr / (int)a.group, h = rr - i * (int)a.group;
                         const int64_t to = (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + 8 * c;
                         *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to) = *reinterpret_cast<const uint4 *>(mine + piece<D>(r, c));
                     }
                     __syncwarp();
                 } else {
-                    const long long rr = sp.r0 + row;
-                    const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
+                    const int rr = sp.r0 + row;
+                    const int i = rr / (int)a.group, h = rr - i * (int)a.group;
                     const int64_t to = (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head;
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
@@ -395,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         if (row >= sp.live) continue;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
-                            store1(a.out, (size_t)(to + c0 + c), a.o_type, !ok ? l : has && l != 0.0f ? __uint_as_float(raw[c]) * f : 0.0f);
+                            store1(a.out, (size_t)(to + c0 + c), a.o_type, !ok ? l : some ? __uint_as_float(raw[c]) * f : 0.0f);
                     }
                 }
             } else {
@@ -431,9 +463,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         for (int e = 0; e < 4; ++e) x[e] += f * from[(c0 + e + r) % D];
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = sum == 0.0f ? 0.0f : x[e] / sum;
-                    const long long rr = sp.r0 + r;
-                    const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
+                    for (int e = 0; e < 4; ++e) x[e] = sum < 1e-30f ? 0.0f : x[e] / sum;
+                    const int rr = sp.r0 + r;
+                    const int i = rr / (int)a.group, h = rr - i * (int)a.group;
                     store4(a.out, (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + c0, a.o_type, a.o_vec, x);
                 }
                 meet(true);
@@ -488,12 +520,53 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                                                     : make_uint4(0, 0, 0, 0);
                 };
                 auto fetch_scales = [&](int j, uint32_t pg) {
-                    kd = 0.0f;
 #pragma unroll
                     for (int w = 0; w < kLoadWarps; ++w) {
                         const int64_t row = row_of(j, pg, 32 * w + lane);
+                        if (w == lw) kd = row >= 0 ? __ldg(a.kv.ks + row) : 0.0f;
                         vd[w] = row >= 0 ? __ldg(a.kv.vs + row) : 0.0f;
-                        if (w == lw && row >= 0) kd = __ldg(a.kv.ks + row);
+                    }
+                };
+                // over the tile's 128 keys: the exponent that their largest scale stays below
+                auto exponent = [&](const float (&d)[kLoadWarps]) {
+                    float top = fabsf(d[0]);
+#pragma unroll
+                    for (int w = 1; w < kLoadWarps; ++w) top = fmaxf(top, fabsf(d[w]));
+                    return min(126, ((int)__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 126);
+                };
+                // the scale of the warp's key `lane` over 2^e, as a high and a low f16 part
+                auto own_scale = [&](const float (&d)[kLoadWarps], int e) {
+                    float x = d[0];
+#pragma unroll
+                    for (int w = 1; w < kLoadWarps; ++w)
+                        if (w == lw) x = d[w];
+                    x *= __int_as_float((127 - e) << 23);
+                    const __half hi = __float2half_rn(x);
+                    const __half2 both = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+                    return *reinterpret_cast<const uint32_t *>(&both);
+                };
+                // codes (times scales, one rounding) into a stage
+                auto unpack_tile = [&](const uint4 (&raw)[PER], bool scaled, uint32_t scales, uint8_t *tile) {
+#pragma unroll
+                    for (int u = 0; u < PER; ++u) {
+                        const int r = row_no(row_ix(u));
+                        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                        const uint32_t d = __shfl_sync(0xffffffffu, scales, r & 31);
+                        const uint32_t d_hi = __byte_perm(d, 0, 0x1010), d_lo = __byte_perm(d, 0, 0x3232);
+                        const __half2 hi2 = *reinterpret_cast<const __half2 *>(&d_hi), lo2 = *reinterpret_cast<const __half2 *>(&d_lo);
+                        uint32_t h[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            h[i] = codes2(w[i / 2] ^ 0x80808080u, i & 1 ? 0x4342 : 0x4140);
+                            if (scaled) {
+                                const __half2 q = *reinterpret_cast<const __half2 *>(&h[i]);
+                                const __half2 v = __hfma2(q, hi2, __hmul2(q, lo2));
+                                h[i] = *reinterpret_cast<const uint32_t *>(&v);
+                            }
+                        }
+                        uint8_t *to = tile + piece<D>(r, 2 * piece_no(u));
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(to + 128) = make_uint4(h[4], h[5], h[6], h[7]);
                     }
                 };
                 int exp_v = -126;
@@ -505,15 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     const uint32_t stage = (ks + j) & 1, turn = (ks + j) >> 1, slot = (ks + j) & 3;
                     fetch(vbase, vraw);
                     const uint32_t holes = __ballot_sync(0xffffffffu, pages >= a.kv.pages) & 0xff;
-                    float top = fabsf(vd[0]), its = vd[0];
-#pragma unroll
-                    for (int w = 1; w < kLoadWarps; ++w) {
-                        top = fmaxf(top, fabsf(vd[w]));
-                        if (w == lw) its = vd[w];
-                    }
-                    const int bits = (int)__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23;
-                    exp_v = max(exp_v, min(126, bits - 126));
-                    its *= __int_as_float((127 - exp_v) << 23);
+                    exp_v = max(exp_v, exponent(vd));
+                    const uint32_t v_own = own_scale(vd, exp_v);
                     if (turn > 0) ok = wait(&sh.k_free[stage], turn - 1);
                     if (!ok) break;
                     sh.k_scale[slot][32 * lw + lane] = kd;
@@ -521,20 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         sh.v_exp[slot] = exp_v;
                         sh.holes[slot] = holes;
                     }
-                    uint8_t *tile = smem + SM::K + stage * SM::TILE;
-#pragma unroll
-                    for (int u = 0; u < PER; ++u) {
-                        const uint32_t w[4] = {kraw[u].x, kraw[u].y, kraw[u].z, kraw[u].w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            h[2 * i] = codes2(w[i] ^ 0x80808080u, 0x4140);
-                            h[2 * i + 1] = codes2(w[i] ^ 0x80808080u, 0x4342);
-                        }
-                        uint8_t *to = tile + piece<D>(row_no(row_ix(u)), 2 * piece_no(u));
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4 *>(to + 128) = make_uint4(h[4], h[5], h[6], h[7]);
-                    }
+                    unpack_tile(kraw, false, 0, smem + SM::K + stage * SM::TILE);
                     publish(&sh.k_full[stage]);
                     if (j + 1 < sp.count) {  // on their way while V is unpacked
                         rows_of(j + 1, next);
@@ -545,29 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     }
                     if (turn > 0) ok = wait(&sh.v_free[stage], turn - 1);
                     if (!ok) break;
-                    tile = smem + SM::V + stage * SM::TILE;
-                    // code * scale with one rounding: the scale as a high and a low f16 part
-                    const __half hi = __float2half_rn(its), lo = __float2half_rn(its - __half2float(hi));
-                    const __half2 both = __halves2half2(hi, lo);
-#pragma unroll
-                    for (int u = 0; u < PER; ++u) {
-                        const int r = row_no(row_ix(u));
-                        const uint32_t w[4] = {vraw[u].x, vraw[u].y, vraw[u].z, vraw[u].w};
-                        const uint32_t d = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&both), r & 31);
-                        const uint32_t d_hi = __byte_perm(d, 0, 0x1010), d_lo = __byte_perm(d, 0, 0x3232);
-                        const __half2 hi2 = *reinterpret_cast<const __half2 *>(&d_hi), lo2 = *reinterpret_cast<const __half2 *>(&d_lo);
-                        uint32_t h[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t y = codes2(w[i / 2] ^ 0x80808080u, i & 1 ? 0x4342 : 0x4140);
-                            const __half2 q = *reinterpret_cast<const __half2 *>(&y);
-                            const __half2 v = __hfma2(q, hi2, __hmul2(q, lo2));
-                            h[i] = *reinterpret_cast<const uint32_t *>(&v);
-                        }
-                        uint8_t *to = tile + piece<D>(r, 2 * piece_no(u));
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4 *>(to + 128) = make_uint4(h[4], h[5], h[6], h[7]);
-                    }
+                    unpack_tile(vraw, true, v_own, smem + SM::V + stage * SM::TILE);
                     publish(&sh.v_full[stage]);
                 }
             } else {
@@ -593,18 +624,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 for (int j = 0; j < sp.count && ok; ++j) {
                     const uint32_t stage = (ks + j) & 1;
                     const uint32_t holes = __ballot_sync(0xffffffffu, pages >= a.kv.pages) & 0xff;
+                    // what has arrived goes out before the next wait for room
+                    if (lw == 0 && lane == 0) sh.holes[(ks + j) & 3] = holes;
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    publish(&sh.k_full[stage]);
                     pages = next;
                     rows_of(j + 1, pages);
                     next = pages_of(j + 2);
                     copy(a.kv.k, SM::K, sh.k_free, j + 1);
-                    if (!ok) break;
-                    if (lw == 0 && lane == 0) sh.holes[(ks + j) & 3] = holes;
-                    asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    publish(&sh.k_full[stage]);
-                    copy(a.kv.v, SM::V, sh.v_free, j + 1);
-                    if (!ok) break;
-                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
                     publish(&sh.v_full[stage]);
+                    copy(a.kv.v, SM::V, sh.v_free, j + 1);
                 }
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
@@ -618,53 +648,55 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         constexpr uint32_t QK = instruction(kKeys, false), PV = instruction(D, true);
         for (uint32_t rt = tile0; rt < row_tiles; rt += tile_step) {
             const Span sp = span_of(rt);
-            if (warp == kMmaWarp && sp.count > 0) {
+            if (warp == kMmaWarp && lane == 0) {
                 const uint64_t q0 = operand(smem_u32(smem + SM::Q), 128, D * 16), k0 = operand(smem_u32(smem + SM::K), 128, D * 16);
                 const uint64_t v0 = operand(smem_u32(smem + SM::V), D * 16, 128);
                 auto scores = [&](int g, int j) {
-                    const uint64_t q = q0 + g * (SM::TILE >> 4), k = k0 + ((ks + j) & 1) * (SM::TILE >> 4);
+                    const uint32_t stage = (ks + j) & 1;
+                    const uint64_t q = q0 + g * (SM::TILE >> 4), k = k0 + stage * (SM::TILE >> 4);
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s) mma_ss(tmem + g * 128, q + s * 16, k + s * 16, QK, s > 0);
                     commit(&sh.s_full[g]);
+                    commit(&sh.k_free[stage]);
+                    if (sp.groups == 1) commit(&sh.k_free[stage]);
                 };
-                bool ok = wait(&sh.q_full, turns) && wait(&sh.k_full[ks & 1], ks >> 1);
-                if (ok && lane == 0) {
-                    fence_after();
-                    for (int g = 0; g < sp.groups; ++g) scores(g, 0);
-                    commit(&sh.k_free[ks & 1]);
-                }
-                for (int j = 0; j < sp.count && ok; ++j) {
-                    const uint32_t stage = (ks + j) & 1;
-                    ok = wait(&sh.v_full[stage], (ks + j) >> 1);
-                    for (int g = 0; g < sp.groups && ok; ++g) {
-                        ok = wait(&sh.p_full[g], ss[g] + j);
-                        if (!ok) break;
+                bool ok = mbar_wait(&sh.q_full, turns & 1);
+                if (sp.count > 0) {
+                    ok = ok && mbar_wait(&sh.k_full[ks & 1], (ks >> 1) & 1);
+                    if (ok) {
                         fence_after();
-                        if (lane == 0) {
+                        for (int g = 0; g < sp.groups; ++g) scores(g, 0);
+                    }
+                    int next[2] = {0, sp.groups > 1 ? 0 : sp.count};  // the groups' next tile of values
+                    uint64_t since = globaltimer();
+                    while (ok && (next[0] < sp.count || next[1] < sp.count)) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const int j = next[g];
+                            const uint32_t i = ks + j, stage = i & 1;
+                            if (j == sp.count || !mbar_test(&sh.p_full[g], (ss[g] + j) & 1) || !mbar_test(&sh.v_full[stage], (i >> 1) & 1) ||
+                                (j + 1 < sp.count && !mbar_test(&sh.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1)))
+                                continue;
+                            fence_after();
                             const uint64_t v = v0 + stage * (SM::TILE >> 4);
 #pragma unroll
                             for (int s = 0; s < kKeys / 16; ++s)
                                 mma_ts(tmem + 256 + g * D, tmem + g * 128 + s * 8, v + s * (2 * D), PV, j > 0 || s > 0);
+                            commit(&sh.v_free[stage]);
+                            if (sp.groups == 1) commit(&sh.v_free[stage]);
+                            if (j + 1 < sp.count) scores(g, j + 1);
+                            next[g] = j + 1;
+                            since = globaltimer();
                         }
-                        __syncwarp();
-                        if (j + 1 == sp.count) continue;
-                        if (g == 0) ok = wait(&sh.k_full[(ks + j + 1) & 1], (ks + j + 1) >> 1);
-                        if (!ok) break;
-                        fence_after();
-                        if (lane == 0) scores(g, j + 1);
-                        __syncwarp();
+                        if (globaltimer() - since > kWaitNs || *reinterpret_cast<volatile int *>(&sh.lost)) ok = false;
                     }
-                    if (ok && lane == 0) {
-                        commit(&sh.v_free[stage]);
-                        if (j + 1 < sp.count) commit(&sh.k_free[(ks + j + 1) & 1]);
-                    }
+                    // also after a lost wait: nothing in flight when the CTA leaves
+                    commit(&sh.o_full);
+                    ok = mbar_wait(&sh.o_full, os & 1) && ok;
                 }
-                // also after a lost wait: nothing in flight when the CTA leaves
-                if (lane == 0) commit(&sh.o_full);
-                wait(&sh.o_full, os);
-            } else if (warp == kMmaWarp) {
-                wait(&sh.q_full, turns);  // one phase a row tile
+                if (!ok) sh.lost = 1;
             }
+            __syncwarp();
             fence_before();
             meet(parts > 1);
             if (parts > 1) meet(true);

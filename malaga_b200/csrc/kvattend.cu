@@ -36,7 +36,7 @@ struct AttendArgs {
     void *out;
     long long q_token, q_head, o_token, o_head;
     int q_type, o_type, causal;
-    bool q_vec, o_vec, o_vec16;  // rows that allow accesses of four numbers, of eight 16-bit ones
+    bool o_vec, q_vec16, o_vec16;  // rows that allow accesses of four numbers, of eight 16-bit ones
     uint32_t group;  // query heads of a cache head
     uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
@@ -662,11 +662,12 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (!bad) bad = check_rows(out);
     if (!bad && (q->tokens != out->tokens || q->heads != out->heads)) bad = "q and out differ in shape";
     if (!bad && (q->heads == 0 || q->heads % kv->heads)) bad = "query heads are not a multiple of the cache's";
+    if (!bad && (uint64_t)q->tokens * q->heads > 0x7fffffffu) bad = "more than 2^31 - 1 query rows";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
     if (seqs->seqs == 0 || q->tokens == 0) return MGB_OK;
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
-                 out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*q), rows_vec(*out),
-                 rows_vec16(*out), q->heads / kv->heads,
+                 out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
+                 q->heads / kv->heads,
                  0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
