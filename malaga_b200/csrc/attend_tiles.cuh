@@ -234,67 +234,60 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             float scale = 0.0f;
             {
                 constexpr int PIECES = D / 8, PER = PIECES < 4 ? 1 : PIECES / 4;
-                // all loads before any use, as the numbers' bits
-                uint4 raw[4][PER];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int rr = sp.r0 + 32 * warp + 8 * q + (lane & 7);
-                    const int i = rr / (int)a.group, h = rr - i * (int)a.group;
+                auto fetch = [&](int q, uint4 (&raw)[PER]) {
+                    // rows past the last read it again; their scores are masked
+                    const int rr = min(sp.r0 + 32 * warp + 8 * q + (lane & 7), rows - 1), i = rr / (int)a.group, h = rr - i * (int)a.group;
                     const uint16_t *from = static_cast<const uint16_t *>(a.q) + (t0 + i) * a.q_token + (long long)(head * a.group + h) * a.q_head;
+                    if (a.q_vec16) {
 #pragma unroll
-                    for (int u = 0; u < PER; ++u) {
-                        const int c = (lane >> 3) + 4 * u;
-                        raw[q][u] = make_uint4(0, 0, 0, 0);
-                        if (rr >= rows || c >= PIECES) continue;
-                        if (a.q_vec16) {
-                            raw[q][u] = __ldg(reinterpret_cast<const uint4 *>(from + 8 * c));
-                        } else {
-                            uint16_t y[8];
+                        for (int u = 0; u < PER; ++u) raw[u] = __ldg(reinterpret_cast<const uint4 *>(from) + min((lane >> 3) + 4 * u, PIECES - 1));
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = from[8 * c + e];
-                            raw[q][u] = *reinterpret_cast<const uint4 *>(y);
+                        for (int u = 0; u < PER; ++u) {
+                            const uint16_t *y = from + 8 * min((lane >> 3) + 4 * u, PIECES - 1);
+                            raw[u] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16, y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
                         }
                     }
-                }
-#pragma unroll
+                };
+                // the loop is kept rolled: code that runs once costs its way into the instruction cache
+                uint4 raw[PER], ahead[PER];
+                fetch(0, ahead);
+#pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
-                    float x[PER][8];
 #pragma unroll
-                    for (int u = 0; u < PER; ++u) {
-                        const uint32_t w[4] = {raw[q][u].x, raw[q][u].y, raw[q][u].z, raw[q][u].w};
+                    for (int u = 0; u < PER; ++u) raw[u] = ahead[u];
+                    if (q < 3) fetch(q + 1, ahead);
+                    float mul = fabsf(a.scale);
+                    const float sign = copysignf(1.0f, a.scale);
+                    if (a.q_type == MGB_F16) {
+                        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = unpack(w[e]);
-                            x[u][2 * e] = a.q_type == MGB_F16 ? f.x : __uint_as_float(w[e] << 16);
-                            x[u][2 * e + 1] = a.q_type == MGB_F16 ? f.y : __uint_as_float(w[e] & 0xffff0000u);
+                        for (int u = 0; u < PER; ++u) raw[u].x ^= flip, raw[u].y ^= flip, raw[u].z ^= flip, raw[u].w ^= flip;
+                    } else {
+                        uint32_t top = 0;  // of the magnitudes' bits
+#pragma unroll
+                        for (int u = 0; u < PER; ++u) {
+                            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fff0000u, w[e] & 0x7fff0000u));
                         }
-                    }
-                    int shift = 0;
-                    if (a.q_type != MGB_F16) {
-                        float m = 0.0f;
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        // 2^shift in two factors, since either may leave the range of f32 alone
+                        const int shift = top && top < 0x7f800000u ? 140 - (int)(top >> 23) : 0;
+                        const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
+                        const float f1 = sign * __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
+                        // above 0, so that -inf times it stays -inf
+                        mul = fmaxf(mul * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23), 1.2e-38f);
+                        auto half2_of = [&](uint32_t w) { return pack(__uint_as_float(w << 16) * f1 * f2, __uint_as_float(w & 0xffff0000u) * f1 * f2); };
 #pragma unroll
-                        for (int u = 0; u < PER; ++u)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[u][e]));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        if (m > 0.0f && m < __int_as_float(0x7f800000)) shift = 13 - ilogbf(m);
+                        for (int u = 0; u < PER; ++u) raw[u] = make_uint4(half2_of(raw[u].x), half2_of(raw[u].y), half2_of(raw[u].z), half2_of(raw[u].w));
                     }
-                    // 2^shift in two factors, since either may leave the range of f32 alone
-                    const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
-                    const float f1 = copysignf(__int_as_float((127 + s1) << 23), a.scale), f2 = __int_as_float((127 + s2) << 23);
-                    // above 0, so that -inf times it stays -inf
-                    const float mul = fmaxf(fabsf(a.scale) * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23), 1.2e-38f);
                     const float its = __shfl_sync(0xffffffffu, mul, lane & 7);
                     if (lane >> 3 == q) scale = its;
 #pragma unroll
-                    for (int u = 0; u < PER; ++u) {
-                        const int c = (lane >> 3) + 4 * u;
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack(x[u][2 * e] * f1 * f2, x[u][2 * e + 1] * f1 * f2);
-                        if (c < PIECES) *reinterpret_cast<uint4 *>(mine + piece<D>(8 * q + (lane & 7), c)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int u = 0; u < PER; ++u)
+                        if ((lane >> 3) + 4 * u < PIECES) *reinterpret_cast<uint4 *>(mine + piece<D>(8 * q + (lane & 7), (lane >> 3) + 4 * u)) = raw[u];
                 }
             }
             fence_smem();
