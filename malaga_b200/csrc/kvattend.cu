@@ -103,7 +103,7 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 // movmatrix turns P^T, as it leaves the first product, into the B operand of
 // the second.
 //
-// A warp takes blocks of 16 keys in turn. Each block of K, V and their scales
+// A warp takes every fourth stage of keys. Each block of 16 keys of K, V and their scales
 // is one contiguous run of its page, which a bulk copy brings into the warp's
 // own ring of stages, so the loads in flight do not depend on registers or on
 // the page table's latency. A warp keeps its own maximum, sum and output. The maximum only has to be near: it is raised when a score passes it
@@ -120,8 +120,9 @@ struct Frag {
     static constexpr int VN = D * ESZ / 8 / VB;
     static constexpr int KW = D * ESZ / 16, VW = D * ESZ / 32 ? D * ESZ / 32 : 1;  // words of a key and lane
     static constexpr int STEPS = D / 16;
-    static constexpr int CTAS = D == 128 ? 4 : 5;  // of an SM, with tiles of 8 rows
-    static constexpr int STATIC = 32 * D + 512;  // static shared memory of a CTA a tile of 8 rows, at most
+    // CTAs of an SM that the registers have to leave room for
+    static constexpr int ctas(int nt) { return D < 128 ? (nt == 1 ? 5 : 3) : nt == 2 && Q8 ? 2 : 3; }
+    static constexpr int STATIC = 32 * D + 1024;  // static shared memory of a CTA a tile of 8 rows, at most
     // dim of element e of lane t's part of a K row, of lane g's part of a V row
     static __device__ __forceinline__ int k_dim(int t, int e) {
         constexpr int VE = KB / ESZ;
@@ -138,11 +139,14 @@ constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
 constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
 constexpr float kRaise = 7.0f;  // p is held as 2^7 p, up to 2^15
 
-// A stage: 16 keys of K and of V, then their scales (8-bit caches).
+// A stage: BLOCKS times 16 keys of K, of V, then (8-bit caches) of their scales.
+// 8-bit codes come 32 keys at a time, which halves what a stage costs beside its
+// arithmetic; f16 ones, twice as large, 16.
 template <int D, bool Q8>
 struct Ring {
-    static constexpr int ROWS = 16 * D * (Q8 ? 1 : 2), SCALES = Q8 ? 64 : 0;
-    static constexpr int STAGE = 2 * ROWS + 2 * SCALES;
+    static constexpr int BLOCKS = Q8 ? 2 : 1;
+    static constexpr int ROWS = 16 * D * (Q8 ? 1 : 2), SCALES = Q8 ? 64 : 0;  // bytes of a block
+    static constexpr int V = BLOCKS * ROWS, KS = 2 * V, VS = KS + BLOCKS * SCALES, STAGE = VS + BLOCKS * SCALES;
     // about 12 KB a warp, 2 to 4 stages: more would cost CTAs of an SM
     static constexpr int FIT = 12800 / STAGE;
     static constexpr int N = FIT < 2 ? 2 : FIT > 4 ? 4 : FIT;
@@ -155,18 +159,18 @@ struct Block {  // a lane's share of 16 keys
     uint32_t v[4][Frag<D, Q8>::VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
     float ks[2], vs[2];              // scales of keys g, g + 8
     // left: keys that exist; the places of the others hold anything
-    __device__ __forceinline__ void load_k(const uint8_t *stage, int g, int t) {
+    __device__ __forceinline__ void load_k(const uint8_t *stage, int blk, int g, int t) {
         using F = Frag<D, Q8>;
         using R = Ring<D, Q8>;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int c = 0; c < F::KN; ++c)
-                load_words<F::KB>(stage + (g + 8 * u) * (D * F::ESZ) + (t + 4 * c) * F::KB, &k[u][c * (F::KB / 4)]);
-            if constexpr (Q8) ks[u] = reinterpret_cast<const float *>(stage + 2 * R::ROWS)[g + 8 * u];
+                load_words<F::KB>(stage + blk * R::ROWS + (g + 8 * u) * (D * F::ESZ) + (t + 4 * c) * F::KB, &k[u][c * (F::KB / 4)]);
+            if constexpr (Q8) ks[u] = reinterpret_cast<const float *>(stage + R::KS)[16 * blk + g + 8 * u];
         }
     }
-    __device__ __forceinline__ void load_v(const uint8_t *stage, int left, int g, int t) {
+    __device__ __forceinline__ void load_v(const uint8_t *stage, int blk, int left, int g, int t) {
         using F = Frag<D, Q8>;
         using R = Ring<D, Q8>;
 #pragma unroll
@@ -174,12 +178,12 @@ struct Block {  // a lane's share of 16 keys
             const int key = 2 * t + (u & 1) + 8 * (u >> 1);
 #pragma unroll
             for (int c = 0; c < F::VN; ++c)
-                load_words<F::VB>(stage + R::ROWS + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &v[u][c * (F::VB / 4)]);
+                load_words<F::VB>(stage + R::V + blk * R::ROWS + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &v[u][c * (F::VB / 4)]);
         }
         if constexpr (Q8) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                vs[u] = reinterpret_cast<const float *>(stage + 2 * R::ROWS + R::SCALES)[g + 8 * u];
+                vs[u] = reinterpret_cast<const float *>(stage + R::VS)[16 * blk + g + 8 * u];
         }
         if (left < 16) {  // 0 times what a stale place holds must stay 0
 #pragma unroll
@@ -226,50 +230,66 @@ struct Rows {
     float m[NT][2], l[NT][2];
     int exp_v;  // V's scales so far are below 2^exp_v
 
-    __device__ __forceinline__ void step(Block<D, Q8> &x, const uint8_t *stage, int key0, int end, int g, int t) {
-        x.load_k(stage, g, t);
-        float s[NT][4];  // key g: rows 2t, 2t + 1; key g + 8: the same
+    // have: bit i, block i of the stage is in the cache; key0: the stage's first key
+    __device__ __forceinline__ void step(const uint8_t *stage, uint32_t have, int key0, int end, int g, int t) {
+        constexpr int B = Ring<D, Q8>::BLOCKS;
+        Block<D, Q8> x[B];
+        float s[B][NT][4];  // key g: rows 2t, 2t + 1; key g + 8: the same
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < B; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int st = 0; st < F::STEPS; ++st) {
-            uint32_t a[4];
-            if constexpr (Q8) {
-                const uint32_t lo = x.k[0][st] ^ 0x80808080u, hi = x.k[1][st] ^ 0x80808080u;
-                a[0] = codes2(lo, 0x4140), a[1] = codes2(hi, 0x4140);
-                a[2] = codes2(lo, 0x4342), a[3] = codes2(hi, 0x4342);
-            } else {
-                a[0] = x.k[0][2 * st], a[1] = x.k[1][2 * st];
-                a[2] = x.k[0][2 * st + 1], a[3] = x.k[1][2 * st + 1];
-            }
+                for (int e = 0; e < 4; ++e) s[i][n][e] = 0.0f;
+            if (B > 1 && !((have >> i) & 1)) continue;
+            x[i].load_k(stage, i, g, t);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma16(s[n], a, q[0][n][st][0], q[0][n][st][1]);
-                if constexpr (SPLIT) mma16(s[n], a, q[1][n][st][0], q[1][n][st][1]);
+            for (int st = 0; st < F::STEPS; ++st) {
+                uint32_t a[4];
+                if constexpr (Q8) {
+                    const uint32_t lo = x[i].k[0][st] ^ 0x80808080u, hi = x[i].k[1][st] ^ 0x80808080u;
+                    a[0] = codes2(lo, 0x4140), a[1] = codes2(hi, 0x4140);
+                    a[2] = codes2(lo, 0x4342), a[3] = codes2(hi, 0x4342);
+                } else {
+                    a[0] = x[i].k[0][2 * st], a[1] = x[i].k[1][2 * st];
+                    a[2] = x[i].k[0][2 * st + 1], a[3] = x[i].k[1][2 * st + 1];
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16(s[i][n], a, q[0][n][st][0], q[0][n][st][1]);
+                    if constexpr (SPLIT) mma16(s[i][n], a, q[1][n][st][0], q[1][n][st][1]);
+                }
             }
         }
-        x.load_v(stage, end - key0, g, t);
-        const bool whole = key0 + 16 <= all;
-        bool see[NT][4], past = false;
+        const bool whole = key0 + 16 * B <= all && have == (1u << B) - 1;
+        bool past = false;
+        float d = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < B; ++i) {
+            if (B > 1 && !((have >> i) & 1)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                see[n][e] = whole || key0 + g + 8 * (e >> 1) < limit[n][e & 1];
-                s[n][e] = see[n][e] ? s[n][e] * (Q8 ? scale[n][e & 1] * x.ks[e >> 1] : scale[n][e & 1]) : kLowest;
-                past |= s[n][e] > m[n][e & 1] + kSlack;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][n][e] = kLowest;
+                x[i].vs[0] = x[i].vs[1] = 0.0f;
+                continue;
             }
-        if constexpr (Q8) {
-            const float d = fmaxf(fabsf(x.vs[0]), fabsf(x.vs[1]));
-            past |= (__float_as_int(d) >> 23) - 126 > exp_v;
+            x[i].load_v(stage, i, end - key0 - 16 * i, g, t);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[i][n][e] *= Q8 ? scale[n][e & 1] * x[i].ks[e >> 1] : scale[n][e & 1];
+                    if (!whole && key0 + 16 * i + g + 8 * (e >> 1) >= limit[n][e & 1]) s[i][n][e] = kLowest;
+                    past |= s[i][n][e] > m[n][e & 1] + kSlack;
+                }
+            if constexpr (Q8) d = fmaxf(d, fmaxf(fabsf(x[i].vs[0]), fabsf(x[i].vs[1])));
         }
+        if constexpr (Q8) past |= (__float_as_int(d) >> 23) - 126 > exp_v;
         if (__any_sync(0xffffffffu, past)) {
             float f = 1.0f;
             if constexpr (Q8) {
-                const float d = max_keys(fmaxf(fabsf(x.vs[0]), fabsf(x.vs[1])));
-                const int e = max(exp_v, min(126, (__float_as_int(d) >> 23) - 126));
+                const int e = max(exp_v, min(126, (__float_as_int(max_keys(d)) >> 23) - 126));
                 f = power_of_2(exp_v - e);
                 exp_v = e;
             }
@@ -277,7 +297,10 @@ struct Rows {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float top = fmaxf(m[n][r], max_keys(fmaxf(s[n][r], s[n][2 + r])));
+                    float top = fmaxf(s[0][n][r], s[0][n][2 + r]);
+#pragma unroll
+                    for (int i = 1; i < B; ++i) top = fmaxf(top, fmaxf(s[i][n][r], s[i][n][2 + r]));
+                    top = fmaxf(m[n][r], max_keys(top));
                     const float w = m[n][r] == kLowest ? 0.0f : exp2_of(m[n][r] - top);
                     m[n][r] = top;
                     l[n][r] *= w;
@@ -288,59 +311,64 @@ struct Rows {
                     }
                 }
         }
-        uint32_t p[SPLIT ? 2 : 1][NT][2];
         const float back = Q8 ? __int_as_float((127 - exp_v) << 23) : 1.0f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            // where nothing was seen yet s is -inf, and any finite maximum gives p = 0
-            const float z[2] = {(m[n][0] == kLowest ? 0.0f : m[n][0]) - kRaise, (m[n][1] == kLowest ? 0.0f : m[n][1]) - kRaise};
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = exp2_of(s[n][e] - z[e & 1]);
-                l[n][e & 1] += w[e];
-                if constexpr (Q8) w[e] = see[n][e] ? w[e] * (x.vs[e >> 1] * back) : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t hi = pack(w[2 * u], w[2 * u + 1]);
-                p[0][n][u] = transpose8(hi);
-                if constexpr (SPLIT) {
-                    const float2 h = unpack(hi);
-                    p[1][n][u] = transpose8(pack(w[2 * u] - h.x, w[2 * u + 1] - h.y));
-                }
-            }
-        }
-        auto pair = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-            const uint32_t f[4] = {a0, a1, a2, a3};
+        for (int i = 0; i < B; ++i) {
+            if (B > 1 && !((have >> i) & 1)) continue;
+            uint32_t p[SPLIT ? 2 : 1][NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma16(o[n][j], f, p[0][n][0], p[0][n][1]);
-                if constexpr (SPLIT) mma16(o[n][j], f, p[1][n][0], p[1][n][1]);
-            }
-        };
+                // where nothing was seen yet s is -inf, and any finite maximum gives p = 0
+                const float z[2] = {(m[n][0] == kLowest ? 0.0f : m[n][0]) - kRaise, (m[n][1] == kLowest ? 0.0f : m[n][1]) - kRaise};
+                float w[4];
 #pragma unroll
-        for (int i = 0; i < F::VW; ++i) {
-            if constexpr (Q8) {
-                const uint32_t x0 = x.v[0][i] ^ 0x80808080u, x1 = x.v[1][i] ^ 0x80808080u;
-                const uint32_t x2 = x.v[2][i] ^ 0x80808080u, x3 = x.v[3][i] ^ 0x80808080u;
-                const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
-                constexpr int PER = F::STEPS < 2 ? 1 : 2;
-                pair(PER * i, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
-                if constexpr (PER == 2) {
-                    const uint32_t hi0 = __byte_perm(x0, x1, 0x7362), hi1 = __byte_perm(x2, x3, 0x7362);
-                    pair(PER * i + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
+                for (int e = 0; e < 4; ++e) {
+                    const bool see = s[i][n][e] != kLowest;  // a masked key's scale may be NaN
+                    w[e] = exp2_of(s[i][n][e] - z[e & 1]);
+                    l[n][e & 1] += w[e];
+                    if constexpr (Q8) w[e] = whole || see ? w[e] * (x[i].vs[e >> 1] * back) : 0.0f;
                 }
-            } else {
-                pair(i, __byte_perm(x.v[0][i], x.v[1][i], 0x5410), __byte_perm(x.v[0][i], x.v[1][i], 0x7632),
-                     __byte_perm(x.v[2][i], x.v[3][i], 0x5410), __byte_perm(x.v[2][i], x.v[3][i], 0x7632));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t hi = pack(w[2 * u], w[2 * u + 1]);
+                    p[0][n][u] = transpose8(hi);
+                    if constexpr (SPLIT) {
+                        const float2 h = unpack(hi);
+                        p[1][n][u] = transpose8(pack(w[2 * u] - h.x, w[2 * u + 1] - h.y));
+                    }
+                }
+            }
+            auto pair = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                const uint32_t f[4] = {a0, a1, a2, a3};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16(o[n][j], f, p[0][n][0], p[0][n][1]);
+                    if constexpr (SPLIT) mma16(o[n][j], f, p[1][n][0], p[1][n][1]);
+                }
+            };
+#pragma unroll
+            for (int c = 0; c < F::VW; ++c) {
+                if constexpr (Q8) {
+                    const uint32_t x0 = x[i].v[0][c] ^ 0x80808080u, x1 = x[i].v[1][c] ^ 0x80808080u;
+                    const uint32_t x2 = x[i].v[2][c] ^ 0x80808080u, x3 = x[i].v[3][c] ^ 0x80808080u;
+                    const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
+                    constexpr int PER = F::STEPS < 2 ? 1 : 2;
+                    pair(PER * c, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
+                    if constexpr (PER == 2) {
+                        const uint32_t hi0 = __byte_perm(x0, x1, 0x7362), hi1 = __byte_perm(x2, x3, 0x7362);
+                        pair(PER * c + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
+                    }
+                } else {
+                    pair(c, __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x5410), __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x7632),
+                         __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x5410), __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x7632));
+                }
             }
         }
     }
 };
 
 template <int D, bool Q8, bool SPLIT, int NT>
-__global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)) attend_rows_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_rows_kernel(const AttendArgs a) {
     using F = Frag<D, Q8>;
     constexpr int R = 8 * NT, PER_ROW = kRowThreads / R, E = D / PER_ROW;
     static_assert(E >= 1, "at most one thread a number");
@@ -349,9 +377,9 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
     static_assert(RG::BYTES >= kRowWarps * R * D * 4, "the warps' outputs take the rings' place");
     float(*so)[R][D] = reinterpret_cast<float(*)[R][D]>(smem);
     __shared__ uint64_t full[kRowWarps][RG::N];
-    __shared__ int have[kRowWarps][RG::N];  // whether the stage's block is in the cache
+    __shared__ uint32_t have[kRowWarps][RG::N];  // which of the stage's blocks are in the cache
     __shared__ __align__(16) __half sq[SPLIT ? 2 : 1][R][D];
-    __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R];
+    __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R], weight[16][R];
     __shared__ int row_limit[R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
@@ -360,44 +388,50 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
     const int t0 = a.seq.first(b, n);
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
-    const long long rows = (long long)n * a.group;
-    if (rows > a.few) return;
+    const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
+    if ((uint32_t)rows > a.few) return;
     if (lane < RG::N) mbar_init(&full[warp][lane], 1);
     __syncwarp();
     uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
     uint32_t put = 0, get = 0, phase = 0;  // next stage to fill and to read, and its barrier's parity
     const uint32_t page_mask = (1u << a.kv.page_log2) - 1;
-    const bool scales = lane & 2;
-    const uint8_t *my_base = static_cast<const uint8_t *>(scales ? (lane & 1 ? (void *)a.kv.vs : (void *)a.kv.ks)
-                                                                 : (lane & 1 ? a.kv.v : a.kv.k));
-    const uint32_t my_row = scales ? 4 : D * F::ESZ, my_bytes = scales ? RG::SCALES : RG::ROWS;
-    const uint32_t my_offset = (scales ? 2 * RG::ROWS : 0) + (lane & 1) * my_bytes;
+    // lane BLOCKS * i + blk copies block blk of a stage's K, V, scales of K, scales of V (i = 0 to 3)
+    constexpr int COPIES = RG::BLOCKS * (Q8 ? 4 : 2);
+    const int kind = lane / RG::BLOCKS, my_blk = lane % RG::BLOCKS;
+    const uint8_t *my_base = static_cast<const uint8_t *>(kind == 0 ? a.kv.k : kind == 1 ? a.kv.v : kind == 2 ? (void *)a.kv.ks : (void *)a.kv.vs);
+    const uint32_t my_row = kind >= 2 ? 4 : D * F::ESZ, my_bytes = kind >= 2 ? RG::SCALES : RG::ROWS;
+    const uint32_t my_offset = (kind == 0 ? 0 : kind == 1 ? RG::V : kind == 2 ? RG::KS : RG::VS) + my_blk * my_bytes;
     // keys that token i sees
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 
-    for (long long r0 = (long long)(blockIdx.y / heads) * R; r0 < rows; r0 += (long long)(gridDim.y / heads) * R) {
-        const int end = limit((int)((min(r0 + R, rows) - 1) / a.group));  // no row of the tile sees further
+    for (int r0 = (int)(blockIdx.y / heads) * R; r0 < rows; r0 += (int)(gridDim.y / heads) * R) {
+        const int live = min(R, rows - r0);
+        const int end = limit((r0 + live - 1) / (int)a.group);  // no row of the tile sees further
+        // the CTA's part of the keys, in 16-key blocks; a warp takes every fourth stage
         const int blocks = (end + 15) / 16;
-        const int first = (int)((long long)blocks * part / parts), stop = (int)((long long)blocks * (part + 1) / parts);
-        const int mine = first + warp < stop ? (stop - first - warp + kRowWarps - 1) / kRowWarps : 0;
-        // block i of the warp is number first + warp + i * kRowWarps; the lanes hold the pages of 32 of them
-        uint32_t pages = 0;
+        const int first = (int)((uint64_t)blocks * part / parts), stop = (int)((uint64_t)blocks * (part + 1) / parts);
+        const int stages = (stop - first + RG::BLOCKS - 1) / RG::BLOCKS;
+        const int mine = warp < stages ? (stages - warp + kRowWarps - 1) / kRowWarps : 0;
+        auto block_of = [&](int i) { return first + (warp + i * kRowWarps) * RG::BLOCKS; };
+        uint32_t pages = 0;  // lane's: of block lane % BLOCKS of stage lane / BLOCKS of the group of stages in hand
+        constexpr int GROUP = 32 / RG::BLOCKS;
         auto issue = [&](int i) {
-            if ((i & 31) == 0) {
-                const int blk = first + warp + (i + lane) * kRowWarps;
-                pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0u;
+            if (i % GROUP == 0) {
+                const int blk = block_of(i + lane / RG::BLOCKS) + my_blk;
+                pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0xffffffffu;
             }
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const uint32_t page = __shfl_sync(0xffffffffu, pages, i % GROUP * RG::BLOCKS + my_blk);
             const bool there = page < a.kv.pages;
+            const uint32_t got = __ballot_sync(0xffffffffu, there) & ((1u << RG::BLOCKS) - 1);
             uint64_t *bar = &full[warp][put];
             if (lane == 0) {
-                have[warp][put] = there;
-                if (there) mbar_expect_tx(bar, RG::STAGE);
+                have[warp][put] = got;
+                if (got) mbar_expect_tx(bar, __popc(got) * (RG::STAGE / RG::BLOCKS));
                 else mbar_arrive_cta(bar);
             }
             __syncwarp();
-            if (lane < (Q8 ? 4 : 2) && there) {  // lane 0 copies K, 1 V, 2 and 3 their scales
-                const size_t row = a.kv.row(page, head, (uint32_t)((first + warp + i * kRowWarps) * 16) & page_mask);
+            if (lane < COPIES && there) {
+                const size_t row = a.kv.row(page, head, (uint32_t)((block_of(i) + my_blk) * 16) & page_mask);
                 bulk_g2s(ring + put * RG::STAGE + my_offset, my_base + row * my_row, my_bytes, bar);
             }
             put = put + 1 == RG::N ? 0 : put + 1;
@@ -407,23 +441,24 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
         // Q: the row's largest number to just below 2^14 (f16 q stays as it is)
         {
             const int r = tid / PER_ROW, c = tid % PER_ROW;
-            const long long rr = r0 + r;
+            const int rr = min(r0 + r, rows - 1), i = rr / (int)a.group, h = rr - i * (int)a.group;
+            const int64_t at = (t0 + i) * a.q_token + (int64_t)(head * a.group + h) * a.q_head + c * E;
             float x[E], m = 0.0f;
-            const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                x[e] = rr < rows ? load1(a.q, (size_t)((t0 + i) * a.q_token + (long long)(head * a.group + h) * a.q_head) + c * E + e,
-                                         a.q_type)
-                                 : 0.0f;
+                x[e] = load1(a.q, (size_t)(at + e), a.q_type);
                 m = fmaxf(m, fabsf(x[e]));
             }
+            float f1 = 1.0f, f2 = 1.0f, undo = a.scale;
+            if (a.q_type != MGB_F16) {
 #pragma unroll
-            for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            int shift = 0;
-            if (a.q_type != MGB_F16 && m > 0.0f && m < __int_as_float(0x7f800000)) shift = 13 - ilogbf(m);
-            // 2^shift in two factors, since either may leave the range of f32 alone
-            const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
-            const float f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
+                for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // 2^shift in two factors, since either may leave the range of f32 alone
+                const int shift = m > 0.0f && m < __int_as_float(0x7f800000) ? 140 - (__float_as_int(m) >> 23) : 0;
+                const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
+                f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
+                undo = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+            }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float y = x[e] * f1 * f2;
@@ -432,15 +467,14 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
                 if constexpr (SPLIT) sq[1][r][c * E + e] = __float2half_rn(y - __half2float(hi));
             }
             if (c == 0) {
-                row_scale[r] = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
-                row_limit[r] = rr < rows ? limit(i) : 0;
+                row_scale[r] = undo;
+                row_limit[r] = r < live ? limit(i) : 0;
             }
         }
         __syncthreads();
         Rows<D, Q8, SPLIT, NT> st;
         st.exp_v = -126;
-        st.all = limit((int)(r0 / a.group));
-        if (r0 + R > rows) st.all = 0;
+        st.all = row_limit[0];  // what the rows past `live` see does not matter
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -466,10 +500,8 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
         bool lost = false;  // a copy did not arrive in time: the rows become NaN
         for (int i = 0; i < mine; ++i) {
             lost |= !mbar_wait(&full[warp][get], phase);
-            if (have[warp][get]) {
-                Block<D, Q8> x;
-                st.step(x, ring + get * RG::STAGE, (first + warp + i * kRowWarps) * 16, end, g, t);
-            }
+            const uint32_t got = have[warp][get];
+            if (got) st.step(ring + get * RG::STAGE, got, block_of(i) * 16, end, g, t);
             __syncwarp();  // every lane has read the stage
             if (i + RG::N < mine) issue(i + RG::N);
             if (++get == RG::N) get = 0, phase ^= 1;
@@ -493,6 +525,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int row = 8 * j + 2 * t + r;
+                if (row >= live) continue;
                 float top = wm[0][row];
 #pragma unroll
                 for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, wm[w][row]);
@@ -503,20 +536,18 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
                     so[warp][row][F::v_dim(g, 2 * s + 1)] = st.o[j][s][2 + r] * f;
                 }
             }
-        if (tid < R) {
+        if (tid < live) {
             float top = kLowest, sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, wm[w][tid]);
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w)
-                if (wm[w][tid] != kLowest) sum += wl[w][tid] * exp2_of(wm[w][tid] - top);
+            for (int w = 0; w < kRowWarps; ++w) sum += wm[w][tid] == kLowest ? wl[w][tid] : wl[w][tid] * exp2_of(wm[w][tid] - top);
             cm[tid] = top;
             cl[tid] = sum;
         }
         __syncthreads();
         namespace cg = cooperative_groups;
         auto cluster = cg::this_cluster();
-        const int live = (int)min((long long)R, rows - r0);
         if (parts > 1) {
             for (int u = tid; u < live * D; u += kRowThreads) {
                 float sum = 0.0f;
@@ -525,29 +556,34 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::CTAS / NT + (NT - 1)
                 (&so[0][0][0])[u] = sum;
             }
             cluster_sync();
+            // the CTAs' weights of a row, over the row's sum
+            if (tid < live) {
+                float top = kLowest, sum = 0.0f;
+                for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, *cluster.map_shared_rank(&cm[tid], c));
+                for (uint32_t c = 0; c < parts; ++c) {
+                    const float m = *cluster.map_shared_rank(&cm[tid], c), l = *cluster.map_shared_rank(&cl[tid], c);
+                    const float f = m == kLowest ? 0.0f : exp2_of(m - top);
+                    weight[c][tid] = f;
+                    sum += m == kLowest ? l : f * l;
+                }
+                row_scale[tid] = sum;
+            }
+            __syncthreads();
         }
         // outputs; with several CTAs each takes its share of the tile
         for (int u = (int)part * kRowThreads + tid; u < live * D; u += (int)parts * kRowThreads) {
             const int r = u / D, d = u % D;
-            float sum = 0.0f, l = 0.0f;
+            float sum = 0.0f;
             if (parts == 1) {
-                l = cl[r];
 #pragma unroll
                 for (int w = 0; w < kRowWarps; ++w) sum += (&so[w][0][0])[u];
             } else {
-                float top = kLowest;
-                for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, *cluster.map_shared_rank(&cm[r], c));
-                for (uint32_t c = 0; c < parts; ++c) {
-                    const float m = *cluster.map_shared_rank(&cm[r], c);
-                    const float f = m == kLowest ? 0.0f : exp2_of(m - top);
-                    l += f * *cluster.map_shared_rank(&cl[r], c);
-                    sum += f * *cluster.map_shared_rank(&so[0][0][0] + u, c);
-                }
+#pragma unroll 4
+                for (uint32_t c = 0; c < parts; ++c) sum += weight[c][r] * *cluster.map_shared_rank(&so[0][0][0] + u, c);
             }
-            const long long rr = r0 + r;
-            const int i = (int)(rr / a.group), h = (int)(rr - (long long)i * a.group);
-            store1(a.out, (size_t)((t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head) + d, a.o_type,
-                   l == 0.0f ? 0.0f : sum / l);
+            const float l = parts == 1 ? cl[r] : row_scale[r];
+            const int rr = r0 + r, i = rr / (int)a.group, h = rr - i * (int)a.group;
+            store1(a.out, (size_t)((t0 + i) * a.o_token + (int64_t)(head * a.group + h) * a.o_head + d), a.o_type, l == 0.0f ? 0.0f : sum / l);
         }
         // the next tile's copies go where this one's outputs stood
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -581,8 +617,8 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
 // more than 2048 keys: sequences of unlike lengths then even out.
 template <int D, bool Q8, bool SPLIT, int NT>
 cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
-    constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, PER_SM = 227 * 1024 / SMEM;
-    constexpr int SLOTS = 148 * (PER_SM < 4 ? PER_SM : 4);
+    constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, FIT = 227 * 1024 / SMEM;
+    constexpr int SLOTS = 148 * (FIT < Frag<D, Q8>::ctas(NT) ? FIT : Frag<D, Q8>::ctas(NT));
     uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
     if (tiles * a.kv.heads > 65535) tiles = 65535 / a.kv.heads;
     const uint64_t base = tiles * a.kv.heads * a.seq.seqs;
