@@ -17,6 +17,12 @@
 //    two per row, and then exact but for numbers 2^-38 of the row's largest.
 //  * for f32 q both are split into a high and a low f16 part (SPLIT), two
 //    products each, which keeps 22 bits.
+//  * Few rows over 8-bit caches: q is cut into 8-bit digits instead, so that
+//    K's codes go into the integer mma as they are (mma.m16n8k32 measured the
+//    rate of the f16 mma.m16n8k16, and unpacking K was a quarter of the
+//    instructions). Two digits hold q to 2^-15 of the row's largest number, an
+//    eighth of the error of P's rounding; three, for f32 q, to 2^-22. The sums
+//    are exact.
 #include <cooperative_groups.h>
 
 #include "numerics.cuh"
@@ -55,6 +61,18 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 8-bit integers, sums of 32 (or, with one word of a row, 16) products.
+__device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0));
 }
 
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -103,10 +121,14 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 // movmatrix turns P^T, as it leaves the first product, into the B operand of
 // the second.
 //
-// A warp takes every fourth stage of keys. Each block of 16 keys of K, V and their scales
-// is one contiguous run of its page, which a bulk copy brings into the warp's
-// own ring of stages, so the loads in flight do not depend on registers or on
-// the page table's latency. A warp keeps its own maximum, sum and output. The maximum only has to be near: it is raised when a score passes it
+// A warp takes every fourth stage of keys and copies it itself, asynchronously,
+// into its own ring of stages: each 16 keys of K, of V and of their scales are a
+// contiguous run of a page, and what is in flight depends neither on registers
+// nor on the page table's latency. (Bulk copies, one for each run, took a loop
+// over the issuing lanes that was a third of all instructions.) The 16-byte
+// pieces of a row stand turned by its key, so that the reads below meet in few
+// banks. A warp keeps its own maximum, sum and output. The maximum only has to
+// be near: it is raised when a score passes it
 // by 2^8, so most blocks need one vote and no reduction across lanes. Warps
 // join in shared memory, the CTAs of a cluster (which cut the keys among them)
 // through distributed shared memory, in a fixed order.
@@ -120,9 +142,17 @@ struct Frag {
     static constexpr int VN = D * ESZ / 8 / VB;
     static constexpr int KW = D * ESZ / 16, VW = D * ESZ / 32 ? D * ESZ / 32 : 1;  // words of a key and lane
     static constexpr int STEPS = D / 16;
+    // place of 16-byte piece c of key `key` in its block of 16
+    static constexpr int PIECES = D * ESZ / 16;
+    static __device__ __forceinline__ int piece(int key, int c) {
+        const int turn = PIECES >= 8 ? ((key >> 1) & 3) << 1 ^ (key & 1) << 2 : PIECES == 4 ? key & 2 : 0;
+        return key * (D * ESZ) + (c ^ turn) * 16;
+    }
+    // place of byte b of key `key`'s row
+    static __device__ __forceinline__ int byte(int key, int b) { return piece(key, b / 16) + b % 16; }
     // CTAs of an SM that the registers have to leave room for
     static constexpr int ctas(int nt) { return D < 128 ? (nt == 1 ? 5 : 3) : nt == 2 && Q8 ? 2 : 3; }
-    static constexpr int STATIC = 32 * D + 1024;  // static shared memory of a CTA a tile of 8 rows, at most
+    static constexpr int STATIC = 32 * D + 1536;  // static shared memory of a CTA a tile of 8 rows, at most
     // dim of element e of lane t's part of a K row, of lane g's part of a V row
     static __device__ __forceinline__ int k_dim(int t, int e) {
         constexpr int VE = KB / ESZ;
@@ -166,7 +196,7 @@ struct Block {  // a lane's share of 16 keys
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int c = 0; c < F::KN; ++c)
-                load_words<F::KB>(stage + blk * R::ROWS + (g + 8 * u) * (D * F::ESZ) + (t + 4 * c) * F::KB, &k[u][c * (F::KB / 4)]);
+                load_words<F::KB>(stage + blk * R::ROWS + F::byte(g + 8 * u, (t + 4 * c) * F::KB), &k[u][c * (F::KB / 4)]);
             if constexpr (Q8) ks[u] = reinterpret_cast<const float *>(stage + R::KS)[16 * blk + g + 8 * u];
         }
     }
@@ -178,7 +208,7 @@ struct Block {  // a lane's share of 16 keys
             const int key = 2 * t + (u & 1) + 8 * (u >> 1);
 #pragma unroll
             for (int c = 0; c < F::VN; ++c)
-                load_words<F::VB>(stage + R::V + blk * R::ROWS + key * (D * F::ESZ) + (g + 8 * c) * F::VB, &v[u][c * (F::VB / 4)]);
+                load_words<F::VB>(stage + R::V + blk * R::ROWS + F::byte(key, (g + 8 * c) * F::VB), &v[u][c * (F::VB / 4)]);
         }
         if constexpr (Q8) {
 #pragma unroll
@@ -222,7 +252,8 @@ __device__ __forceinline__ float sum_keys(float x) {
 template <int D, bool Q8, bool SPLIT, int NT>
 struct Rows {
     using F = Frag<D, Q8>;
-    uint32_t q[SPLIT ? 2 : 1][NT][F::STEPS][2];
+    static constexpr int DIGITS = SPLIT ? 3 : 2;  // of q, with 8-bit caches
+    uint32_t q[Q8 ? DIGITS : SPLIT ? 2 : 1][NT][F::STEPS][Q8 ? 1 : 2];
     float scale[NT][2];
     int limit[NT][2];
     int all;  // keys below are seen by every row
@@ -243,21 +274,36 @@ struct Rows {
                 for (int e = 0; e < 4; ++e) s[i][n][e] = 0.0f;
             if (B > 1 && !((have >> i) & 1)) continue;
             x[i].load_k(stage, i, g, t);
-#pragma unroll
-            for (int st = 0; st < F::STEPS; ++st) {
-                uint32_t a[4];
-                if constexpr (Q8) {
-                    const uint32_t lo = x[i].k[0][st] ^ 0x80808080u, hi = x[i].k[1][st] ^ 0x80808080u;
-                    a[0] = codes2(lo, 0x4140), a[1] = codes2(hi, 0x4140);
-                    a[2] = codes2(lo, 0x4342), a[3] = codes2(hi, 0x4342);
-                } else {
-                    a[0] = x[i].k[0][2 * st], a[1] = x[i].k[1][2 * st];
-                    a[2] = x[i].k[0][2 * st + 1], a[3] = x[i].k[1][2 * st + 1];
-                }
+            if constexpr (Q8) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma16(s[i][n], a, q[0][n][st][0], q[0][n][st][1]);
-                    if constexpr (SPLIT) mma16(s[i][n], a, q[1][n][st][0], q[1][n][st][1]);
+                    int c[DIGITS][4];
+#pragma unroll
+                    for (int z = 0; z < DIGITS; ++z) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[z][e] = 0;
+                        if constexpr (F::STEPS == 1) {
+                            mma8(c[z], x[i].k[0][0], x[i].k[1][0], q[z][n][0][0]);
+                        } else {
+#pragma unroll
+                            for (int st = 0; st < F::STEPS; st += 2)
+                                mma8(c[z], x[i].k[0][st], x[i].k[1][st], x[i].k[0][st + 1], x[i].k[1][st + 1], q[z][n][st][0], q[z][n][st + 1][0]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[i][n][e] = SPLIT ? __fmaf_rn((float)c[0][e], 16384.0f, (float)(c[1][e] * 128 + c[DIGITS - 1][e]))
+                                           : (float)(c[0][e] * 128 + c[1][e]);
+                }
+            } else {
+#pragma unroll
+                for (int st = 0; st < F::STEPS; ++st) {
+                    const uint32_t a[4] = {x[i].k[0][2 * st], x[i].k[1][2 * st], x[i].k[0][2 * st + 1], x[i].k[1][2 * st + 1]};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16(s[i][n], a, q[0][n][st][0], q[0][n][st][1]);
+                        if constexpr (SPLIT) mma16(s[i][n], a, q[SPLIT][n][st][0], q[SPLIT][n][st][1]);
+                    }
                 }
             }
         }
@@ -376,9 +422,9 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
     extern __shared__ __align__(128) uint8_t smem[];
     static_assert(RG::BYTES >= kRowWarps * R * D * 4, "the warps' outputs take the rings' place");
     float(*so)[R][D] = reinterpret_cast<float(*)[R][D]>(smem);
-    __shared__ uint64_t full[kRowWarps][RG::N];
-    __shared__ uint32_t have[kRowWarps][RG::N];  // which of the stage's blocks are in the cache
-    __shared__ __align__(16) __half sq[SPLIT ? 2 : 1][R][D];
+    constexpr int DIGITS = Rows<D, Q8, SPLIT, NT>::DIGITS;
+    __shared__ __align__(16) __half sq[Q8 ? 1 : SPLIT ? 2 : 1][R][D];  // Q as f16 parts,
+    __shared__ __align__(16) int8_t sd[Q8 ? DIGITS : 1][R][D];         // or as 8-bit digits
     __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R], weight[16][R];
     __shared__ int row_limit[R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -390,17 +436,10 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
     if ((uint32_t)rows > a.few) return;
-    if (lane < RG::N) mbar_init(&full[warp][lane], 1);
-    __syncwarp();
     uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
-    uint32_t put = 0, get = 0, phase = 0;  // next stage to fill and to read, and its barrier's parity
+    uint32_t put = 0, get = 0;  // next stage to fill and to read
+    uint32_t have = 0;          // BLOCKS bits a stage: which of its blocks are in the cache
     const uint32_t page_mask = (1u << a.kv.page_log2) - 1;
-    // lane BLOCKS * i + blk copies block blk of a stage's K, V, scales of K, scales of V (i = 0 to 3)
-    constexpr int COPIES = RG::BLOCKS * (Q8 ? 4 : 2);
-    const int kind = lane / RG::BLOCKS, my_blk = lane % RG::BLOCKS;
-    const uint8_t *my_base = static_cast<const uint8_t *>(kind == 0 ? a.kv.k : kind == 1 ? a.kv.v : kind == 2 ? (void *)a.kv.ks : (void *)a.kv.vs);
-    const uint32_t my_row = kind >= 2 ? 4 : D * F::ESZ, my_bytes = kind >= 2 ? RG::SCALES : RG::ROWS;
-    const uint32_t my_offset = (kind == 0 ? 0 : kind == 1 ? RG::V : kind == 2 ? RG::KS : RG::VS) + my_blk * my_bytes;
     // keys that token i sees
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 
@@ -415,56 +454,99 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         auto block_of = [&](int i) { return first + (warp + i * kRowWarps) * RG::BLOCKS; };
         uint32_t pages = 0;  // lane's: of block lane % BLOCKS of stage lane / BLOCKS of the group of stages in hand
         constexpr int GROUP = 32 / RG::BLOCKS;
-        auto issue = [&](int i) {
-            if (i % GROUP == 0) {
-                const int blk = block_of(i + lane / RG::BLOCKS) + my_blk;
-                pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0xffffffffu;
-            }
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, i % GROUP * RG::BLOCKS + my_blk);
-            const bool there = page < a.kv.pages;
-            const uint32_t got = __ballot_sync(0xffffffffu, there) & ((1u << RG::BLOCKS) - 1);
-            uint64_t *bar = &full[warp][put];
-            if (lane == 0) {
-                have[warp][put] = got;
-                if (got) mbar_expect_tx(bar, __popc(got) * (RG::STAGE / RG::BLOCKS));
-                else mbar_arrive_cta(bar);
-            }
-            __syncwarp();
-            if (lane < COPIES && there) {
-                const size_t row = a.kv.row(page, head, (uint32_t)((block_of(i) + my_blk) * 16) & page_mask);
-                bulk_g2s(ring + put * RG::STAGE + my_offset, my_base + row * my_row, my_bytes, bar);
-            }
-            put = put + 1 == RG::N ? 0 : put + 1;
+        // 16 rows of K or V, 16 bytes a lane and access
+        auto copy_rows = [&](uint8_t *to, const void *base, size_t row) {
+            const uint8_t *src = static_cast<const uint8_t *>(base) + row * (D * F::ESZ) + 16 * lane;
+#pragma unroll
+            for (int u = 0; u < RG::ROWS / 16; u += 32)
+                if (RG::ROWS >= 512 || lane < RG::ROWS / 16)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to) + F::piece((u + lane) / F::PIECES, (u + lane) % F::PIECES)),
+                                 "l"(src + 16 * u));
         };
-        for (int i = 0; i < min(mine, RG::N); ++i) issue(i);
+        auto issue = [&](int i) {  // one group of copies, empty past the last stage
+            if (i < mine) {
+                if (i % GROUP == 0) {
+                    const int blk = block_of(i + lane / RG::BLOCKS) + lane % RG::BLOCKS;
+                    pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0xffffffffu;
+                }
+                uint8_t *to = ring + put * RG::STAGE;
+                uint32_t got = 0;
+#pragma unroll
+                for (int blk = 0; blk < RG::BLOCKS; ++blk) {
+                    const uint32_t page = __shfl_sync(0xffffffffu, pages, i % GROUP * RG::BLOCKS + blk);
+                    if (page >= a.kv.pages) continue;
+                    got |= 1u << blk;
+                    const size_t row = a.kv.row(page, head, (uint32_t)((block_of(i) + blk) * 16) & page_mask);
+                    copy_rows(to + blk * RG::ROWS, a.kv.k, row);
+                    copy_rows(to + RG::V + blk * RG::ROWS, a.kv.v, row);
+                    if (Q8 && lane < 8) {  // four pieces of either side's scales
+                        const float *from = (lane < 4 ? a.kv.ks : a.kv.vs) + row + 4 * (lane & 3);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                         smem_u32(to + (lane < 4 ? RG::KS : RG::VS) + blk * RG::SCALES) + 16 * (lane & 3)),
+                                     "l"(from));
+                    }
+                }
+                constexpr uint32_t ALL = (1u << RG::BLOCKS) - 1;
+                have = (have & ~(ALL << (put * RG::BLOCKS))) | got << (put * RG::BLOCKS);
+                put = put + 1 == RG::N ? 0 : put + 1;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < RG::N; ++i) issue(i);
 
-        // Q: the row's largest number to just below 2^14 (f16 q stays as it is)
         {
             const int r = tid / PER_ROW, c = tid % PER_ROW;
             const int rr = min(r0 + r, rows - 1), i = rr / (int)a.group, h = rr - i * (int)a.group;
             const int64_t at = (t0 + i) * a.q_token + (int64_t)(head * a.group + h) * a.q_head + c * E;
+            constexpr float kHuge = 3.402823466e38f;
             float x[E], m = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 x[e] = load1(a.q, (size_t)(at + e), a.q_type);
-                m = fmaxf(m, fabsf(x[e]));
+                m = fabsf(x[e]) <= kHuge ? fmaxf(m, fabsf(x[e])) : __int_as_float(0x7f800000);
             }
-            float f1 = 1.0f, f2 = 1.0f, undo = a.scale;
-            if (a.q_type != MGB_F16) {
+            float undo = a.scale;
+            if (Q8 || a.q_type != MGB_F16) {
 #pragma unroll
                 for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                // 2^shift in two factors, since either may leave the range of f32 alone
-                const int shift = m > 0.0f && m < __int_as_float(0x7f800000) ? 140 - (__float_as_int(m) >> 23) : 0;
-                const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
-                f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
-                undo = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
             }
+            if constexpr (Q8) {
+                // q as whole numbers over the row's largest; a row with an infinity or NaN gets an infinite scale, and
+                // so scores of NaN
+                constexpr float kMost = SPLIT ? 127 * 16384 + 8191 : 127 * 128 + 63;
+                const bool tiny = m < 1e-30f;  // as good as zeros, whose scores are 0
+                const float inv = tiny ? 0.0f : kMost / m;
+                undo = tiny ? a.scale : a.scale * (m / kMost);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float y = x[e] * f1 * f2;
-                const __half hi = __float2half_rn(y);
-                sq[0][r][c * E + e] = hi;
-                if constexpr (SPLIT) sq[1][r][c * E + e] = __float2half_rn(y - __half2float(hi));
+                for (int e = 0; e < E; ++e) {
+                    int v = __float2int_rn(x[e] * inv);
+                    if constexpr (SPLIT) {
+                        const int hi = (v + 8192) >> 14;
+                        sd[0][r][c * E + e] = (int8_t)hi;
+                        v -= hi << 14;
+                    }
+                    const int mid = (v + 64) >> 7;
+                    sd[DIGITS - 2][r][c * E + e] = (int8_t)mid;
+                    sd[DIGITS - 1][r][c * E + e] = (int8_t)(v - (mid << 7));
+                }
+            } else {
+                // the row's largest number to just below 2^14 (f16 q stays as it is)
+                float f1 = 1.0f, f2 = 1.0f;
+                if (a.q_type != MGB_F16) {
+                    // 2^shift in two factors, since either may leave the range of f32 alone
+                    const int shift = m > 0.0f && m <= kHuge ? 140 - (__float_as_int(m) >> 23) : 0;
+                    const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
+                    f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
+                    undo = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float y = x[e] * f1 * f2;
+                    const __half hi = __float2half_rn(y);
+                    sq[0][r][c * E + e] = hi;
+                    if constexpr (SPLIT) sq[SPLIT][r][c * E + e] = __float2half_rn(y - __half2float(hi));
+                }
             }
             if (c == 0) {
                 row_scale[r] = undo;
@@ -477,13 +559,21 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         st.all = row_limit[0];  // what the rows past `live` see does not matter
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            if constexpr (Q8) {
 #pragma unroll
-            for (int z = 0; z < (SPLIT ? 2 : 1); ++z)
+                for (int z = 0; z < DIGITS; ++z)
 #pragma unroll
-                for (int s = 0; s < F::STEPS; ++s) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(&sq[z][8 * j + g][F::k_dim(t, 4 * s)]);
-                    st.q[z][j][s][0] = x.x, st.q[z][j][s][1] = x.y;
-                }
+                    for (int s = 0; s < F::STEPS; ++s)
+                        st.q[z][j][s][0] = *reinterpret_cast<const uint32_t *>(&sd[z][8 * j + g][F::k_dim(t, 4 * s)]);
+            } else {
+#pragma unroll
+                for (int z = 0; z < (SPLIT ? 2 : 1); ++z)
+#pragma unroll
+                    for (int s = 0; s < F::STEPS; ++s) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(&sq[z][8 * j + g][F::k_dim(t, 4 * s)]);
+                        st.q[z][j][s][0] = x.x, st.q[z][j][s][1] = x.y;
+                    }
+            }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 st.scale[j][r] = row_scale[8 * j + 2 * t + r];
@@ -497,16 +587,15 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                 for (int e = 0; e < 4; ++e) st.o[j][s][e] = 0.0f;
         }
 
-        bool lost = false;  // a copy did not arrive in time: the rows become NaN
         for (int i = 0; i < mine; ++i) {
-            lost |= !mbar_wait(&full[warp][get], phase);
-            const uint32_t got = have[warp][get];
+            asm volatile("cp.async.wait_group %0;" ::"n"(RG::N - 1) : "memory");
+            __syncwarp();
+            const uint32_t got = (have >> (get * RG::BLOCKS)) & ((1u << RG::BLOCKS) - 1);
             if (got) st.step(ring + get * RG::STAGE, got, block_of(i) * 16, end, g, t);
             __syncwarp();  // every lane has read the stage
-            if (i + RG::N < mine) issue(i + RG::N);
-            if (++get == RG::N) get = 0, phase ^= 1;
+            issue(i + RG::N);
+            get = get + 1 == RG::N ? 0 : get + 1;
         }
-        if (lost) st.l[0][0] = st.l[0][1] = st.l[NT - 1][0] = st.l[NT - 1][1] = __int_as_float(0x7fffffff);
 
         // the CTA's warps
 #pragma unroll
@@ -585,8 +674,6 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
             const int rr = r0 + r, i = rr / (int)a.group, h = rr - i * (int)a.group;
             store1(a.out, (size_t)((t0 + i) * a.o_token + (int64_t)(head * a.group + h) * a.o_head + d), a.o_type, l == 0.0f ? 0.0f : sum / l);
         }
-        // the next tile's copies go where this one's outputs stood
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (parts > 1) cluster_sync();
         else __syncthreads();
     }
@@ -622,11 +709,12 @@ cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, c
     uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
     if (tiles * a.kv.heads > 65535) tiles = 65535 / a.kv.heads;
     const uint64_t base = tiles * a.kv.heads * a.seq.seqs;
-    uint32_t parts = 1;
-    while (parts < 16 && most_len / (parts * 2) >= kRowWarps * 32 &&
-           (base * parts * 2 <= SLOTS || most_len / parts > 2048))
-        parts *= 2;
-    return launch_rows<D, Q8, SPLIT, NT>(a, dim3(parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
+    uint64_t parts = base < SLOTS ? SLOTS / base : 1;
+    if (parts < most_len / 2048) parts = most_len / 2048;
+    if (parts > most_len / (kRowWarps * 32)) parts = most_len / (kRowWarps * 32);
+    // sizes that pack into the GPU's clusters of 16 or 18 SMs
+    parts = parts >= 16 ? 16 : parts >= 8 ? 8 : parts >= 4 ? 4 : parts < 1 ? 1 : parts;
+    return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
 }
 
 // 8-row tiles where a call has no more rows a cache head than that, else 16.
