@@ -142,14 +142,15 @@ struct Frag {
     static constexpr int VN = D * ESZ / 8 / VB;
     static constexpr int KW = D * ESZ / 16, VW = D * ESZ / 32 ? D * ESZ / 32 : 1;  // words of a key and lane
     static constexpr int STEPS = D / 16;
-    // place of 16-byte piece c of key `key` in its block of 16
-    static constexpr int PIECES = D * ESZ / 16;
-    static __device__ __forceinline__ int piece(int key, int c) {
-        const int turn = PIECES >= 8 ? ((key >> 1) & 3) << 1 ^ (key & 1) << 2 : PIECES == 4 ? key & 2 : 0;
-        return key * (D * ESZ) + (c ^ turn) * 16;
+    // Piece c (16 bytes) of key `key` stands at piece c ^ turn(key) of its row in a
+    // stage. turn is linear over xor, and so are the places that a lane's reads and
+    // copies derive from its first one.
+    static constexpr int PIECES = D * ESZ / 16, ROW = D * ESZ;
+    static __host__ __device__ constexpr int turn(int key) {
+        return PIECES >= 8 ? ((key >> 1) & 3) << 1 ^ (key & 1) << 2 : PIECES == 4 ? key & 2 : 0;
     }
     // place of byte b of key `key`'s row
-    static __device__ __forceinline__ int byte(int key, int b) { return piece(key, b / 16) + b % 16; }
+    static __device__ __forceinline__ int byte(int key, int b) { return key * ROW + ((b / 16 ^ turn(key)) * 16) + b % 16; }
     // CTAs of an SM that the registers have to leave room for
     static constexpr int ctas(int nt) { return D < 128 ? (nt == 1 ? 5 : 3) : nt == 2 && Q8 ? 2 : 3; }
     static constexpr int STATIC = 32 * D + 1536;  // static shared memory of a CTA a tile of 8 rows, at most
@@ -189,26 +190,26 @@ struct Block {  // a lane's share of 16 keys
     uint32_t v[4][Frag<D, Q8>::VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
     float ks[2], vs[2];              // scales of keys g, g + 8
     // left: keys that exist; the places of the others hold anything
-    __device__ __forceinline__ void load_k(const uint8_t *stage, int blk, int g, int t) {
+    // k_at, v_at: F::byte(g, t * KB), F::byte(2 * t, g * VB)
+    __device__ __forceinline__ void load_k(const uint8_t *stage, int blk, int g, int k_at) {
         using F = Frag<D, Q8>;
         using R = Ring<D, Q8>;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int c = 0; c < F::KN; ++c)
-                load_words<F::KB>(stage + blk * R::ROWS + F::byte(g + 8 * u, (t + 4 * c) * F::KB), &k[u][c * (F::KB / 4)]);
+                load_words<F::KB>(stage + blk * R::ROWS + 8 * u * F::ROW + (k_at ^ 64 * c), &k[u][c * (F::KB / 4)]);
             if constexpr (Q8) ks[u] = reinterpret_cast<const float *>(stage + R::KS)[16 * blk + g + 8 * u];
         }
     }
-    __device__ __forceinline__ void load_v(const uint8_t *stage, int blk, int left, int g, int t) {
+    __device__ __forceinline__ void load_v(const uint8_t *stage, int blk, int left, int g, int t, int v_at) {
         using F = Frag<D, Q8>;
         using R = Ring<D, Q8>;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int key = 2 * t + (u & 1) + 8 * (u >> 1);
 #pragma unroll
             for (int c = 0; c < F::VN; ++c)
-                load_words<F::VB>(stage + R::V + blk * R::ROWS + F::byte(key, (g + 8 * c) * F::VB), &v[u][c * (F::VB / 4)]);
+                load_words<F::VB>(stage + R::V + blk * R::ROWS + ((u & 1) + 8 * (u >> 1)) * F::ROW + (v_at ^ F::turn(u & 1) * 16 ^ 128 * c), &v[u][c * (F::VB / 4)]);
         }
         if constexpr (Q8) {
 #pragma unroll
@@ -260,6 +261,7 @@ struct Rows {
     float o[NT][F::STEPS][4];
     float m[NT][2], l[NT][2];
     int exp_v;  // V's scales so far are below 2^exp_v
+    int k_at, v_at;  // where the lane's reads of a stage begin
 
     // have: bit i, block i of the stage is in the cache; key0: the stage's first key
     __device__ __forceinline__ void step(const uint8_t *stage, uint32_t have, int key0, int end, int g, int t) {
@@ -273,7 +275,7 @@ struct Rows {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][n][e] = 0.0f;
             if (B > 1 && !((have >> i) & 1)) continue;
-            x[i].load_k(stage, i, g, t);
+            x[i].load_k(stage, i, g, k_at);
             if constexpr (Q8) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -320,15 +322,22 @@ struct Rows {
                 x[i].vs[0] = x[i].vs[1] = 0.0f;
                 continue;
             }
-            x[i].load_v(stage, i, end - key0 - 16 * i, g, t);
+            x[i].load_v(stage, i, end - key0 - 16 * i, g, t, v_at);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[i][n][e] *= Q8 ? scale[n][e & 1] * x[i].ks[e >> 1] : scale[n][e & 1];
-                    if (!whole && key0 + 16 * i + g + 8 * (e >> 1) >= limit[n][e & 1]) s[i][n][e] = kLowest;
-                    past |= s[i][n][e] > m[n][e & 1] + kSlack;
-                }
+                for (int e = 0; e < 4; ++e) s[i][n][e] *= Q8 ? scale[n][e & 1] * x[i].ks[e >> 1] : scale[n][e & 1];
+            if (!whole) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key0 + 16 * i + g + 8 * (e >> 1) >= limit[n][e & 1]) s[i][n][e] = kLowest;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) past |= s[i][n][e] > m[n][e & 1] + kSlack;
             if constexpr (Q8) d = fmaxf(d, fmaxf(fabsf(x[i].vs[0]), fabsf(x[i].vs[1])));
         }
         if constexpr (Q8) past |= (__float_as_int(d) >> 23) - 126 > exp_v;
@@ -369,10 +378,14 @@ struct Rows {
                 float w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool see = s[i][n][e] != kLowest;  // a masked key's scale may be NaN
                     w[e] = exp2_of(s[i][n][e] - z[e & 1]);
                     l[n][e & 1] += w[e];
-                    if constexpr (Q8) w[e] = whole || see ? w[e] * (x[i].vs[e >> 1] * back) : 0.0f;
+                    if constexpr (Q8) w[e] *= x[i].vs[e >> 1] * back;
+                }
+                if (Q8 && !whole) {  // a masked key's scale may be NaN
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (s[i][n][e] == kLowest) w[e] = 0.0f;
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -455,13 +468,14 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         uint32_t pages = 0;  // lane's: of block lane % BLOCKS of stage lane / BLOCKS of the group of stages in hand
         constexpr int GROUP = 32 / RG::BLOCKS;
         // 16 rows of K or V, 16 bytes a lane and access
-        auto copy_rows = [&](uint8_t *to, const void *base, size_t row) {
-            const uint8_t *src = static_cast<const uint8_t *>(base) + row * (D * F::ESZ) + 16 * lane;
+        constexpr int KEYS = F::PIECES < 32 ? 32 / F::PIECES : 1;  // of an access
+        const int copy_at = F::byte(lane / F::PIECES, lane % F::PIECES * 16);
+        auto copy_rows = [&](uint32_t to, const void *base, size_t row) {
+            const uint8_t *src = static_cast<const uint8_t *>(base) + row * F::ROW + 16 * lane;
 #pragma unroll
-            for (int u = 0; u < RG::ROWS / 16; u += 32)
-                if (RG::ROWS >= 512 || lane < RG::ROWS / 16)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to) + F::piece((u + lane) / F::PIECES, (u + lane) % F::PIECES)),
-                                 "l"(src + 16 * u));
+            for (int u = 0; u < 16; u += KEYS)
+                if (KEYS <= 16 || lane < 16 * F::PIECES)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * F::ROW + (copy_at ^ F::turn(u) * 16)), "l"(src + u * F::ROW));
         };
         auto issue = [&](int i) {  // one group of copies, empty past the last stage
             if (i < mine) {
@@ -469,7 +483,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                     const int blk = block_of(i + lane / RG::BLOCKS) + lane % RG::BLOCKS;
                     pages = blk < stop ? (uint32_t)__ldg(table + ((uint32_t)(blk * 16) >> a.kv.page_log2)) : 0xffffffffu;
                 }
-                uint8_t *to = ring + put * RG::STAGE;
+                const uint32_t to = smem_u32(ring) + put * RG::STAGE;
                 uint32_t got = 0;
 #pragma unroll
                 for (int blk = 0; blk < RG::BLOCKS; ++blk) {
@@ -482,7 +496,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                     if (Q8 && lane < 8) {  // four pieces of either side's scales
                         const float *from = (lane < 4 ? a.kv.ks : a.kv.vs) + row + 4 * (lane & 3);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                         smem_u32(to + (lane < 4 ? RG::KS : RG::VS) + blk * RG::SCALES) + 16 * (lane & 3)),
+                                         to + (lane < 4 ? RG::KS : RG::VS) + blk * RG::SCALES + 16 * (lane & 3)),
                                      "l"(from));
                     }
                 }
@@ -556,6 +570,8 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         __syncthreads();
         Rows<D, Q8, SPLIT, NT> st;
         st.exp_v = -126;
+        st.k_at = F::byte(g, t * F::KB);
+        st.v_at = F::byte(2 * t, g * F::VB);
         st.all = row_limit[0];  // what the rows past `live` see does not matter
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
