@@ -111,7 +111,7 @@ struct Shared {
     alignas(16) float k_scale[4][kKeys];
     int v_exp[4];       // V of the tile is over 2^v_exp
     uint32_t holes[4];  // bit i: keys 16 i .. 16 i + 15 of the tile have no page
-    float m[256], l[256];
+    float m[256], l[256], weight[8][256];
     uint32_t tmem;
     int lost;  // a wait ran out: nothing more is computed, the rows become NaN
 };
@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     int n;
     const int t0 = a.seq.first(b, n);
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
+    let_next_start();
     if ((uint32_t)rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
@@ -424,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     }
                 }
             } else {
-                // this CTA's part of the row where the keys stood, turned so that the warp's stores miss each other's banks
+                // this CTA's part of the row where the keys stood, turned by 16 bytes a row so that stores miss each
+                // other's banks
                 float *o = reinterpret_cast<float *>(smem + SM::K) + row * D;
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 16) {
@@ -432,7 +434,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     tmem_load16(o_at + c0, raw);
                     tmem_wait_load();
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[(c0 + c + row) % D] = has ? __uint_as_float(raw[c]) * back : 0.0f;
+                    for (int c = 0; c < 16; c += 4) {
+                        float4 x = make_float4(__uint_as_float(raw[c]) * back, __uint_as_float(raw[c + 1]) * back,
+                                               __uint_as_float(raw[c + 2]) * back, __uint_as_float(raw[c + 3]) * back);
+                        if (!has) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        reinterpret_cast<float4 *>(o)[((c0 + c) / 4 + row) % (D / 4)] = x;
+                    }
                 }
                 sh.m[row] = m;
                 sh.l[row] = l;
@@ -442,24 +449,40 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (parts > 1) {
                 namespace cg = cooperative_groups;
                 auto cluster = cg::this_cluster();
-                const float *o = reinterpret_cast<const float *>(smem + SM::K);
-                for (int u = (int)part * (kSoftWarps * 32) + tid; u < sp.live * (D / 4); u += (int)parts * (kSoftWarps * 32)) {
-                    const int r = u / (D / 4), c0 = u % (D / 4) * 4;
-                    float best = kLowest, sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (uint32_t c = 0; c < parts; ++c) best = fmaxf(best, *cluster.map_shared_rank(&sh.m[r], c));
-                    for (uint32_t c = 0; c < parts; ++c) {
-                        const float its = *cluster.map_shared_rank(&sh.m[r], c), lc = *cluster.map_shared_rank(&sh.l[r], c);
-                        const float f = its == kLowest ? 0.0f : exp2_of(its - best);
-                        sum += its == kLowest ? lc : f * lc;
-                        const float *from = cluster.map_shared_rank(o + r * D, c);
+                // the parts' weights of a row, over the row's sum
+                if (row < sp.live) {
+                    float its[8], sum = 0.0f, best = kLowest;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] += f * from[(c0 + e + r) % D];
+                    for (int c = 0; c < 8; ++c) {
+                        its[c] = c < (int)parts ? *cluster.map_shared_rank(&sh.m[row], c) : kLowest;
+                        best = fmaxf(best, its[c]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = sum < 1e-30f ? 0.0f : x[e] / sum;
+                    for (int c = 0; c < 8; ++c) {
+                        const float lc = c < (int)parts ? *cluster.map_shared_rank(&sh.l[row], c) : 0.0f;
+                        its[c] = its[c] == kLowest ? 0.0f : exp2_of(its[c] - best);
+                        sum += lc != lc ? lc : its[c] * lc;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) sh.weight[c][row] = sum < 1e-30f ? 0.0f : sum != sum ? sum : its[c] / sum;
+                }
+                asm volatile("barrier.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+                const float4 *o = reinterpret_cast<const float4 *>(smem + SM::K);
+                for (int u = (int)part * (kSoftWarps * 32) + tid; u < sp.live * (D / 4); u += (int)parts * (kSoftWarps * 32)) {
+                    const int r = u / (D / 4), c4 = u % (D / 4);
+                    float4 from[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        from[c] = c < (int)parts ? *cluster.map_shared_rank(o + r * (D / 4) + (c4 + r) % (D / 4), c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float f = sh.weight[c][r];
+                        x[0] += f * from[c].x, x[1] += f * from[c].y, x[2] += f * from[c].z, x[3] += f * from[c].w;
+                    }
                     const int rr = sp.r0 + r;
                     const int i = rr / (int)a.group, h = rr - i * (int)a.group;
-                    store4(a.out, (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + c0, a.o_type, a.o_vec, x);
+                    store4(a.out, (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + 4 * c4, a.o_type, a.o_vec, x);
                 }
                 meet(true);
             }

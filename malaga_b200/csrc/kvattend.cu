@@ -108,6 +108,11 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
     }
 }
 
+// Programmatic dependent launch: the next kernel may start once every CTA of this one has; wait until the one before
+// has ended.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // Few rows: tiles of 8 or 16 rows (token, head of the group) of one cache head.
 //
@@ -448,7 +453,12 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
-    if ((uint32_t)rows > a.few) return;
+    // After a launch for many rows, which this one may overlap, one CTA sees to it that this kernel does not end first.
+    const bool keeper = blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && b == gridDim.z - 1;
+    if ((uint32_t)rows > a.few) {
+        if (keeper) wait_for_previous();
+        return;
+    }
     uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
     uint32_t put = 0, get = 0;  // next stage to fill and to read
     uint32_t have = 0;          // BLOCKS bits a stage: which of its blocks are in the cache
@@ -693,10 +703,11 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         if (parts > 1) cluster_sync();
         else __syncthreads();
     }
+    if (keeper) wait_for_previous();
 }
 
 template <int D, bool Q8, bool SPLIT, int NT>
-cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, dim3 grid, bool overlap, cudaStream_t s) {
     constexpr int SMEM = Ring<D, Q8>::BYTES;
     static std::atomic<bool> done[kMaxDevices];
     cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT, NT>, SMEM, true, done);
@@ -706,12 +717,19 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
     c.blockDim = dim3(kRowThreads);
     c.dynamicSmemBytes = SMEM;
     c.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = grid.x;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
     c.attrs = at;
-    c.numAttrs = grid.x > 1 ? 1 : 0;
+    if (grid.x > 1) {
+        at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[c.numAttrs].val.clusterDim.x = grid.x;
+        at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
+        ++c.numAttrs;
+    }
+    if (overlap) {
+        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++c.numAttrs;
+    }
     return cudaLaunchKernelEx(&c, attend_rows_kernel<D, Q8, SPLIT, NT>, a);
 }
 
@@ -719,7 +737,7 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
 // at once and every warp keeps two blocks, and further while a CTA would have
 // more than 2048 keys: sequences of unlike lengths then even out.
 template <int D, bool Q8, bool SPLIT, int NT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
     constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, FIT = 227 * 1024 / SMEM;
     constexpr int SLOTS = 148 * (FIT < Frag<D, Q8>::ctas(NT) ? FIT : Frag<D, Q8>::ctas(NT));
     uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
@@ -730,28 +748,29 @@ cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, c
     if (parts > most_len / (kRowWarps * 32)) parts = most_len / (kRowWarps * 32);
     // sizes that pack into the GPU's clusters of 16 or 18 SMs
     parts = parts >= 16 ? 16 : parts >= 8 ? 8 : parts >= 4 ? 4 : parts < 1 ? 1 : parts;
-    return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
+    return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), overlap, s);
 }
 
 // 8-row tiles where a call has no more rows a cache head than that, else 16.
 template <int D, bool Q8, bool SPLIT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
-    const uint64_t rows = most_new * a.group;
-    return rows <= 8 ? launch_rows<D, Q8, SPLIT, 1>(a, rows, most_len, s) : launch_rows<D, Q8, SPLIT, 2>(a, rows, most_len, s);
+cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
+    return rows <= 8 ? launch_rows<D, Q8, SPLIT, 1>(a, rows, most_len, overlap, s)
+                     : launch_rows<D, Q8, SPLIT, 2>(a, rows, most_len, overlap, s);
 }
 
 template <int D>
-cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
     if (a.q_type == MGB_F32)
-        return q8 ? launch_rows<D, true, true>(a, most_new, most_len, s) : launch_rows<D, false, true>(a, most_new, most_len, s);
-    return q8 ? launch_rows<D, true, false>(a, most_new, most_len, s) : launch_rows<D, false, false>(a, most_new, most_len, s);
+        return q8 ? launch_rows<D, true, true>(a, rows, most_len, overlap, s) : launch_rows<D, false, true>(a, rows, most_len, overlap, s);
+    return q8 ? launch_rows<D, true, false>(a, rows, most_len, overlap, s) : launch_rows<D, false, false>(a, rows, most_len, overlap, s);
 }
 
 #include "attend_tiles.cuh"
 
-// A row tile's keys are cut over the CTAs of a cluster (at most 8) while that
-// fills SMs that would stay idle (one CTA an SM, 148 SMs) and leaves each CTA
-// four key tiles.
+// A row tile's keys are cut over the CTAs of a cluster, in as many parts as make
+// the shortest: rounds of CTAs (one an SM, 148 SMs) times the key tiles of a CTA,
+// with four more for its beginning and end and two to join parts. The row tiles are estimated from all
+// rows and half a tile a sequence, since lengths are only known on the device.
 template <int D, bool Q8>
 cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
@@ -759,9 +778,15 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
     if (e != cudaSuccess) return e;
     uint64_t row_tiles = (most_new * a.group + 255) / 256;
     if (row_tiles * a.kv.heads > 65535) row_tiles = 65535 / a.kv.heads;
-    const uint64_t base = row_tiles * a.kv.heads * a.seq.seqs;
+    const uint64_t some = ((uint64_t)a.seq.tokens * a.group + 255) / 256 + a.seq.seqs / 2;
+    const uint64_t base = a.kv.heads * (some < row_tiles * a.seq.seqs ? some : row_tiles * a.seq.seqs);
+    const uint64_t key_tiles = (most_len + tiles::kKeys - 1) / tiles::kKeys;
     uint32_t parts = 1;
-    while (parts < 8 && base * parts * 2 <= 148 && most_len / (parts * 2) >= 4 * tiles::kKeys) parts *= 2;
+    uint64_t best = ~0ull;
+    for (uint32_t p = 1; p <= 8 && (p == 1 || key_tiles >= 4 * p); p *= 2) {
+        const uint64_t cost = (base * p + 147) / 148 * ((key_tiles + p - 1) / p + 4 + (p > 1 ? 2 : 0));
+        if (cost < best) best = cost, parts = p;
+    }
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(parts, (unsigned)(row_tiles * a.kv.heads), a.seq.seqs);
     c.blockDim = dim3(tiles::kThreads);
@@ -780,12 +805,12 @@ template <int D>
 cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
     // Sequences of more than 64 rows a cache head go to the tensor-core tiles, but
     // for f32 queries, whose two f16 parts only the other kernel takes.
-    if (a.q_type == MGB_F32 || most_new * a.group <= kFewRows) return launch_rows<D>(a, q8, most_new, most_len, s);
+    if (a.q_type == MGB_F32 || most_new * a.group <= kFewRows) return launch_rows<D>(a, q8, most_new * a.group, most_len, false, s);
     a.few = kFewRows;
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
     // sequences of unlike lengths: there may be some of few rows
     if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs)
-        e = launch_rows<D>(a, q8, (kFewRows + a.group - 1) / a.group, most_len, s);
+        e = launch_rows<D>(a, q8, kFewRows, most_len, true, s);
     return e;
 }
 
