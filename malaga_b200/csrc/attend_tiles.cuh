@@ -146,13 +146,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
 
 // What all roles of a CTA know of its row tile.
 struct Span {
-    int r0, live;      // its first row, its rows
+    int r0, live, groups;  // its first row; rows of the tile; 128-row groups that have some
     int end, all;      // keys that its last row sees; keys that every row sees
     int first, count;  // its part's key tiles
-    // At most 128 rows: both groups take them, and of the key tiles every other one.
-    bool split;
-    __device__ __forceinline__ int tiles(int g) const { return split ? (count - g + 1) / 2 : count; }
-    __device__ __forceinline__ int tile(int g, int j) const { return split ? 2 * j + g : j; }  // the group's j-th
 };
 
 template <int D, bool Q8>
@@ -200,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         Span s;
         s.r0 = (int)(row_tiles - 1 - rt) * 256;
         s.live = min(256, rows - s.r0);
-        s.split = s.live <= 128;
+        s.groups = s.live > 128 ? 2 : 1;
         s.end = limit((s.r0 + s.live - 1) / (int)a.group);
         s.all = limit(s.r0 / (int)a.group);
         const int total = (s.end + kKeys - 1) / kKeys;
@@ -221,28 +217,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     auto next_tile = [&](const Span &s) {
         ks += s.count;
         os += s.count > 0;
-        ss[0] += s.tiles(0);
-        ss[1] += s.tiles(1);
+        ss[0] += s.count;
+        ss[1] += s.groups > 1 ? s.count : 0;
         ++turns;
     };
 
     if (warp < kSoftWarps) {
         // ---------------------------------------------------------- softmax
         more_registers<kSoftRegs>();
-        const int group = warp >> 2;
+        const int group = warp >> 2, row = tid;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor-memory lanes of the warp
         const uint32_t s_at = tmem + lanes + group * 128, o_at = tmem + lanes + 256 + group * D;
         uint8_t *mine = smem + SM::Q + group * SM::TILE + (warp & 3) * (32 * D * 2);  // the warp's 32 rows of Q
         for (uint32_t rt = tile0; rt < row_tiles; rt += tile_step) {
             const Span sp = span_of(rt);
-            const int warp_row = 32 * (sp.split ? warp & 3 : warp), row = warp_row + lane;
             // Q of the warp's rows, eight at a time, four lanes a row; bf16 rows scaled by a power of two to just below 2^14
             float scale = 0.0f;
             {
                 constexpr int PIECES = D / 8, PER = PIECES < 4 ? 1 : PIECES / 4;
                 auto fetch = [&](int q, uint4 (&raw)[PER]) {
                     // rows past the last read it again; their scores are masked
-                    const int rr = min(sp.r0 + warp_row + 8 * q + (lane & 7), rows - 1), i = rr / (int)a.group, h = rr - i * (int)a.group;
+                    const int rr = min(sp.r0 + 32 * warp + 8 * q + (lane & 7), rows - 1), i = rr / (int)a.group, h = rr - i * (int)a.group;
                     const uint16_t *from = static_cast<const uint16_t *>(a.q) + (t0 + i) * a.q_token + (long long)(head * a.group + h) * a.q_head;
                     if (a.q_vec16) {
 #pragma unroll
@@ -304,16 +299,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             float m = kLowest, l = 0.0f;
             int exp_v = -126;
             bool ok = !sh.lost;
-            const int count = sp.tiles(group);
+            const int count = group < sp.groups ? sp.count : 0;
             for (int j = 0; j < count && ok; ++j) {
-                const int tile = sp.tile(group, j), key0 = (sp.first + tile) * kKeys;
+                const int key0 = (sp.first + j) * kKeys;
                 ok = wait(&sh.s_full[group], ss[group] + j);
                 if (!ok) break;
                 fence_after();
                 float2 x[kKeys / 2];
 #pragma unroll
                 for (int c0 = 0; c0 < kKeys; c0 += 32) tmem_load32(s_at + c0, reinterpret_cast<uint32_t *>(&x[c0 / 2]));
-                const uint32_t slot = (ks + tile) & 3, holes = sh.holes[slot];
+                const uint32_t slot = (ks + j) & 3, holes = sh.holes[slot];
                 const float *kscale = sh.k_scale[slot];
                 auto rescale_o = [&](float f) {
 #pragma unroll 1
@@ -382,8 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (!ok) l = __int_as_float(0x7fffffff);
             const float back = Q8 ? power_of_2(exp_v) : 1.0f;
             const bool has = count > 0;
-            const bool join = parts > 1 || sp.split;
-            if (!join) {
+            if (parts == 1) {
                 const bool some = has && !(l < 1e-30f);  // a row that sees nothing has at most 128 times 2^-126 a tile
                 const float f = some ? back / l : 0.0f;
                 if (a.o_vec16) {
@@ -408,8 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 4
                     for (int u = lane; u < 32 * PIECES; u += 32) {
                         const int r = u / PIECES, c = u % PIECES;
-                        const int rr = sp.r0 + warp_row + r;
-                        if (warp_row + r >= sp.live) break;
+                        const int rr = sp.r0 + 32 * warp + r;
+                        if (32 * warp + r >= sp.live) break;
                         const int i = rr / (int)a.group, h = rr - i * (int)a.group;
                         const int64_t to = (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + 8 * c;
                         *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to) = *reinterpret_cast<const uint4 *>(mine + piece<D>(r, c));
@@ -433,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             } else {
                 // this CTA's part of the row where the keys stood, turned by 16 bytes a row so that stores miss each
                 // other's banks
-                float *o = reinterpret_cast<float *>(smem + SM::K) + tid * D;
+                float *o = reinterpret_cast<float *>(smem + SM::K) + row * D;
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 16) {
                     uint32_t raw[16];
@@ -444,56 +438,53 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         float4 x = make_float4(__uint_as_float(raw[c]) * back, __uint_as_float(raw[c + 1]) * back,
                                                __uint_as_float(raw[c + 2]) * back, __uint_as_float(raw[c + 3]) * back);
                         if (!has) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        reinterpret_cast<float4 *>(o)[((c0 + c) / 4 + tid) % (D / 4)] = x;
+                        reinterpret_cast<float4 *>(o)[((c0 + c) / 4 + row) % (D / 4)] = x;
                     }
                 }
-                sh.m[tid] = m;
-                sh.l[tid] = l;
+                sh.m[row] = m;
+                sh.l[row] = l;
             }
             fence_before();
             meet(parts > 1);
-            if (join) {
+            if (parts > 1) {
                 namespace cg = cooperative_groups;
                 auto cluster = cg::this_cluster();
-                // the weights of a row's shares (of the cluster's CTAs, of both groups) over its sum
-                const int shares = sp.split ? 2 : 1;
-                if (tid < sp.live) {
-                    float best = kLowest, sum = 0.0f;
-                    for (int k = 0; k < shares; ++k)
-                        for (uint32_t c = 0; c < parts; ++c) best = fmaxf(best, *cluster.map_shared_rank(&sh.m[128 * k + tid], c));
-                    for (int k = 0; k < shares; ++k)
-                        for (uint32_t c = 0; c < parts; ++c) {
-                            const float its = *cluster.map_shared_rank(&sh.m[128 * k + tid], c), lc = *cluster.map_shared_rank(&sh.l[128 * k + tid], c);
-                            const float f = its == kLowest ? 0.0f : exp2_of(its - best);
-                            sum += lc != lc ? lc : f * lc;
-                            sh.weight[c][128 * k + tid] = f;
-                        }
-                    const float over = sum < 1e-30f ? 0.0f : 1.0f / sum;
-                    for (int k = 0; k < shares; ++k)
-                        for (uint32_t c = 0; c < parts; ++c) sh.weight[c][128 * k + tid] *= over;
+                // the parts' weights of a row, over the row's sum
+                if (row < sp.live) {
+                    float its[8], sum = 0.0f, best = kLowest;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        its[c] = c < (int)parts ? *cluster.map_shared_rank(&sh.m[row], c) : kLowest;
+                        best = fmaxf(best, its[c]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float lc = c < (int)parts ? *cluster.map_shared_rank(&sh.l[row], c) : 0.0f;
+                        its[c] = its[c] == kLowest ? 0.0f : exp2_of(its[c] - best);
+                        sum += lc != lc ? lc : its[c] * lc;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) sh.weight[c][row] = sum < 1e-30f ? 0.0f : sum != sum ? sum : its[c] / sum;
                 }
                 asm volatile("barrier.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
                 const float4 *o = reinterpret_cast<const float4 *>(smem + SM::K);
                 for (int u = (int)part * (kSoftWarps * 32) + tid; u < sp.live * (D / 4); u += (int)parts * (kSoftWarps * 32)) {
                     const int r = u / (D / 4), c4 = u % (D / 4);
+                    float4 from[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        from[c] = c < (int)parts ? *cluster.map_shared_rank(o + r * (D / 4) + (c4 + r) % (D / 4), c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int k = 0; k < shares; ++k) {
-                        const int from_row = 128 * k + r;
-                        float4 from[8];
 #pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            from[c] = c < (int)parts ? *cluster.map_shared_rank(o + from_row * (D / 4) + (c4 + from_row) % (D / 4), c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const float f = c < (int)parts ? sh.weight[c][from_row] : 0.0f;
-                            x[0] += f * from[c].x, x[1] += f * from[c].y, x[2] += f * from[c].z, x[3] += f * from[c].w;
-                        }
+                    for (int c = 0; c < 8; ++c) {
+                        const float f = sh.weight[c][r];
+                        x[0] += f * from[c].x, x[1] += f * from[c].y, x[2] += f * from[c].z, x[3] += f * from[c].w;
                     }
                     const int rr = sp.r0 + r;
                     const int i = rr / (int)a.group, h = rr - i * (int)a.group;
                     store4(a.out, (t0 + i) * a.o_token + (long long)(head * a.group + h) * a.o_head + 4 * c4, a.o_type, a.o_vec, x);
                 }
-                meet(parts > 1);
+                meet(true);
             }
             next_tile(sp);
         }
@@ -664,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             meet(parts > 1);
-            if (parts > 1 || sp.split) meet(parts > 1);
+            if (parts > 1) meet(true);
             next_tile(sp);
         }
     } else {
@@ -676,46 +667,42 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (warp == kMmaWarp && lane == 0) {
                 const uint64_t q0 = operand(smem_u32(smem + SM::Q), 128, D * 16), k0 = operand(smem_u32(smem + SM::K), 128, D * 16);
                 const uint64_t v0 = operand(smem_u32(smem + SM::V), D * 16, 128);
-                // scores of the group's j-th tile
                 auto scores = [&](int g, int j) {
-                    const uint32_t stage = (ks + sp.tile(g, j)) & 1;
+                    const uint32_t stage = (ks + j) & 1;
                     const uint64_t q = q0 + g * (SM::TILE >> 4), k = k0 + stage * (SM::TILE >> 4);
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s) mma_ss(tmem + g * 128, q + s * 16, k + s * 16, QK, s > 0);
                     commit(&sh.s_full[g]);
                     commit(&sh.k_free[stage]);
-                    if (sp.split) commit(&sh.k_free[stage]);  // the other group does not read it
+                    if (sp.groups == 1) commit(&sh.k_free[stage]);
                 };
-                auto has_come = [&](uint64_t (&bar)[2], int tile) { return mbar_test(&bar[(ks + tile) & 1], ((ks + tile) >> 1) & 1); };
                 bool ok = mbar_wait(&sh.q_full, turns & 1);
                 if (sp.count > 0) {
-                    // Of each group the next tile of scores and of values. Either goes out as soon as it can: values that
-                    // waited for the next keys could wait for ever, since those may need the room of these values.
-                    int next_s[2] = {0, 0}, next_v[2] = {0, 0};
+                    ok = ok && mbar_wait(&sh.k_full[ks & 1], (ks >> 1) & 1);
+                    if (ok) {
+                        fence_after();
+                        for (int g = 0; g < sp.groups; ++g) scores(g, 0);
+                    }
+                    int next[2] = {0, sp.groups > 1 ? 0 : sp.count};  // the groups' next tile of values
                     uint64_t since = globaltimer();
-                    while (ok && (next_v[0] < sp.tiles(0) || next_v[1] < sp.tiles(1))) {
+                    while (ok && (next[0] < sp.count || next[1] < sp.count)) {
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const int j = next_v[g], count = sp.tiles(g), tile = sp.tile(g, j);
-                            if (next_s[g] > j && mbar_test(&sh.p_full[g], (ss[g] + j) & 1) && has_come(sh.v_full, tile)) {
-                                fence_after();
-                                const uint32_t stage = (ks + tile) & 1;
-                                const uint64_t v = v0 + stage * (SM::TILE >> 4);
+                            const int j = next[g];
+                            const uint32_t i = ks + j, stage = i & 1;
+                            if (j == sp.count || !mbar_test(&sh.p_full[g], (ss[g] + j) & 1) || !mbar_test(&sh.v_full[stage], (i >> 1) & 1) ||
+                                (j + 1 < sp.count && !mbar_test(&sh.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1)))
+                                continue;
+                            fence_after();
+                            const uint64_t v = v0 + stage * (SM::TILE >> 4);
 #pragma unroll
-                                for (int s = 0; s < kKeys / 16; ++s)
-                                    mma_ts(tmem + 256 + g * D, tmem + g * 128 + s * 8, v + s * (2 * D), PV, j > 0 || s > 0);
-                                commit(&sh.v_free[stage]);
-                                if (sp.split) commit(&sh.v_free[stage]);
-                                next_v[g] = j + 1;
-                                since = globaltimer();
-                            }
-                            // the scores take the place of P, so they follow its product
-                            if (next_s[g] == next_v[g] && next_s[g] < count && has_come(sh.k_full, sp.tile(g, next_s[g]))) {
-                                fence_after();
-                                scores(g, next_s[g]);
-                                next_s[g] += 1;
-                                since = globaltimer();
-                            }
+                            for (int s = 0; s < kKeys / 16; ++s)
+                                mma_ts(tmem + 256 + g * D, tmem + g * 128 + s * 8, v + s * (2 * D), PV, j > 0 || s > 0);
+                            commit(&sh.v_free[stage]);
+                            if (sp.groups == 1) commit(&sh.v_free[stage]);
+                            if (j + 1 < sp.count) scores(g, j + 1);
+                            next[g] = j + 1;
+                            since = globaltimer();
                         }
                         if (globaltimer() - since > kWaitNs || *reinterpret_cast<volatile int *>(&sh.lost)) ok = false;
                     }
@@ -728,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             __syncwarp();
             fence_before();
             meet(parts > 1);
-            if (parts > 1 || sp.split) meet(parts > 1);
+            if (parts > 1) meet(true);
             next_tile(sp);
         }
         if (warp == kMmaWarp) {

@@ -24,7 +24,6 @@
 //    eighth of the error of P's rounding; three, for f32 q, to 2^-22. The sums
 //    are exact.
 #include <cooperative_groups.h>
-#include <cstdlib>
 
 #include "numerics.cuh"
 #include "serving.cuh"
@@ -171,7 +170,7 @@ struct Frag {
     }
 };
 
-static const int kFewRows = getenv("MGB_FEW") ? atoi(getenv("MGB_FEW")) : 64;  // DEV
+constexpr int kFewRows = 64;
 constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
 constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
 constexpr float kRaise = 7.0f;  // p is held as 2^7 p, up to 2^15
