@@ -170,6 +170,8 @@ struct Frag {
     }
 };
 
+// Sequences of at most kFewRows rows a cache head go to the kernel for few rows;
+// the others to the tensor-core tiles, but where that takes longer (launch()).
 constexpr int kFewRows = 64;
 constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
 constexpr float kSlack = 8.0f;  // a score may pass the running maximum by 2^8
@@ -769,8 +771,23 @@ cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t rows, uint64_t mo
 
 // A row tile's keys are cut over the CTAs of a cluster, in as many parts as make
 // the shortest: rounds of CTAs (one an SM, 148 SMs) times the key tiles of a CTA,
-// with four more for its beginning and end and two to join parts. The row tiles are estimated from all
-// rows and half a tile a sequence, since lengths are only known on the device.
+// with four more for its beginning and end and two to join parts. The row tiles
+// are estimated from all rows and half a tile a sequence, since lengths are only
+// known on the device. Returns the key tiles one after another.
+uint64_t tiles_cost(const AttendArgs &a, uint64_t most_new, uint64_t most_len, uint32_t &parts) {
+    const uint64_t most = a.seq.seqs * ((most_new * a.group + 255) / 256);
+    const uint64_t some = ((uint64_t)a.seq.tokens * a.group + 255) / 256 + a.seq.seqs / 2;
+    const uint64_t base = a.kv.heads * (some < most ? some : most);
+    const uint64_t key_tiles = (most_len + tiles::kKeys - 1) / tiles::kKeys;
+    uint64_t best = ~0ull;
+    parts = 1;
+    for (uint32_t p = 1; p <= 8 && (p == 1 || key_tiles >= 4 * p); p *= 2) {
+        const uint64_t cost = (base * p + 147) / 148 * ((key_tiles + p - 1) / p + 4 + (p > 1 ? 2 : 0));
+        if (cost < best) best = cost, parts = p;
+    }
+    return best;
+}
+
 template <int D, bool Q8>
 cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
@@ -778,15 +795,8 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
     if (e != cudaSuccess) return e;
     uint64_t row_tiles = (most_new * a.group + 255) / 256;
     if (row_tiles * a.kv.heads > 65535) row_tiles = 65535 / a.kv.heads;
-    const uint64_t some = ((uint64_t)a.seq.tokens * a.group + 255) / 256 + a.seq.seqs / 2;
-    const uint64_t base = a.kv.heads * (some < row_tiles * a.seq.seqs ? some : row_tiles * a.seq.seqs);
-    const uint64_t key_tiles = (most_len + tiles::kKeys - 1) / tiles::kKeys;
-    uint32_t parts = 1;
-    uint64_t best = ~0ull;
-    for (uint32_t p = 1; p <= 8 && (p == 1 || key_tiles >= 4 * p); p *= 2) {
-        const uint64_t cost = (base * p + 147) / 148 * ((key_tiles + p - 1) / p + 4 + (p > 1 ? 2 : 0));
-        if (cost < best) best = cost, parts = p;
-    }
+    uint32_t parts;
+    tiles_cost(a, most_new, most_len, parts);
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(parts, (unsigned)(row_tiles * a.kv.heads), a.seq.seqs);
     c.blockDim = dim3(tiles::kThreads);
@@ -801,16 +811,28 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
     return cudaLaunchKernelEx(&c, tiles::attend_tiles_kernel<D, Q8>, a);
 }
 
+// Which kernel. f32 queries, whose two f16 parts only the kernel for few rows
+// takes, and calls of at most kFewRows rows a cache head go there. So do calls of
+// at most 256 rows where it is faster, which measurements at dims 64 and 128 (100
+// and 200 new tokens, 300 to 30,000 positions, 2 to 16 heads, 1 to 16 sequences)
+// put as: it takes 4 us and (dim + 16) / 80 us for every 28,500 pairs of a 16-row
+// tile and a key, the tiles 1.3 + dim / 70 us for each of tiles_cost's key tiles.
+// 100 rows over 4000 positions, 16 heads of 64: 24 against 34 us; over 1500 in 16
+// sequences 93 against 68.
 template <int D>
 cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
-    // Sequences of more than 64 rows a cache head go to the tensor-core tiles, but
-    // for f32 queries, whose two f16 parts only the other kernel takes.
-    if (a.q_type == MGB_F32 || most_new * a.group <= kFewRows) return launch_rows<D>(a, q8, most_new * a.group, most_len, false, s);
+    const uint64_t rows = most_new * a.group;
+    bool few = a.q_type == MGB_F32 || rows <= kFewRows;
+    if (!few && rows <= 256) {
+        uint32_t parts;
+        const double pairs = (double)((rows + 15) / 16 * a.kv.heads * a.seq.seqs) * (double)most_len;
+        few = 4.0 + pairs / 28500.0 * ((D + 16) / 80.0) < (double)tiles_cost(a, most_new, most_len, parts) * (1.3 + D / 70.0);
+    }
+    if (few) return launch_rows<D>(a, q8, rows, most_len, false, s);
     a.few = kFewRows;
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
     // sequences of unlike lengths: there may be some of few rows
-    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs)
-        e = launch_rows<D>(a, q8, kFewRows, most_len, true, s);
+    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs) e = launch_rows<D>(a, q8, kFewRows, most_len, true, s);
     return e;
 }
 

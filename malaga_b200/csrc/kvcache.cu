@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 4;       // rows of a thread in flight
-constexpr int kMaxTokens = 16;  // tokens of a CTA
+constexpr int kMaxTokens = 256;  // tokens of a CTA, at most its threads
 
 #define kInf __int_as_float(0x7f800000)
 #define kNan __int_as_float(0x7fffffff)
@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     }
 }
 
-// As many tokens a CTA as leave two CTAs an SM (148 SMs) on either side, at
-// most kMaxTokens.
+// As many tokens a CTA as leave two CTAs an SM (148 SMs) on either side, so that
+// all run at once and look their places up once.
 template <int DIM, bool Q8, bool WRITE>
 cudaError_t launch(MoveArgs a, int sides, int type, bool vec, cudaStream_t s) {
     const uint32_t n = a.seq.tokens / (2 * 148);
