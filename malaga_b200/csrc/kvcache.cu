@@ -4,8 +4,8 @@
 // A CTA takes a run of the call's tokens: its threads first look up each
 // token's place (a search for its sequence, then the page table), then move the
 // rows of all heads, K and V. A row is spread over dim / 8 lanes of 8 numbers;
-// the lanes' pieces are laid out so that a warp's accesses to the packed rows
-// are contiguous for 32-bit and for 16-bit numbers. Tokens are cut evenly over
+// the lanes' pieces are laid out so that a warp's 16-byte accesses to the packed
+// rows are contiguous for 32-bit and for 16-bit numbers. Tokens are cut evenly over
 // the CTAs whatever the sequences' lengths.
 #include "serving.cuh"
 
@@ -13,8 +13,7 @@ namespace mgb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;       // rows of a thread in flight
-constexpr int kMaxTokens = 256;  // tokens of a CTA, at most its threads
+constexpr int kMaxTokens = 32;  // tokens of a CTA, at most its threads (16 to 32 measured best of 4 to 64)
 
 #define kInf __int_as_float(0x7f800000)
 #define kNan __int_as_float(0x7fffffff)
@@ -66,9 +65,42 @@ __device__ __forceinline__ void values_of(uint32_t codes, float d, float *x) {
     for (int e = 0; e < 4; ++e) x[e] = d * (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + e)) - 8388736.0f);
 }
 
+// A lane's eight numbers of the row at `at`: two pieces of four, or one of eight.
+template <int TYPE, bool VEC, bool APART>
+__device__ __forceinline__ void load_pieces(const void *rows, int64_t at, int p0, int p1, float (&x)[8]) {
+    if constexpr (VEC && TYPE != MGB_F32 && !APART) {
+        const uint4 h = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(rows) + at + p0);
+        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = TYPE == MGB_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[e]))
+                                             : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+            x[2 * e] = f.x, x[2 * e + 1] = f.y;
+        }
+    } else {
+        load4(rows, at + p0, TYPE, VEC, &x[0]);
+        load4(rows, at + p1, TYPE, VEC, &x[4]);
+    }
+}
+
+template <int TYPE, bool VEC, bool APART>
+__device__ __forceinline__ void store_pieces(void *rows, int64_t at, int p0, int p1, const float (&x)[8]) {
+    if constexpr (VEC && TYPE != MGB_F32 && !APART) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = to_16(x[2 * e], TYPE) | (uint32_t)to_16(x[2 * e + 1], TYPE) << 16;
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(rows) + at + p0) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        store4(rows, at + p0, TYPE, VEC, &x[0]);
+        store4(rows, at + p1, TYPE, VEC, &x[4]);
+    }
+}
+
 template <int DIM, bool Q8, bool WRITE, int TYPE, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     constexpr int LANES = DIM / 8, ROWS = kThreads / LANES;
+    // rows of a thread in flight: more cost warps of an SM (reading, 1 / 2 / 4: 67 / 75 / 89 us; writing 87 / 77 / 77)
+    constexpr int kBatch = WRITE ? 2 : 1;
     __shared__ int64_t place[kMaxTokens];  // row of head 0 in the cache, -1 where there is none
     const uint32_t first = blockIdx.x * a.per_cta, tokens = min(a.per_cta, a.seq.tokens - first);
     if (threadIdx.x < tokens) {
@@ -98,8 +130,9 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     uint8_t *data = side.data;
     float *scale = side.scale;
     // a lane's two pieces of four numbers: apart for 32-bit rows, side by side for 16-bit ones
+    constexpr bool APART = TYPE == MGB_F32;
     const int lane = threadIdx.x % LANES;
-    const int p0 = TYPE == MGB_F32 ? 4 * lane : 8 * lane, p1 = TYPE == MGB_F32 ? DIM / 2 + 4 * lane : 8 * lane + 4;
+    const int p0 = APART ? 4 * lane : 8 * lane, p1 = APART ? DIM / 2 + 4 * lane : 8 * lane + 4;
     const uint32_t heads = a.kv.heads, total = tokens * heads;
 
     for (uint32_t r0 = 0; r0 < total; r0 += ROWS * kBatch) {
@@ -115,24 +148,24 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
             for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
             if (row[u] < 0) continue;
             if constexpr (WRITE) {
-                load4(rows, at[u] + p0, TYPE, VEC, &x[u][0]);
-                load4(rows, at[u] + p1, TYPE, VEC, &x[u][4]);
+                load_pieces<TYPE, VEC, APART>(rows, at[u], p0, p1, x[u]);
             } else if constexpr (Q8) {
                 const uint8_t *c = data + row[u] * DIM;
                 const float d = scale[row[u]];
-                values_of(*reinterpret_cast<const uint32_t *>(c + p0), d, &x[u][0]);
-                values_of(*reinterpret_cast<const uint32_t *>(c + p1), d, &x[u][4]);
+                uint2 code;
+                if constexpr (APART) code = make_uint2(*reinterpret_cast<const uint32_t *>(c + p0), *reinterpret_cast<const uint32_t *>(c + p1));
+                else code = *reinterpret_cast<const uint2 *>(c + p0);
+                values_of(code.x, d, &x[u][0]);
+                values_of(code.y, d, &x[u][4]);
             } else {
-                load4(data, row[u] * DIM + p0, MGB_F16, true, &x[u][0]);
-                load4(data, row[u] * DIM + p1, MGB_F16, true, &x[u][4]);
+                load_pieces<MGB_F16, true, APART>(data, row[u] * DIM, p0, p1, x[u]);
             }
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if constexpr (!WRITE) {
                 if (row[u] == -2) continue;
-                store4(rows, at[u] + p0, TYPE, VEC, &x[u][0]);
-                store4(rows, at[u] + p1, TYPE, VEC, &x[u][4]);
+                store_pieces<TYPE, VEC, APART>(rows, at[u], p0, p1, x[u]);
             } else if constexpr (Q8) {
                 float m = 0.0f;
 #pragma unroll
@@ -143,13 +176,16 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
                 const uint2 code = codes_of(x[u], d);
                 if (row[u] >= 0) {
                     uint8_t *c = data + row[u] * DIM;
-                    *reinterpret_cast<uint32_t *>(c + p0) = code.x;
-                    *reinterpret_cast<uint32_t *>(c + p1) = code.y;
+                    if constexpr (APART) {
+                        *reinterpret_cast<uint32_t *>(c + p0) = code.x;
+                        *reinterpret_cast<uint32_t *>(c + p1) = code.y;
+                    } else {
+                        *reinterpret_cast<uint2 *>(c + p0) = code;
+                    }
                     if (lane == 0) scale[row[u]] = d;
                 }
             } else if (row[u] >= 0) {
-                store4(data, row[u] * DIM + p0, MGB_F16, true, &x[u][0]);
-                store4(data, row[u] * DIM + p1, MGB_F16, true, &x[u][4]);
+                store_pieces<MGB_F16, true, APART>(data, row[u] * DIM, p0, p1, x[u]);
             }
         }
     }
@@ -179,6 +215,9 @@ cudaError_t launch(const MoveArgs &a, int sides, bool q8, int type, bool vec, cu
     }
 }
 
+// Whether 16-byte accesses fit.
+bool rows_wide(const mgb_rows &r) { return r.type == MGB_F32 ? rows_vec(r) : rows_vec16(r); }
+
 template <bool WRITE>
 mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, const mgb_rows *v, void *stream,
                 const char *op) {
@@ -196,11 +235,11 @@ mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, co
                0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
-    if (k->type == v->type) return op_launch_status(launch<WRITE>(a, 2, q8, k->type, rows_vec(*k) && rows_vec(*v), s), op);
+    if (k->type == v->type) return op_launch_status(launch<WRITE>(a, 2, q8, k->type, rows_wide(*k) && rows_wide(*v), s), op);
     // rows of two types: a launch each
-    cudaError_t e = launch<WRITE>(a, 1, q8, k->type, rows_vec(*k), s);
+    cudaError_t e = launch<WRITE>(a, 1, q8, k->type, rows_wide(*k), s);
     a.side[0] = a.side[1];
-    if (e == cudaSuccess) e = launch<WRITE>(a, 1, q8, v->type, rows_vec(*v), s);
+    if (e == cudaSuccess) e = launch<WRITE>(a, 1, q8, v->type, rows_wide(*v), s);
     return op_launch_status(e, op);
 }
 

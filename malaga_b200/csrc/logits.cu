@@ -8,10 +8,9 @@
 // on global memory, and the merge order is fixed.
 //
 // The penalties and biases touch few tokens of a row. Each CTA marks those of
-// its tile in a bitmap (one bit a token). Most warps then stream the tile and
-// leave the marked tokens out; meanwhile one warp (four for long lists) gives
-// every marked token a compact slot, by the bitmap's running popcount, collects
-// its count and bias there and deals with it.
+// its tile in a bitmap (one bit a token), whose running popcount gives each
+// marked token a compact slot with its count and bias. The streaming pass
+// leaves marked tokens out; a second, short pass goes over the slots.
 #include <cooperative_groups.h>
 
 #include "serving.cuh"
@@ -20,7 +19,6 @@
 namespace mgb {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxTile = 32768;  // tokens of one bitmap
 constexpr int kSlotBytes = 96 * 1024;  // shared memory for slots at most
 constexpr uint32_t kNone = 0xffffffffu;
@@ -129,14 +127,20 @@ __device__ __forceinline__ uint32_t bits_at(const uint32_t *row, uint32_t words,
     return __funnelshift_r(lo, hi, (uint32_t)off & 31);
 }
 
-template <int TYPE, bool RULES>
-__global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a) {
+// THREADS of a CTA: 256, of which an SM holds four CTAs; 512 where all CTAs have
+// an SM of their own, so that each has more in flight (one row of 256,206 tokens:
+// 7.6 against 9.1 us).
+template <int TYPE, bool RULES, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) choose_kernel(const ChooseArgs a) {
+    constexpr int kThreads = THREADS, kWarps = kThreads / 32;
+    constexpr int kPer = (kMaxTile / 32 + kThreads) / kThreads;  // words of a bit map a thread
     using N = Num<TYPE>;
     using T = typename N::T;
     constexpr int W = 16 / sizeof(T), UNROLL = 16 / W;
     extern __shared__ uint32_t smem[];
     __shared__ Best warp_best[kWarps];
     __shared__ Best cta_best[16];
+    __shared__ uint32_t warp_sum[kWarps];
     const uint32_t parts = gridDim.x, part = blockIdx.x, row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -173,9 +177,7 @@ __global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a)
             if (g >= 0 && (uint32_t)g < r.allow_rows) allow = r.allow + (size_t)g * r.allow_stride;
         }
     }
-    // warps for the marked tokens; the others stream
-    const int slot_warps = !RULES || !(nh || bias_ids) ? 0 : nh + r.bias_count <= 512 ? 1 : 4;
-    const int streamers = kThreads - 32 * slot_warps;
+    const bool slotted = nh || bias_ids;
 
     Best best{kLowest, 0.0f, kNone};
     for (uint32_t v0 = c0; v0 < c1; v0 += a.tile) {
@@ -189,18 +191,19 @@ __global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a)
         auto fetch = [&](uint32_t j0) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const uint32_t j = j0 + u * streamers;
+                const uint32_t j = j0 + u * kThreads;
                 if (j >= whole0 && j < whole1) raw[u] = __ldcs(vectors + j);
             }
         };
-        if (tid < streamers) fetch(tid);  // on their way while the bit maps are built
+        fetch(tid);  // on their way while the bit maps are built
+        uint32_t slots = 0;
         if constexpr (RULES) {
             for (uint32_t w = tid; w < words; w += kThreads) {
                 mark[w] = 0;
                 off[w] = allow ? ~bits_at(allow, r.allow_stride, (int64_t)v0 + 32 * w - shift) : 0u;
             }
             __syncthreads();
-            if (slot_warps) {
+            if (slotted) {
                 auto touch = [&](int32_t id) {
                     const uint32_t i = (uint32_t)id - v0;
                     if (i < width) atomicOr(&mark[(i + shift) >> 5], 1u << ((i + shift) & 31));
@@ -208,102 +211,116 @@ __global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a)
                 for (uint32_t i = tid; i < nh; i += kThreads) touch(hist[i]);
                 for (uint32_t i = tid; i < r.bias_count; i += kThreads) touch(bias_ids[i]);
                 __syncthreads();
-            }
-        }
-
-        if (tid < streamers) {
-            const bool y_vec = y && (((uintptr_t)(y + v0) & 15) / sizeof(T)) == shift;
-            for (uint32_t j0 = tid; j0 < nvec; j0 += streamers * UNROLL) {
-                if (j0 != tid) fetch(j0);
-                float f[UNROLL * W];
+                // rank[w]: touched tokens before word w; a thread has kPer words
+                uint32_t pop[kPer], upto = 0;
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) {
-                    const uint32_t j = j0 + u * streamers;
-                    uint32_t cut = 0, touched = 0;  // bits of the vector
-                    if constexpr (RULES) {
-                        if (j < nvec) {
-                            touched = mark[(j * W) >> 5] >> ((j * W) & 31) & ((1u << W) - 1);
-                            cut = off[(j * W) >> 5] >> ((j * W) & 31);
-                        }
-                    }
-                    T h[W];
-                    const bool whole = j >= whole0 && j < whole1;
-                    if (whole) {
-                        *reinterpret_cast<uint4 *>(h) = raw[u];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < W; ++e) {
-                            const uint32_t o = j * W + e - shift;
-                            h[e] = N::put(kLowest);
-                            if (j < nvec && o < width) h[e] = x[v0 + o];
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < W; ++e)
-                        if ((cut >> e) & 1) h[e] = N::put(kLowest);
-                    if (y && j < nvec) {
-                        if (y_vec && whole && !touched) {
-                            reinterpret_cast<uint4 *>(y + v0 - shift)[j] = *reinterpret_cast<const uint4 *>(h);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < W; ++e)
-                                if (j * W + e - shift < width && !((touched >> e) & 1)) y[v0 + j * W + e - shift] = h[e];
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        const float g = fmaxf(N::get(h[e]), kLowest);  // drops NaN
-                        f[u * W + e] = RULES && ((touched >> e) & 1) ? kLowest : g;
-                    }
+                for (int e = 0; e < kPer; ++e) {
+                    pop[e] = kPer * tid + e < words ? __popc(mark[kPer * tid + e]) : 0;
+                    upto += pop[e];
                 }
-                const uint32_t apart = streamers * W;
-                add(best, f, v0 - shift + j0 * W, [&](int e) { return (uint32_t)(e / W) * apart + (uint32_t)(e % W); });
-            }
-        } else if constexpr (RULES) {
-            const uint32_t ws = warp - (kWarps - slot_warps), ts = ws * 32 + lane, ns = 32 * slot_warps;
-            auto together = [&] { asm volatile("barrier.sync 1, %0;" ::"r"(ns) : "memory"); };
-            // rank[w]: marked tokens before word w; every warp of the group goes over all words, each writes its share
-            uint32_t slots = 0;
-            for (uint32_t w0 = 0; w0 < words; w0 += 32) {
-                const uint32_t w = w0 + lane, pop = w < words ? __popc(mark[w]) : 0;
-                uint32_t upto = pop;
+                const uint32_t mine = upto;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
                     if (lane >= o) upto += u;
                 }
-                if (w < words && (w0 / 32) % slot_warps == ws) rank[w] = slots + upto - pop;
-                slots += __shfl_sync(0xffffffffu, upto, 31);
-            }
-            for (uint32_t k = ts; k < slots; k += ns) {
-                count[k] = 0;
-                bias[k] = 0.0f;
-            }
-            together();
-            auto slot_of = [&](uint32_t i) {
-                const uint32_t bit = i + shift, k = rank[bit >> 5] + __popc(mark[bit >> 5] & ((1u << (bit & 31)) - 1));
-                token[k] = i;
-                return k;
-            };
-            for (uint32_t i = ts; i < nh; i += ns) {
-                const uint32_t at = (uint32_t)hist[i] - v0;
-                if (at < width) atomicAdd(&count[slot_of(at)], 1u);
-            }
-            // a warp an entry: the first entry of a token adds up all of them, in their order
-            for (uint32_t i = ws; i < r.bias_count; i += slot_warps) {
-                const int32_t id = bias_ids[i];
-                if ((uint32_t)id - v0 >= width) continue;
-                float sum = 0.0f;
-                bool first = true;
-                for (uint32_t j0 = 0; j0 < r.bias_count && first; j0 += 32) {
-                    uint32_t same = __ballot_sync(0xffffffffu, j0 + lane < r.bias_count && bias_ids[j0 + lane] == id);
-                    if (same && j0 + __ffs(same) - 1 < i) first = false;
-                    for (; same && first; same &= same - 1) sum += r.bias[(size_t)row * r.bias_count + j0 + __ffs(same) - 1];
+                if (lane == 31) warp_sum[warp] = upto;
+                __syncthreads();
+                uint32_t before = upto - mine;
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    before += k < warp ? warp_sum[k] : 0;
+                    slots += warp_sum[k];
                 }
-                if (first && lane == 0) bias[slot_of((uint32_t)id - v0)] = sum;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    if (kPer * tid + e < words) rank[kPer * tid + e] = before;
+                    before += pop[e];
+                }
+                for (uint32_t k = tid; k < slots; k += kThreads) {
+                    count[k] = 0;
+                    bias[k] = 0.0f;
+                }
+                __syncthreads();
+                auto slot_of = [&](uint32_t i) {
+                    const uint32_t bit = i + shift, k = rank[bit >> 5] + __popc(mark[bit >> 5] & ((1u << (bit & 31)) - 1));
+                    token[k] = i;
+                    return k;
+                };
+                for (uint32_t i = tid; i < nh; i += kThreads) {
+                    const uint32_t at = (uint32_t)hist[i] - v0;
+                    if (at < width) atomicAdd(&count[slot_of(at)], 1u);
+                }
+                // a warp an entry: the first entry of a token adds up all of them, in their order
+                for (uint32_t i = warp; i < r.bias_count; i += kWarps) {
+                    const int32_t id = bias_ids[i];
+                    if ((uint32_t)id - v0 >= width) continue;
+                    float sum = 0.0f;
+                    bool first = true;
+                    for (uint32_t j0 = 0; j0 < r.bias_count && first; j0 += 32) {
+                        uint32_t same = __ballot_sync(0xffffffffu, j0 + lane < r.bias_count && bias_ids[j0 + lane] == id);
+                        if (same && j0 + __ffs(same) - 1 < i) first = false;
+                        for (; same && first; same &= same - 1) sum += r.bias[(size_t)row * r.bias_count + j0 + __ffs(same) - 1];
+                    }
+                    if (first && lane == 0) bias[slot_of((uint32_t)id - v0)] = sum;
+                }
+                __syncthreads();
             }
-            together();
-            for (uint32_t k = ts; k < slots; k += ns) {
+        }
+
+        // streaming pass
+        const bool y_vec = y && (((uintptr_t)(y + v0) & 15) / sizeof(T)) == shift;
+        for (uint32_t j0 = tid; j0 < nvec; j0 += kThreads * UNROLL) {
+            float f[UNROLL * W];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t j = j0 + u * kThreads;
+                uint32_t out_of = 0, touched = 0;  // bits of the vector
+                if constexpr (RULES) {
+                    const uint32_t w = (j * W) >> 5, s = (j * W) & 31;
+                    if (j < nvec) {
+                        touched = mark[w] >> s;
+                        out_of = off[w] >> s;
+                    }
+                }
+                T h[W];
+                if (j >= whole0 && j < whole1) {
+                    *reinterpret_cast<uint4 *>(h) = raw[u];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const uint32_t o = j * W + e - shift;
+                        h[e] = N::put(kLowest);
+                        if (j < nvec && o < width) h[e] = x[v0 + o];
+                    }
+                }
+                // touched tokens keep their logit until the second pass
+                const uint32_t cut = out_of & ~touched;
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    if ((cut >> e) & 1) h[e] = N::put(kLowest);
+                if (y && j < nvec) {
+                    if (y_vec && j >= whole0 && j < whole1) {
+                        reinterpret_cast<uint4 *>(y + v0 - shift)[j] = *reinterpret_cast<const uint4 *>(h);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < W; ++e)
+                            if (j * W + e - shift < width) y[v0 + j * W + e - shift] = h[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    // fmax drops NaN
+                    const float g = fmaxf(N::get(h[e]), kLowest);
+                    f[u * W + e] = RULES && ((touched >> e) & 1) ? kLowest : g;
+                }
+            }
+            fetch(j0 + kThreads * UNROLL);  // on its way during the sums
+            add(best, f, v0 - shift + j0 * W, [](int e) { return (uint32_t)((e / W) * kThreads * W + e % W); });
+        }
+        if constexpr (RULES) {
+            __syncthreads();
+            for (uint32_t k = tid; k < slots; k += kThreads) {
                 const uint32_t id = v0 + token[k], c = count[k];
                 float f = N::get(x[id]);
                 if (c) {
@@ -316,8 +333,8 @@ __global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a)
                 const Best one{fmaxf(f, kLowest), 0.0f, id};
                 if (one.m > kLowest) best = merge(best, one);
             }
+            __syncthreads();
         }
-        if (RULES && v0 + a.tile < c1) __syncthreads();  // the next tile's bit maps take the place of these
     }
 
 #pragma unroll
@@ -349,14 +366,14 @@ __global__ void __launch_bounds__(kThreads, 4) choose_kernel(const ChooseArgs a)
     }
 }
 
-template <int TYPE, bool RULES>
+template <int TYPE, bool RULES, int THREADS>
 cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
-    cudaError_t e = op_allow(choose_kernel<TYPE, RULES>, kSlotBytes + (int)(kMaxTile / 32 + 1) * 12, true, done);
+    cudaError_t e = op_allow(choose_kernel<TYPE, RULES, THREADS>, kSlotBytes + (int)(kMaxTile / 32 + 1) * 12, true, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(parts, rows);
-    c.blockDim = dim3(kThreads);
+    c.blockDim = dim3(THREADS);
     c.dynamicSmemBytes = smem;
     c.stream = s;
     cudaLaunchAttribute at[1];
@@ -365,7 +382,13 @@ cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem,
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     c.attrs = at;
     c.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, RULES>, a);
+    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, RULES, THREADS>, a);
+}
+
+template <int TYPE>
+cudaError_t launch(const ChooseArgs &a, bool ruled, bool wide, uint32_t rows, uint32_t parts, int smem, cudaStream_t s) {
+    if (wide) return ruled ? launch<TYPE, true, 512>(a, rows, parts, smem, s) : launch<TYPE, false, 512>(a, rows, parts, smem, s);
+    return ruled ? launch<TYPE, true, 256>(a, rows, parts, smem, s) : launch<TYPE, false, 256>(a, rows, parts, smem, s);
 }
 
 }  // namespace
@@ -407,13 +430,14 @@ extern "C" MGB_API mgb_status mgb_logits_choose(const void *logits, int type, in
     auto cap = [&] { return (uint32_t)(entries < a.tile ? entries : a.tile); };
     while ((uint64_t)cap() * 12 > (uint64_t)kSlotBytes) a.tile = (a.tile / 2 + 63) & ~63u;
     a.cap = cap();
+    const bool wide = (uint64_t)rows * parts <= 148;
     const int smem = ruled ? (int)((a.tile / 32 + 1) * 12 + a.cap * 12) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     switch (type) {
-        case MGB_F32: e = ruled ? launch<MGB_F32, true>(a, rows, parts, smem, s) : launch<MGB_F32, false>(a, rows, parts, smem, s); break;
-        case MGB_F16: e = ruled ? launch<MGB_F16, true>(a, rows, parts, smem, s) : launch<MGB_F16, false>(a, rows, parts, smem, s); break;
-        default: e = ruled ? launch<MGB_BF16, true>(a, rows, parts, smem, s) : launch<MGB_BF16, false>(a, rows, parts, smem, s); break;
+        case MGB_F32: e = launch<MGB_F32>(a, ruled, wide, rows, parts, smem, s); break;
+        case MGB_F16: e = launch<MGB_F16>(a, ruled, wide, rows, parts, smem, s); break;
+        default: e = launch<MGB_BF16>(a, ruled, wide, rows, parts, smem, s); break;
     }
     return op_launch_status(e, op);
 }
