@@ -159,10 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
+    begin();
     int n;
     const int t0 = a.seq.first(b, n);
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
-    let_next_start();
     if ((uint32_t)rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;

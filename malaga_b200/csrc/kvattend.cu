@@ -44,6 +44,7 @@ struct AttendArgs {
     int q_type, o_type, causal;
     bool o_vec, q_vec16, o_vec16;  // rows that allow accesses of four numbers, of eight 16-bit ones
     uint32_t group;  // query heads of a cache head
+    bool overlap;    // the kernel for few rows runs beside the one for many
     uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
 };
@@ -107,11 +108,6 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
         w[0] = *reinterpret_cast<const uint16_t *>(p);
     }
 }
-
-// Programmatic dependent launch: the next kernel may start once every CTA of this one has; wait until the one before
-// has ended.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // Few rows: tiles of 8 or 16 rows (token, head of the group) of one cache head.
@@ -450,13 +446,16 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
+    // beside the launch for many rows, which has seen the one before it end
+    if (a.overlap) let_next_start();
+    else begin();
     int n;
     const int t0 = a.seq.first(b, n);
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
-    // After a launch for many rows, which this one may overlap, one CTA sees to it that this kernel does not end first.
-    const bool keeper = blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && b == gridDim.z - 1;
+    // then one CTA sees to it that this kernel does not end first
+    const bool keeper = a.overlap && blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && b == gridDim.z - 1;
     if ((uint32_t)rows > a.few) {
         if (keeper) wait_for_previous();
         return;
@@ -709,37 +708,19 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
 }
 
 template <int D, bool Q8, bool SPLIT, int NT>
-cudaError_t launch_rows(const AttendArgs &a, dim3 grid, bool overlap, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
     constexpr int SMEM = Ring<D, Q8>::BYTES;
     static std::atomic<bool> done[kMaxDevices];
     cudaError_t e = op_allow(attend_rows_kernel<D, Q8, SPLIT, NT>, SMEM, true, done);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = grid;
-    c.blockDim = dim3(kRowThreads);
-    c.dynamicSmemBytes = SMEM;
-    c.stream = s;
-    cudaLaunchAttribute at[2];
-    c.attrs = at;
-    if (grid.x > 1) {
-        at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        at[c.numAttrs].val.clusterDim.x = grid.x;
-        at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
-        ++c.numAttrs;
-    }
-    if (overlap) {
-        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[c.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-        ++c.numAttrs;
-    }
-    return cudaLaunchKernelEx(&c, attend_rows_kernel<D, Q8, SPLIT, NT>, a);
+    return op_launch(attend_rows_kernel<D, Q8, SPLIT, NT>, grid, kRowThreads, SMEM, grid.x, a, s);
 }
 
 // Keys are cut over the CTAs of a cluster (at most 16) while all CTAs still run
 // at once and every warp keeps two blocks, and further while a CTA would have
 // more than 2048 keys: sequences of unlike lengths then even out.
 template <int D, bool Q8, bool SPLIT, int NT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
     constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, FIT = 227 * 1024 / SMEM;
     constexpr int SLOTS = 148 * (FIT < Frag<D, Q8>::ctas(NT) ? FIT : Frag<D, Q8>::ctas(NT));
     uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
@@ -750,21 +731,21 @@ cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, b
     if (parts > most_len / (kRowWarps * 32)) parts = most_len / (kRowWarps * 32);
     // sizes that pack into the GPU's clusters of 16 or 18 SMs
     parts = parts >= 16 ? 16 : parts >= 8 ? 8 : parts >= 4 ? 4 : parts < 1 ? 1 : parts;
-    return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), overlap, s);
+    return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
 }
 
 // 8-row tiles where a call has no more rows a cache head than that, else 16.
 template <int D, bool Q8, bool SPLIT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
-    return rows <= 8 ? launch_rows<D, Q8, SPLIT, 1>(a, rows, most_len, overlap, s)
-                     : launch_rows<D, Q8, SPLIT, 2>(a, rows, most_len, overlap, s);
+cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
+    return rows <= 8 ? launch_rows<D, Q8, SPLIT, 1>(a, rows, most_len, s)
+                     : launch_rows<D, Q8, SPLIT, 2>(a, rows, most_len, s);
 }
 
 template <int D>
-cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t rows, uint64_t most_len, bool overlap, cudaStream_t s) {
+cudaError_t launch_rows(const AttendArgs &a, bool q8, uint64_t rows, uint64_t most_len, cudaStream_t s) {
     if (a.q_type == MGB_F32)
-        return q8 ? launch_rows<D, true, true>(a, rows, most_len, overlap, s) : launch_rows<D, false, true>(a, rows, most_len, overlap, s);
-    return q8 ? launch_rows<D, true, false>(a, rows, most_len, overlap, s) : launch_rows<D, false, false>(a, rows, most_len, overlap, s);
+        return q8 ? launch_rows<D, true, true>(a, rows, most_len, s) : launch_rows<D, false, true>(a, rows, most_len, s);
+    return q8 ? launch_rows<D, true, false>(a, rows, most_len, s) : launch_rows<D, false, false>(a, rows, most_len, s);
 }
 
 #include "attend_tiles.cuh"
@@ -797,18 +778,8 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
     if (row_tiles * a.kv.heads > 65535) row_tiles = 65535 / a.kv.heads;
     uint32_t parts;
     tiles_cost(a, most_new, most_len, parts);
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(parts, (unsigned)(row_tiles * a.kv.heads), a.seq.seqs);
-    c.blockDim = dim3(tiles::kThreads);
-    c.dynamicSmemBytes = tiles::Smem<D>::ASKED;
-    c.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    c.attrs = at;
-    c.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, tiles::attend_tiles_kernel<D, Q8>, a);
+    return op_launch(tiles::attend_tiles_kernel<D, Q8>, dim3(parts, (unsigned)(row_tiles * a.kv.heads), a.seq.seqs), tiles::kThreads,
+                     tiles::Smem<D>::ASKED, parts, a, s);
 }
 
 // Which kernel. f32 queries, whose two f16 parts only the kernel for few rows
@@ -828,11 +799,14 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
         const double pairs = (double)((rows + 15) / 16 * a.kv.heads * a.seq.seqs) * (double)most_len;
         few = 4.0 + pairs / 28500.0 * ((D + 16) / 80.0) < (double)tiles_cost(a, most_new, most_len, parts) * (1.3 + D / 70.0);
     }
-    if (few) return launch_rows<D>(a, q8, rows, most_len, false, s);
+    if (few) return launch_rows<D>(a, q8, rows, most_len, s);
     a.few = kFewRows;
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
     // sequences of unlike lengths: there may be some of few rows
-    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs) e = launch_rows<D>(a, q8, kFewRows, most_len, true, s);
+    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs) {
+        a.overlap = true;
+        e = launch_rows<D>(a, q8, kFewRows, most_len, s);
+    }
     return e;
 }
 
@@ -855,7 +829,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
-                 0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e};
+                 false, 0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;

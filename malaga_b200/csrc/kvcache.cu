@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     // rows of a thread in flight: more cost warps of an SM (reading, 1 / 2 / 4: 67 / 75 / 89 us; writing 87 / 77 / 77)
     constexpr int kBatch = WRITE ? 2 : 1;
     __shared__ int64_t place[kMaxTokens];  // row of head 0 in the cache, -1 where there is none
+    begin();
     const uint32_t first = blockIdx.x * a.per_cta, tokens = min(a.per_cta, a.seq.tokens - first);
     if (threadIdx.x < tokens) {
         const int token = (int)(first + threadIdx.x);
@@ -198,11 +199,10 @@ cudaError_t launch(MoveArgs a, int sides, int type, bool vec, cudaStream_t s) {
     const uint32_t n = a.seq.tokens / (2 * 148);
     a.per_cta = n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n;
     const dim3 grid((a.seq.tokens + a.per_cta - 1) / a.per_cta, sides);
-    auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a); };
-    if (type == MGB_F32) vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, false>);
-    else if (type == MGB_F16) vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, false>);
-    else vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, false>);
-    return cudaGetLastError();
+    auto go = [&](auto kernel) { return op_launch(kernel, grid, kThreads, 0, 1, a, s); };
+    if (type == MGB_F32) return vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F32, false>);
+    if (type == MGB_F16) return vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_F16, false>);
+    return vec ? go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, true>) : go(kv_move_kernel<DIM, Q8, WRITE, MGB_BF16, false>);
 }
 
 template <bool WRITE>

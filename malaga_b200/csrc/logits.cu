@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) choose_kernel
     const uint32_t parts = gridDim.x, part = blockIdx.x, row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    begin();
 
     const mgb_logit_rules &r = a.rules;
     const T *x = reinterpret_cast<const T *>(a.x) + (size_t)row * a.stride;
@@ -322,12 +323,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) choose_kernel
             __syncthreads();
             for (uint32_t k = tid; k < slots; k += kThreads) {
                 const uint32_t id = v0 + token[k], c = count[k];
-                float f = N::get(x[id]);
-                if (c) {
-                    f = f > 0.0f ? __fdiv_rn(f, rep) : f * rep;
-                    f = f - (freq * (float)c + pres);
-                }
-                if (bias_ids) f = f + bias[k];
+                // a few numbers: in 64 bits and rounded once, since many occurrences make them large
+                double d = N::get(x[id]);
+                if (c) d = (d > 0.0 ? d / rep : d * rep) - ((double)freq * c + pres);
+                if (bias_ids) d += bias[k];
+                float f = (float)d;
                 if (allow && !((allow[id >> 5] >> (id & 31)) & 1)) f = kLowest;
                 if (y) y[id] = N::put(f);
                 const Best one{fmaxf(f, kLowest), 0.0f, id};
@@ -371,18 +371,7 @@ cudaError_t launch(const ChooseArgs &a, uint32_t rows, uint32_t parts, int smem,
     static std::atomic<bool> done[kMaxDevices];
     cudaError_t e = op_allow(choose_kernel<TYPE, RULES, THREADS>, kSlotBytes + (int)(kMaxTile / 32 + 1) * 12, true, done);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(parts, rows);
-    c.blockDim = dim3(THREADS);
-    c.dynamicSmemBytes = smem;
-    c.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = parts;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    c.attrs = at;
-    c.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, choose_kernel<TYPE, RULES, THREADS>, a);
+    return op_launch(choose_kernel<TYPE, RULES, THREADS>, dim3(parts, rows), THREADS, smem, parts, a, s);
 }
 
 template <int TYPE>

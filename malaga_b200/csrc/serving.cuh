@@ -51,6 +51,37 @@ cudaError_t op_allow(F *kernel, int smem, bool big_cluster, std::atomic<bool> (&
     return e;
 }
 
+// Every launch is a programmatic dependent one: its CTAs may be scheduled once
+// those of the kernel before it (if that one, too, lets it) have all started, and
+// wait in begin() until it has ended, before they touch memory. That takes the
+// launch out of the way of short kernels (a decode step's attention 5.8 -> 4.4 us
+// back to back).
+template <typename Args>
+cudaError_t op_launch(void (*kernel)(Args), dim3 grid, int threads, int smem, unsigned cluster, const Args &args, cudaStream_t s) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&c, kernel, args);
+}
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// In this order: that the next kernel has started says that the one before this has ended.
+__device__ __forceinline__ void begin() {
+    wait_for_previous();
+    let_next_start();
+}
+
 // The cache as the kernels see it. A position's row of one head starts
 // row(page, head, slot) rows into k and v; products are 64-bit, since a cache
 // of a 180 GB GPU has more than 2^31 numbers.
