@@ -23,8 +23,10 @@ from . import _lib
 from ._lib import check
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+# The quick forms of current_stream(device).cuda_stream and current_device(), where this torch has them.
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _need(ok: bool, what: str) -> None:
@@ -40,23 +42,22 @@ def _cuda(x: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = 
     return x.data_ptr()
 
 
-def _rows(x: torch.Tensor, name: str, device: torch.device, dim: int) -> _lib.Rows:
+def _rows(x: torch.Tensor, name: str, index: int, dim: int) -> _lib.Rows:
     """Packed rows [tokens, heads, dim] as the library takes them: any strides of tokens and heads."""
     kind = _TYPES.get(x.dtype)
     if kind is None:
         raise ValueError(f"{name} must be float32, float16 or bfloat16")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the cache on {device}")
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, the cache on GPU {index}")
     shape, strides = x.shape, x.stride()
     if len(shape) != 3 or shape[2] != dim or strides[2] != 1:
         raise ValueError(f"{name} must be [tokens, heads, {dim}] with contiguous rows")
     return _lib.Rows(x.data_ptr(), strides[0], strides[1], shape[0], shape[1], kind)
 
 
-def _call(device: torch.device, fn, *args) -> None:
-    """fn(*args, current stream) with the tensors' device current."""
-    index = device.index
-    if torch.cuda.current_device() == index:
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, current stream) with GPU `index`, the tensors', current."""
+    if _current_device() == index:
         code = fn(*args, _stream_of(index))
     else:
         with torch.cuda.device(index):
@@ -89,7 +90,7 @@ class Seqs:
         _need(table.dim() == 2, "table must be [seqs, pages]")
         n, device = table.size(0), table.device
         self.tensors = (table, q_start, kv_len)  # kept alive
-        self.device = device
+        self.device, self.index = device, table.get_device()
         self.tokens = tokens
         self._c = _lib.KvSeqs(_cuda(table, "table", torch.int32), _cuda(q_start, "q_start", torch.int32, (n + 1,), device),
                               _cuda(kv_len, "kv_len", torch.int32, (n,), device), n, table.size(1),
@@ -121,6 +122,7 @@ class PagedKV:
         _need(k.dtype in (torch.float16, torch.int8), "the cache must be float16 or int8")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device, self.q8 = k.device, k.dtype == torch.int8
+        self.index = k.get_device()
         self.pages, self.heads, self.page, self.dim = k.shape
         _need(self.dim in (16, 32, 64, 128), f"head dim {self.dim} is not 16, 32, 64 or 128")
         _need(16 <= self.page <= 1024 and self.page & (self.page - 1) == 0,
@@ -131,6 +133,7 @@ class PagedKV:
         vs = _cuda(v_scale, "v_scale", torch.float32, k.shape[:3], k.device) if self.q8 else None
         self._c = _lib.Kv(kp, vp, ks, vs, self.pages, self.heads, self.page, self.dim, int(self.q8))
         self._ref = ctypes.byref(self._c)
+        self._scale = self.dim ** -0.5
         self._lib = _lib.load()
 
     @classmethod
@@ -144,14 +147,14 @@ class PagedKV:
         return cls(*data, *scales)
 
     def _check(self, seqs: Seqs) -> None:
-        if seqs.device != self.device:
+        if seqs.index != self.index:
             raise ValueError(f"the sequences are on {seqs.device}, the cache on {self.device}")
 
     def write(self, seqs: Seqs, k: torch.Tensor, v: torch.Tensor) -> None:
         """Writes the new tokens' rows k, v [tokens, heads, dim] into their pages."""
         self._check(seqs)
-        ck, cv = _rows(k, "k", self.device, self.dim), _rows(v, "v", self.device, self.dim)
-        _call(self.device, self._lib.mgb_kv_write, self._ref, seqs._ref, ctypes.byref(ck), ctypes.byref(cv))
+        ck, cv = _rows(k, "k", self.index, self.dim), _rows(v, "v", self.index, self.dim)
+        _call(self.index, self._lib.mgb_kv_write, self._ref, seqs._ref, ctypes.byref(ck), ctypes.byref(cv))
 
     def read(self, seqs: Seqs, dtype: torch.dtype = torch.float16,
              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -160,13 +163,14 @@ class PagedKV:
         Into out = (K, V) where given, else into new tensors of seqs.tokens rows."""
         self._check(seqs)
         if out is None:
-            _need(seqs.tokens is not None, "read needs out, or sequences that know their number of tokens")
-            k = torch.empty((seqs.tokens, self.heads, self.dim), dtype=dtype, device=self.device)
+            if seqs.tokens is None:
+                raise ValueError("read needs out, or sequences that know their number of tokens")
+            k = self.k.new_empty((seqs.tokens, self.heads, self.dim), dtype=dtype)
             v = torch.empty_like(k)
         else:
             k, v = out
-        ck, cv = _rows(k, "k", self.device, self.dim), _rows(v, "v", self.device, self.dim)
-        _call(self.device, self._lib.mgb_kv_read, self._ref, seqs._ref, ctypes.byref(ck), ctypes.byref(cv))
+        ck, cv = _rows(k, "k", self.index, self.dim), _rows(v, "v", self.index, self.dim)
+        _call(self.index, self._lib.mgb_kv_read, self._ref, seqs._ref, ctypes.byref(ck), ctypes.byref(cv))
         return k, v
 
     def attend(self, seqs: Seqs, q: torch.Tensor, scale: float | None = None, causal: bool = True,
@@ -176,12 +180,15 @@ class PagedKV:
         h // (query heads / heads). causal: a token sees the positions up to its own, else all of its
         sequence. A token that sees nothing gets zeros. Returns out (q's type and shape unless given)."""
         self._check(seqs)
-        cq = _rows(q, "q", self.device, self.dim)
+        cq = _rows(q, "q", self.index, self.dim)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        co = _rows(out, "out", self.device, self.dim)
-        _call(self.device, self._lib.mgb_kv_attend, self._ref, seqs._ref, ctypes.byref(cq), ctypes.byref(co),
-              self.dim ** -0.5 if scale is None else scale, causal)
+            heads = cq.heads
+            co = _lib.Rows(out.data_ptr(), heads * self.dim, self.dim, cq.tokens, heads, cq.type)
+        else:
+            co = _rows(out, "out", self.index, self.dim)
+        _call(self.index, self._lib.mgb_kv_attend, self._ref, seqs._ref, ctypes.byref(cq), ctypes.byref(co),
+              self._scale if scale is None else scale, causal)
         return out
 
 
@@ -212,6 +219,7 @@ class LogitRules:
                    if x is not None]
         self.rows = per_row[0].size(0) if per_row else None  # None: any number of rows
         self.device = per_row[0].device if per_row else allow.device if allow is not None else None
+        self.index = None if self.device is None else (per_row[0] if per_row else allow).get_device()
         self.tensors = (history, history_len, repetition, frequency, presence, bias_ids, bias, allow, allow_row)
         n, dev = self.rows, self.device
 
@@ -247,19 +255,19 @@ class LogitRules:
             raise ValueError("logits must be float32, float16 or bfloat16")
         if len(shape) != 2 or not logits.is_cuda or strides[1] != 1:
             raise ValueError("logits must be [rows, vocab] on a GPU with contiguous rows")
-        device, (rows, vocab) = logits.device, shape
+        index, (rows, vocab) = logits.get_device(), shape
         if self.rows is not None and self.rows != rows:
             raise ValueError(f"the rules are for {self.rows} rows, the logits have {rows}")
-        if self.device is not None and self.device != device:
-            raise ValueError(f"the rules are on {self.device}, the logits on {device}")
+        if self.index is not None and self.index != index:
+            raise ValueError(f"the rules are on GPU {self.index}, the logits on {logits.device}")
         y, y_stride = None, 0
         if adjusted is not None:
-            if (adjusted.dtype != logits.dtype or adjusted.shape != shape or adjusted.device != device
+            if (adjusted.dtype != logits.dtype or adjusted.shape != shape or adjusted.get_device() != index
                     or adjusted.stride(1) != 1):
                 raise ValueError("adjusted must be like the logits")
             y, y_stride = adjusted.data_ptr(), adjusted.stride(0)
-        ids = torch.empty(rows, dtype=torch.int32, device=device)
-        logp = torch.empty(rows, dtype=torch.float32, device=device)
-        _call(device, self._lib.mgb_logits_choose, logits.data_ptr(), kind, strides[0], rows, vocab, self._ref,
+        ids = logits.new_empty((rows,), dtype=torch.int32)
+        logp = torch.empty_like(ids, dtype=torch.float32)
+        _call(index, self._lib.mgb_logits_choose, logits.data_ptr(), kind, strides[0], rows, vocab, self._ref,
               ids.data_ptr(), logp.data_ptr(), y, y_stride)
         return (ids, logp) if adjusted is None else (ids, logp, adjusted)
