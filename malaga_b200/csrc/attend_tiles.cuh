@@ -103,6 +103,7 @@ __device__ __forceinline__ uint32_t piece(int r, int c) {
     return (uint32_t)((r >> 3) * (D * 16) + c * 128 + (r & 7) * 16);
 }
 
+template <int D>
 struct Shared {
     uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full;
     // Of tile j at j & 3: the softmax of tile j may still read when the loading
@@ -112,6 +113,10 @@ struct Shared {
     int v_exp[4];       // V of the tile is over 2^v_exp
     uint32_t holes[4];  // bit i: keys 16 i .. 16 i + 15 of the tile have no page
     float m[256], l[256], weight[8][256];
+    // Where some rows of the tile do not see a key, an infinity or NaN in its V is
+    // taken out (0 times it would reach them) and noted: rows that see key wild[d]
+    // get NaN in dim d. wild_any: whether there is one.
+    int wild[D], wild_any;
     uint32_t tmem;
     int lost;  // a wait ran out: nothing more is computed, the rows become NaN
 };
@@ -155,7 +160,7 @@ template <int D, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendArgs a) {
     using SM = Smem<D>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ Shared sh;
+    __shared__ Shared<D> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
@@ -184,7 +189,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         }
         mbar_init(&sh.o_full, 1);
         sh.lost = 0;
+        sh.wild_any = 0;
     }
+    if (tid < D) sh.wild[tid] = 0x7fffffff;
     fence_before();
     __syncthreads();
     fence_after();
@@ -377,6 +384,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (!ok) l = __int_as_float(0x7fffffff);
             const float back = Q8 ? power_of_2(exp_v) : 1.0f;
             const bool has = count > 0;
+            // columns c0 .. c0 + 15 of the row's sum
+            auto load_o = [&](int c0, uint32_t (&raw)[16]) {
+                tmem_load16(o_at + c0, raw);
+                tmem_wait_load();
+                if (sh.wild_any) {
+#pragma unroll 1
+                    for (int c = 0; c < 16; ++c)
+                        if (sh.wild[c0 + c] < lim) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (k == c) raw[k] = 0x7fffffffu;
+                        }
+                }
+            };
             if (parts == 1) {
                 const bool some = has && !(l < 1e-30f);  // a row that sees nothing has at most 128 times 2^-126 a tile
                 const float f = some ? back / l : 0.0f;
@@ -386,8 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t raw[16], w[8];
-                        tmem_load16(o_at + c0, raw);
-                        tmem_wait_load();
+                        load_o(c0, raw);
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             const float u = some ? __uint_as_float(raw[2 * c]) * f : 0.0f;
@@ -416,8 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t raw[16];
-                        tmem_load16(o_at + c0, raw);
-                        tmem_wait_load();
+                        load_o(c0, raw);
                         if (row >= sp.live) continue;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
@@ -431,8 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 16) {
                     uint32_t raw[16];
-                    tmem_load16(o_at + c0, raw);
-                    tmem_wait_load();
+                    load_o(c0, raw);
 #pragma unroll
                     for (int c = 0; c < 16; c += 4) {
                         float4 x = make_float4(__uint_as_float(raw[c]) * back, __uint_as_float(raw[c + 1]) * back,
@@ -444,6 +462,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 sh.m[row] = m;
                 sh.l[row] = l;
             }
+            asm volatile("barrier.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+            if (tid < D) sh.wild[tid] = 0x7fffffff;
+            if (tid == 0) sh.wild_any = 0;
             fence_before();
             meet(parts > 1);
             if (parts > 1) {
@@ -595,6 +616,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     fetch(vbase, vraw);
                     const uint32_t holes = __ballot_sync(0xffffffffu, pages >= a.kv.pages) & 0xff;
                     exp_v = max(exp_v, exponent(vd));
+                    if ((sp.first + j + 1) * kKeys > sp.all) {
+#pragma unroll
+                        for (int w = 0; w < kLoadWarps; ++w) {
+                            if (w != lw || fabsf(vd[w]) <= 3.402823466e38f) continue;
+                            vd[w] = 0.0f;
+                            for (int d = 0; d < D; ++d) atomicMin(&sh.wild[d], (sp.first + j) * kKeys + 32 * w + lane);
+                            sh.wild_any = 1;
+                        }
+                    }
                     const uint32_t v_own = own_scale(vd, exp_v);
                     if (turn > 0) ok = wait(&sh.k_free[stage], turn - 1);
                     if (!ok) break;
@@ -649,6 +679,29 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     next = pages_of(j + 2);
                     copy(a.kv.k, SM::K, sh.k_free, j + 1);
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    if ((sp.first + j + 1) * kKeys > sp.all) {
+#pragma unroll 1
+                        for (int u = 0; u < PER; ++u) {
+                            const int r = row_no(PIECES < 4 ? u : u / (PER / ROWS)), c = piece_no(u);
+                            uint4 *at_piece = reinterpret_cast<uint4 *>(smem + SM::V + stage * SM::TILE + piece<D>(r, c));
+                            uint4 x = *at_piece;
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                            bool found = false;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const uint32_t half = 0xffffu << (16 * (e & 1));
+                                if ((w[e / 2] & half & 0x7c007c00u) == (half & 0x7c007c00u)) {
+                                    w[e / 2] &= ~half;
+                                    atomicMin(&sh.wild[8 * c + e], (sp.first + j) * kKeys + r);
+                                    found = true;
+                                }
+                            }
+                            if (found) {
+                                *at_piece = make_uint4(w[0], w[1], w[2], w[3]);
+                                sh.wild_any = 1;
+                            }
+                        }
+                    }
                     publish(&sh.v_full[stage]);
                     copy(a.kv.v, SM::V, sh.v_free, j + 1);
                 }

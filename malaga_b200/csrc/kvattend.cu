@@ -396,7 +396,7 @@ struct Rows {
                     p[0][n][u] = transpose8(hi);
                     if constexpr (SPLIT) {
                         const float2 h = unpack(hi);
-                        p[1][n][u] = transpose8(pack(w[2 * u] - h.x, w[2 * u + 1] - h.y));
+                        p[SPLIT][n][u] = transpose8(pack(w[2 * u] - h.x, w[2 * u + 1] - h.y));
                     }
                 }
             }
@@ -405,26 +405,70 @@ struct Rows {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mma16(o[n][j], f, p[0][n][0], p[0][n][1]);
-                    if constexpr (SPLIT) mma16(o[n][j], f, p[1][n][0], p[1][n][1]);
+                    if constexpr (SPLIT) mma16(o[n][j], f, p[SPLIT][n][0], p[SPLIT][n][1]);
                 }
             };
+            auto products = [&] {
 #pragma unroll
-            for (int c = 0; c < F::VW; ++c) {
-                if constexpr (Q8) {
-                    const uint32_t x0 = x[i].v[0][c] ^ 0x80808080u, x1 = x[i].v[1][c] ^ 0x80808080u;
-                    const uint32_t x2 = x[i].v[2][c] ^ 0x80808080u, x3 = x[i].v[3][c] ^ 0x80808080u;
-                    const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
-                    constexpr int PER = F::STEPS < 2 ? 1 : 2;
-                    pair(PER * c, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
-                    if constexpr (PER == 2) {
-                        const uint32_t hi0 = __byte_perm(x0, x1, 0x7362), hi1 = __byte_perm(x2, x3, 0x7362);
-                        pair(PER * c + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
+                for (int c = 0; c < F::VW; ++c) {
+                    if constexpr (Q8) {
+                        const uint32_t x0 = x[i].v[0][c] ^ 0x80808080u, x1 = x[i].v[1][c] ^ 0x80808080u;
+                        const uint32_t x2 = x[i].v[2][c] ^ 0x80808080u, x3 = x[i].v[3][c] ^ 0x80808080u;
+                        const uint32_t lo0 = __byte_perm(x0, x1, 0x5140), lo1 = __byte_perm(x2, x3, 0x5140);
+                        constexpr int PER = F::STEPS < 2 ? 1 : 2;
+                        pair(PER * c, codes2(lo0, 0x4140), codes2(lo0, 0x4342), codes2(lo1, 0x4140), codes2(lo1, 0x4342));
+                        if constexpr (PER == 2) {
+                            const uint32_t hi0 = __byte_perm(x0, x1, 0x7362), hi1 = __byte_perm(x2, x3, 0x7362);
+                            pair(PER * c + 1, codes2(hi0, 0x4140), codes2(hi0, 0x4342), codes2(hi1, 0x4140), codes2(hi1, 0x4342));
+                        }
+                    } else {
+                        pair(c, __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x5410), __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x7632),
+                             __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x5410), __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x7632));
                     }
-                } else {
-                    pair(c, __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x5410), __byte_perm(x[i].v[0][c], x[i].v[1][c], 0x7632),
-                         __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x5410), __byte_perm(x[i].v[2][c], x[i].v[3][c], 0x7632));
+                }
+            };
+            if constexpr (!Q8) {
+                // 0 times an infinity or NaN would reach rows that do not see its key: such a block goes key by key,
+                // and every row keeps what it had where the key is masked
+                bool wild = false;
+                if (!whole) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int c = 0; c < F::VW; ++c) {
+                            const uint32_t e = x[i].v[u][c] & 0x7c007c00u;
+                            wild |= (e & 0x7c00u) == 0x7c00u || (e >> 16) == 0x7c00u;
+                        }
+                    wild = __any_sync(0xffffffffu, wild);
+                }
+                if (wild) {
+                    const Block<D, Q8> all_keys = x[i];
+#pragma unroll 1
+                    for (int key = 0; key < 16; ++key) {
+                        float kept[NT][F::STEPS][4];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < F::STEPS; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) kept[n][j][e] = o[n][j][e];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+#pragma unroll
+                            for (int c = 0; c < F::VW; ++c) x[i].v[u][c] = 2 * t + (u & 1) + 8 * (u >> 1) == key ? all_keys.v[u][c] : 0u;
+                        products();
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < F::STEPS; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (key0 + 16 * i + key >= limit[n][e & 1]) o[n][j][e] = kept[n][j][e];
+                    }
+                    continue;
                 }
             }
+            products();
         }
     }
 };
