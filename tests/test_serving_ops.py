@@ -761,3 +761,48 @@ def test_python_refuses(ops):
         rules.choose(z(3, 100), z(3, 100).half())
     with pytest.raises(ops._lib.MgbError):
         ops.LogitRules(allow=z(1, 2, **i32)).choose(z(1, 100))
+
+
+# ---------------------------------------------------------------------------
+# Together
+
+@gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+def test_example_serves_what_a_dense_model_says(ops, fmt):
+    """examples/paged_decode.py: every token that it chose is, for a dense model in 64 bits over the same tokens, within
+    the cache's rounding of the best under the rules. A row's numbers are stored to 2^-11 (f16) or 1 / 254 of its
+    largest (8 bits); two layers pass that on to logits of standard deviation 1 by at most a few tenths of it."""
+    import os
+    import sys
+
+    torch = _torch()
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import paged_decode as ex
+
+    model = ex.Decoder()
+    gen = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, model.vocab, (n,), generator=gen).tolist() for n in (1, 70, 33, 16)]
+    bits = torch.rand(-(-model.vocab // 32), 32, generator=gen) < 0.5
+    allow = (bits * torch.tensor([1 << i for i in range(31)] + [-(1 << 31)])).sum(-1).to(torch.int32).cuda()
+    tokens, scores = ex.serve(model, prompts, 12, fmt, allow=allow)
+    slack = 0.01 if fmt == "f16" else 0.1
+    banned = (~bits.flatten()[: model.vocab]).cuda()
+    for prompt, new, score in zip(prompts, tokens, scores):
+        assert len(new) == 12
+        seq = torch.tensor(prompt + new, device="cuda")
+        x = model.start(seq, torch.arange(len(seq), device="cuda")).double()
+        for layer in range(model.layers):
+            q, k, v = model.project(layer, x)
+            k, v = (y.repeat_interleave(model.heads // model.kv_heads, 1) for y in (k, v))
+            s = torch.einsum("nhd,lhd->hnl", q, k) / model.dim ** 0.5
+            s += torch.full(s.shape[1:], -math.inf, device="cuda", dtype=torch.float64).triu_(1)
+            x = x + torch.einsum("hnl,lhd->nhd", s.softmax(-1), v).flatten(1) @ model.out[layer].double().T
+        y = model.logits(x)
+        for i, (t, logp) in enumerate(zip(new, score)):
+            z = y[len(prompt) + i - 1].clone()
+            said = torch.tensor(sorted(set(prompt + new[:i])), device="cuda")
+            z[said] = torch.where(z[said] > 0, z[said] / 1.2, z[said] * 1.2)
+            z[banned] = -math.inf
+            assert not banned[t]
+            assert z[t] >= z.max() - slack
+            assert abs(logp - float(z[t] - z.logsumexp(0))) < slack
