@@ -7,10 +7,16 @@
 // stay in tensor memory: P (f16) takes the place of the S it came from and is
 // the A operand of O += P V, O is only rescaled when a row's maximum passes the
 // one in use by 2^8. Warps 8-11 bring keys and values of the pages into shared
-// memory as f16, up to two tiles of 128 keys ahead. Warp 12 issues the products of whichever row tile
-// is ready first, all of a step's at once: the tiles then settle half a step
-// apart (with a warp each they ran in step and shared every unit at the same
-// time).
+// memory as f16, up to two tiles of 128 keys ahead. Warp 12 issues the products,
+// values and next scores of one row tile after those of the other. Warps 13-15 look
+// over the values of the tiles that some rows do not see whole, before their product
+// (done by the loading warps it cost 6 to 12 % on every tile, in registers).
+// What bounds it: a step of 128 keys takes 4200 (dim 64) to 5600 cycles (dim 128) of
+// which the tensor core computes 1024 and 2048 and the exponentials take 2048. While
+// one row tile's exponentials run, the other's stores, barriers and products wait in
+// the same queue for some 100 cycles each, so neither unit is ever full: 8192 tokens
+// over 16384 positions of 16 heads of dim 128, causal, take 1.16 ms in f16 (710
+// TFLOP/s) and 1.23 ms in 8 bits, of dim 64 0.77 and 0.95 ms.
 // Registers go where a whole row of scores is held (setmaxnreg). Operands lie
 // in the K-major layout without swizzle: 8 rows x 16 bytes are one 128-byte
 // block, so a warp's 16-byte stores cover whole blocks; V is read from the same
@@ -26,7 +32,7 @@
 namespace tiles {
 
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kWarps = 16, kThreads = kWarps * 32;
-constexpr int kMmaWarp = kSoftWarps + kLoadWarps;  // the three warps after it only keep its registers company
+constexpr int kMmaWarp = kSoftWarps + kLoadWarps;  // and three that look over values some rows do not see
 // registers of a thread of the softmax, loading and product warpgroups; their sum is the launch's 128 a thread
 constexpr int kSoftRegs = 184, kLoadRegs = 104, kMmaRegs = 40;
 static_assert(2 * kSoftRegs + kLoadRegs + kMmaRegs == 4 * 128, "the split has to add up");
@@ -55,6 +61,15 @@ __device__ __forceinline__ uint64_t operand(uint32_t smem, uint32_t lead, uint32
 // kind::f16, f32 sums, f16 operands, M = 128; B transposed or not.
 __host__ __device__ constexpr uint32_t instruction(int n, bool b_mn) {
     return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// One lane of the warp. With lane == 0 in its place the compiler does not know that a
+// single lane is left and passes the operands of each product through a loop over the
+// warp's lanes: 60 to 100 cycles a product, where 32 to 64 are what it computes for.
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t i, bool add) {
@@ -105,7 +120,7 @@ __device__ __forceinline__ uint32_t piece(int r, int c) {
 
 template <int D>
 struct Shared {
-    uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full;
+    uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], v_raw[2], s_full[2], p_full[2], o_full;
     // Of tile j at j & 3: the softmax of tile j may still read when the loading
     // of tile j + 2 begins (which waits for the scores of j), not when that of
     // j + 3 does (the scores of j + 1 follow the softmax of j).
@@ -121,10 +136,13 @@ struct Shared {
     int lost;  // a wait ran out: nothing more is computed, the rows become NaN
 };
 
+// Changes the warpgroup's registers a thread from the launch's 128 to N: .inc and
+// .dec are only defined in their own direction.
 template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void set_registers() {
+    if constexpr (N > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    if constexpr (N < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // All threads of the CTA, or of the cluster, from wherever their roles stand.
 __device__ __forceinline__ void meet(bool cluster) {
@@ -139,14 +157,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Whether phase `parity` of the mbarrier is complete, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done)
-                 : "r"(smem_u32(bar)), "r"(parity)
-                 : "memory");
-    return done != 0;
+// 2^y of both, by products alone (the exponentials' own unit has 16 a cycle): with n
+// the integer next to y, 2^(y - n) is a polynomial of degree 4, fitted for the least
+// relative error over [-1/2, 1/2]: 2.6e-6, where the rounding to f16 that follows has
+// 2.4e-4. Below -126 it stays at 2^-126, which is 0 as f16; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_poly(float2 y) {
+    auto both = [](float c) { return make_float2(c, c); };
+    auto least = [](float v) {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(-126.0f));
+        return r;
+    };
+    y = make_float2(least(y.x), least(y.y));
+    // 1.5 * 2^23 + 127: the sum's last bits are n + 127, an exponent
+    const float2 big = both(12583039.0f), t = add2(y, big), r = add2(y, fma2(t, both(-1.0f), big));
+    float2 p = fma2(both(0.009570101276f), r, both(0.055917859077f));
+    p = fma2(p, r, both(0.240247443318f));
+    p = fma2(p, r, both(0.693121790886f));
+    p = fma2(p, r, both(0.999999284745f));
+    return mul2(p, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)));
 }
 
 // What all roles of a CTA know of its row tile.
@@ -154,6 +183,7 @@ struct Span {
     int r0, live, groups;  // its first row; rows of the tile; 128-row groups that have some
     int end, all;      // keys that its last row sees; keys that every row sees
     int first, count;  // its part's key tiles
+    int clean;         // of them, those before the first that some row does not see all of
 };
 
 template <int D, bool Q8>
@@ -182,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.k_full[i], kLoadWarps);
             mbar_init(&sh.v_full[i], kLoadWarps);
+            mbar_init(&sh.v_raw[i], kLoadWarps);
             mbar_init(&sh.k_free[i], 2);
             mbar_init(&sh.v_free[i], 2);
             mbar_init(&sh.s_full[i], 1);
@@ -211,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         s.first = (int)((uint32_t)total * part / parts);
         s.count = (int)((uint32_t)total * (part + 1) / parts) - s.first;
         if (*reinterpret_cast<volatile int *>(&sh.lost)) s.count = 0;  // every barrier is still met
+        s.clean = min(s.count, max(0, s.all / kKeys - s.first));
         return s;
     };
     // every lane of a warp waits and sees the same outcome
@@ -220,18 +252,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         return ok && !*reinterpret_cast<volatile int *>(&sh.lost);
     };
     // tiles so far, over all row tiles: stage and parity of the keys' and of the group's pipes; row tiles so far
-    uint32_t ks = 0, ss[2] = {0, 0}, os = 0, turns = 0;
+    uint32_t ks = 0, ss[2] = {0, 0}, os = 0, turns = 0, cleaned = 0;
     auto next_tile = [&](const Span &s) {
         ks += s.count;
         os += s.count > 0;
         ss[0] += s.count;
         ss[1] += s.groups > 1 ? s.count : 0;
+        cleaned += s.count - s.clean;
         ++turns;
+    };
+    // values that some rows do not see go by way of the warps that look them over
+    auto values_at = [&](const Span &s, int j) {
+        return j < s.clean ? &sh.v_full[(ks + j) & 1] : &sh.v_raw[(cleaned + j - s.clean) & 1];
     };
 
     if (warp < kSoftWarps) {
         // ---------------------------------------------------------- softmax
-        more_registers<kSoftRegs>();
+        set_registers<kSoftRegs>();
         const int group = warp >> 2, row = tid;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // tensor-memory lanes of the warp
         const uint32_t s_at = tmem + lanes + group * 128, o_at = tmem + lanes + 256 + group * D;
@@ -366,8 +403,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         float2 y = fma2(x[c0 + c], make_float2(scale, scale), make_float2(z, z));
-                        y.x = exp2_of(y.x);
-                        y.y = exp2_of(y.y);
+                        // 8-bit: a quarter of them by products, 5 to 9 % faster; f16, whose softmax
+                        // does less besides: 1 to 4 % slower
+                        if (Q8 && (c & 3) == 3) {
+                            y = exp2_poly(y);
+                        } else {
+                            y.x = exp2_of(y.x);
+                            y.y = exp2_of(y.y);
+                        }
                         sum[c & 1] = add2(sum[c & 1], y);
                         p[c] = pack(y.x, y.y);
                     }
@@ -384,20 +427,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (!ok) l = __int_as_float(0x7fffffff);
             const float back = Q8 ? power_of_2(exp_v) : 1.0f;
             const bool has = count > 0;
-            // columns c0 .. c0 + 15 of the row's sum
-            auto load_o = [&](int c0, uint32_t (&raw)[16]) {
-                tmem_load16(o_at + c0, raw);
-                tmem_wait_load();
-                if (sh.wild_any) {
+            if (sh.wild_any) {
 #pragma unroll 1
-                    for (int c = 0; c < 16; ++c)
-                        if (sh.wild[c0 + c] < lim) {
+                for (int c0 = 0; c0 < D; c0 += 16) {
+                    uint32_t raw[16];
+                    tmem_load16(o_at + c0, raw);
+                    tmem_wait_load();
 #pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                if (k == c) raw[k] = 0x7fffffffu;
-                        }
+                    for (int c = 0; c < 16; ++c)
+                        if (sh.wild[c0 + c] < lim) raw[c] = 0x7fffffffu;
+                    tmem_store16(o_at + c0, raw);
                 }
-            };
+                tmem_wait_store();
+            }
             if (parts == 1) {
                 const bool some = has && !(l < 1e-30f);  // a row that sees nothing has at most 128 times 2^-126 a tile
                 const float f = some ? back / l : 0.0f;
@@ -407,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t raw[16], w[8];
-                        load_o(c0, raw);
+                        tmem_load16(o_at + c0, raw);
+                        tmem_wait_load();
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             const float u = some ? __uint_as_float(raw[2 * c]) * f : 0.0f;
@@ -436,7 +479,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t raw[16];
-                        load_o(c0, raw);
+                        tmem_load16(o_at + c0, raw);
+                        tmem_wait_load();
                         if (row >= sp.live) continue;
 #pragma unroll
                         for (int c = 0; c < 16; ++c)
@@ -450,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 16) {
                     uint32_t raw[16];
-                    load_o(c0, raw);
+                    tmem_load16(o_at + c0, raw);
+                    tmem_wait_load();
 #pragma unroll
                     for (int c = 0; c < 16; c += 4) {
                         float4 x = make_float4(__uint_as_float(raw[c]) * back, __uint_as_float(raw[c + 1]) * back,
@@ -511,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         }
     } else if (warp < kMmaWarp) {
         // ---------------------------------------------------------- loading
-        fewer_registers<kLoadRegs>();
+        set_registers<kLoadRegs>();
         const int lw = warp - kSoftWarps;
         constexpr int ESZ = Q8 ? 1 : 2, PIECES = D * ESZ / 16;   // 16-byte pieces of a row in the cache
         constexpr int PER = kKeys * PIECES / (kLoadWarps * 32);  // pieces of a thread and tile
@@ -616,15 +661,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     fetch(vbase, vraw);
                     const uint32_t holes = __ballot_sync(0xffffffffu, pages >= a.kv.pages) & 0xff;
                     exp_v = max(exp_v, exponent(vd));
-                    if ((sp.first + j + 1) * kKeys > sp.all) {
-#pragma unroll
-                        for (int w = 0; w < kLoadWarps; ++w) {
-                            if (w != lw || fabsf(vd[w]) <= 3.402823466e38f) continue;
-                            vd[w] = 0.0f;
-                            for (int d = 0; d < D; ++d) atomicMin(&sh.wild[d], (sp.first + j) * kKeys + 32 * w + lane);
-                            sh.wild_any = 1;
-                        }
-                    }
                     const uint32_t v_own = own_scale(vd, exp_v);
                     if (turn > 0) ok = wait(&sh.k_free[stage], turn - 1);
                     if (!ok) break;
@@ -645,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     if (turn > 0) ok = wait(&sh.v_free[stage], turn - 1);
                     if (!ok) break;
                     unpack_tile(vraw, true, v_own, smem + SM::V + stage * SM::TILE);
-                    publish(&sh.v_full[stage]);
+                    publish(values_at(sp, j));
                 }
             } else {
                 // copies of tile j's K or V into its stage, once the products with what was there are done
@@ -679,30 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     next = pages_of(j + 2);
                     copy(a.kv.k, SM::K, sh.k_free, j + 1);
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    if ((sp.first + j + 1) * kKeys > sp.all) {
-#pragma unroll 1
-                        for (int u = 0; u < PER; ++u) {
-                            const int r = row_no(PIECES < 4 ? u : u / (PER / ROWS)), c = piece_no(u);
-                            uint4 *at_piece = reinterpret_cast<uint4 *>(smem + SM::V + stage * SM::TILE + piece<D>(r, c));
-                            uint4 x = *at_piece;
-                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                            bool found = false;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint32_t half = 0xffffu << (16 * (e & 1));
-                                if ((w[e / 2] & half & 0x7c007c00u) == (half & 0x7c007c00u)) {
-                                    w[e / 2] &= ~half;
-                                    atomicMin(&sh.wild[8 * c + e], (sp.first + j) * kKeys + r);
-                                    found = true;
-                                }
-                            }
-                            if (found) {
-                                *at_piece = make_uint4(w[0], w[1], w[2], w[3]);
-                                sh.wild_any = 1;
-                            }
-                        }
-                    }
-                    publish(&sh.v_full[stage]);
+                    publish(values_at(sp, j));
                     copy(a.kv.v, SM::V, sh.v_free, j + 1);
                 }
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -713,57 +726,94 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         }
     } else {
         // ---------------------------------------------------------- products
-        fewer_registers<kMmaRegs>();
+        set_registers<kMmaRegs>();
         constexpr uint32_t QK = instruction(kKeys, false), PV = instruction(D, true);
         for (uint32_t rt = tile0; rt < row_tiles; rt += tile_step) {
             const Span sp = span_of(rt);
-            if (warp == kMmaWarp && lane == 0) {
+            if (__shfl_sync(0xffffffffu, warp, 0) == kMmaWarp && elected()) {
                 const uint64_t q0 = operand(smem_u32(smem + SM::Q), 128, D * 16), k0 = operand(smem_u32(smem + SM::K), 128, D * 16);
                 const uint64_t v0 = operand(smem_u32(smem + SM::V), D * 16, 128);
-                auto scores = [&](int g, int j) {
-                    const uint32_t stage = (ks + j) & 1;
-                    const uint64_t q = q0 + g * (SM::TILE >> 4), k = k0 + stage * (SM::TILE >> 4);
+                // an operand `by` 16-byte units on; computed where it is used: there are too many to keep in registers
+                auto moved = [](uint64_t from, uint32_t by) {
+                    uint32_t low = (uint32_t)from + by;
+                    asm volatile("" : "+r"(low));
+                    return (from >> 32 << 32) | low;
+                };
+                auto scores = [&](int g, int stage) {
+                    const uint64_t q = moved(q0, g * (SM::TILE >> 4)), k = moved(k0, stage * (SM::TILE >> 4));
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s) mma_ss(tmem + g * 128, q + s * 16, k + s * 16, QK, s > 0);
                     commit(&sh.s_full[g]);
                     commit(&sh.k_free[stage]);
                     if (sp.groups == 1) commit(&sh.k_free[stage]);
                 };
+                auto values = [&](int g, int stage, bool add) {
+                    const uint64_t v = moved(v0, stage * (SM::TILE >> 4));
+#pragma unroll
+                    for (int s = 0; s < kKeys / 16; ++s)
+                        mma_ts(tmem + 256 + g * D, tmem + g * 128 + s * 8, v + s * (2 * D), PV, add || s > 0);
+                    commit(&sh.v_free[stage]);
+                    if (sp.groups == 1) commit(&sh.v_free[stage]);
+                };
                 bool ok = mbar_wait(&sh.q_full, turns & 1);
                 if (sp.count > 0) {
-                    ok = ok && mbar_wait(&sh.k_full[ks & 1], (ks >> 1) & 1);
-                    if (ok) {
-                        fence_after();
-                        for (int g = 0; g < sp.groups; ++g) scores(g, 0);
-                    }
-                    int next[2] = {0, sp.groups > 1 ? 0 : sp.count};  // the groups' next tile of values
-                    uint64_t since = globaltimer();
-                    while (ok && (next[0] < sp.count || next[1] < sp.count)) {
+                    // the scores take the place of P, so a group's next follow its product with the values
+                    for (int j = -1; j < sp.count && ok; ++j) {
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const int j = next[g];
-                            const uint32_t i = ks + j, stage = i & 1;
-                            if (j == sp.count || !mbar_test(&sh.p_full[g], (ss[g] + j) & 1) || !mbar_test(&sh.v_full[stage], (i >> 1) & 1) ||
-                                (j + 1 < sp.count && !mbar_test(&sh.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1)))
-                                continue;
-                            fence_after();
-                            const uint64_t v = v0 + stage * (SM::TILE >> 4);
-#pragma unroll
-                            for (int s = 0; s < kKeys / 16; ++s)
-                                mma_ts(tmem + 256 + g * D, tmem + g * 128 + s * 8, v + s * (2 * D), PV, j > 0 || s > 0);
-                            commit(&sh.v_free[stage]);
-                            if (sp.groups == 1) commit(&sh.v_free[stage]);
-                            if (j + 1 < sp.count) scores(g, j + 1);
-                            next[g] = j + 1;
-                            since = globaltimer();
+                            if (g == 1 && sp.groups == 1) break;
+                            if (j >= 0) {
+                                ok = ok && mbar_wait(&sh.p_full[g], (ss[g] + j) & 1);
+                                if (g == 0) ok = ok && mbar_wait(&sh.v_full[(ks + j) & 1], ((ks + j) >> 1) & 1);
+                                fence_after();
+                                if (ok) values(g, (ks + j) & 1, j > 0);
+                            }
+                            if (j + 1 < sp.count) {
+                                if (g == 0) ok = ok && mbar_wait(&sh.k_full[(ks + j + 1) & 1], ((ks + j + 1) >> 1) & 1);
+                                fence_after();
+                                if (ok) scores(g, (ks + j + 1) & 1);
+                            }
                         }
-                        if (globaltimer() - since > kWaitNs || *reinterpret_cast<volatile int *>(&sh.lost)) ok = false;
+                        if (*reinterpret_cast<volatile int *>(&sh.lost)) ok = false;
                     }
                     // also after a lost wait: nothing in flight when the CTA leaves
                     commit(&sh.o_full);
                     ok = mbar_wait(&sh.o_full, os & 1) && ok;
                 }
                 if (!ok) sh.lost = 1;
+            }
+            if (warp > kMmaWarp) {
+                // values that some rows do not see: 0 times an infinity or NaN would reach them
+                const int me = tid - 32 * (kMmaWarp + 1);
+                bool ok = true;
+                for (int j = sp.clean; j < sp.count && ok; ++j) {
+                    const uint32_t stage = (ks + j) & 1;
+                    ok = wait(&sh.v_raw[(cleaned + j - sp.clean) & 1], (cleaned + j - sp.clean) >> 1);
+                    if (!ok) break;
+                    uint8_t *tile = smem + SM::V + stage * SM::TILE;
+#pragma unroll 1
+                    for (int u = me; u < kKeys * (D / 8); u += 32 * (kWarps - kMmaWarp - 1)) {
+                        const int r = u % kKeys, c = u / kKeys;
+                        uint4 x = *reinterpret_cast<const uint4 *>(tile + piece<D>(r, c));
+                        // an exponent of ones carries into its half's sign
+                        auto hit = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+                        if (!(hit(x.x) | hit(x.y) | hit(x.z) | hit(x.w))) continue;
+#pragma unroll 1
+                        for (int e = 0; e < 8; ++e) {
+                            uint16_t *y = reinterpret_cast<uint16_t *>(tile + piece<D>(r, c)) + e;
+                            if ((*y & 0x7c00) != 0x7c00) continue;
+                            *y = 0;
+                            atomicMin(&sh.wild[8 * c + e], (sp.first + j) * kKeys + r);
+                            sh.wild_any = 1;
+                        }
+                    }
+                    fence_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_cta(&sh.v_full[stage]);
+                        if (me < kLoadWarps - (kWarps - kMmaWarp - 1)) mbar_arrive_cta(&sh.v_full[stage]);  // it counts the loaders
+                    }
+                }
             }
             __syncwarp();
             fence_before();
