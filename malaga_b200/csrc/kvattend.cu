@@ -828,12 +828,13 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
 
 // Which kernel. f32 queries, whose two f16 parts only the kernel for few rows
 // takes, and calls of at most kFewRows rows a cache head go there. So do calls of
-// at most 256 rows where it is faster, which measurements at dims 64 and 128 (100
-// and 200 new tokens, 300 to 30,000 positions, 2 to 16 heads, 1 to 16 sequences)
-// put as: it takes 4 us and (dim + 16) / 80 us for every 28,500 pairs of a 16-row
-// tile and a key, the tiles 1.3 + dim / 70 us for each of tiles_cost's key tiles.
-// 100 rows over 4000 positions, 16 heads of 64: 24 against 34 us; over 1500 in 16
-// sequences 93 against 68.
+// at most 256 rows where it is faster, which measurements at dims 16, 64 and 128
+// (100 to 250 new tokens, 1500 to 16,000 positions, 8 and 16 heads, 1 to 16
+// sequences) put as: it takes 6 us and 0.3 + dim / 95 us (8 bits: 0.6 + dim / 105)
+// for every 28,500 pairs of a 16-row tile and a key, the tiles 30 us (8 bits: 34)
+// and 0.3 + dim / 120 us for each of tiles_cost's key tiles. Over 4000 positions,
+// 16 heads of 64, f16: 100 rows 22 against 32 us, 200 rows 30 against 40; 100 rows
+// over 1500 in 16 sequences 98 against 63.
 template <int D>
 cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, cudaStream_t s) {
     const uint64_t rows = most_new * a.group;
@@ -841,7 +842,8 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
     if (!few && rows <= 256) {
         uint32_t parts;
         const double pairs = (double)((rows + 15) / 16 * a.kv.heads * a.seq.seqs) * (double)most_len;
-        few = 4.0 + pairs / 28500.0 * ((D + 16) / 80.0) < (double)tiles_cost(a, most_new, most_len, parts) * (1.3 + D / 70.0);
+        few = 6.0 + pairs / 28500.0 * (q8 ? 0.6 + D / 105.0 : 0.3 + D / 95.0) <
+              (q8 ? 34.0 : 30.0) + (double)tiles_cost(a, most_new, most_len, parts) * (0.3 + D / 120.0);
     }
     if (few) return launch_rows<D>(a, q8, rows, most_len, s);
     a.few = kFewRows;

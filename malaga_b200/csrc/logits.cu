@@ -25,7 +25,7 @@ constexpr uint32_t kNone = 0xffffffffu;
 
 #define kPosInf __int_as_float(0x7f800000)
 #define kLowest __int_as_float(0xff800000)
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLog2e = 1.44269504088896341f, kLog2eRest = 1.92596299e-8f;  // their sum is log2 e to 48 bits
 
 struct ChooseArgs {
     const void *x;
@@ -52,8 +52,14 @@ struct Best {
     uint32_t i;
 };
 
+// exp(m - top). It scales whole sums, so the rounding of its argument is made good:
+// over a row of 250,000 logits that error (1e-6 of the sum) was what the result's was.
 __device__ __forceinline__ float weight_of(float m, float top) {
-    return m == top ? 1.0f : m == kLowest ? 0.0f : exp2_of((m - top) * kLog2e);
+    if (m == top) return 1.0f;
+    const float d = m - top, h = d * kLog2e;
+    if (!(h > -150.0f)) return 0.0f;
+    const float rest = __fmaf_rn(d, kLog2e, -h) + d * kLog2eRest;
+    return exp2_of(h) * __fmaf_rn(rest, 0.693147180559945f, 1.0f);
 }
 
 __device__ __forceinline__ Best merge(const Best &a, const Best &b) {
@@ -64,9 +70,17 @@ __device__ __forceinline__ Best merge(const Best &a, const Best &b) {
     return Best{m, first ? a.l + (own + b.l) * w : b.l + (own + a.l) * w, first ? a.i : b.i};
 }
 
-__device__ __forceinline__ Best shfl_xor(const Best &a, int o) {
-    return Best{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.l, o),
-                __shfl_xor_sync(0xffffffffu, a.i, o)};
+// All lanes' together: the maximum first, so that each sum is scaled once.
+__device__ __forceinline__ Best join(const Best &a) {
+    Best b = a;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b.m = fmaxf(b.m, __shfl_xor_sync(0xffffffffu, b.m, o));
+    b.i = __reduce_min_sync(0xffffffffu, a.m == b.m ? a.i : kNone);
+    // a lane's own term joins the sum, unless it has none or it is the maximum's
+    b.l = ((a.i == kNone || a.i == b.i ? 0.0f : 1.0f) + a.l) * weight_of(a.m, b.m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b.l += __shfl_xor_sync(0xffffffffu, b.l, o);
+    return b;
 }
 
 // N logits y (-inf where they do not count) at tokens `first` + place(e) into b.
@@ -77,7 +91,7 @@ __device__ __forceinline__ void add(Best &b, const float (&y)[N], uint32_t first
     for (int e = 1; e < N; ++e) top = fmaxf(top, y[e]);
     float own = 0.0f;  // the new maximum's own term, which the sum below would add
     if (top > b.m) {
-        b.l = b.m == kLowest ? 0.0f : (1.0f + b.l) * exp2_of((b.m - top) * kLog2e);
+        b.l = b.m == kLowest ? 0.0f : (1.0f + b.l) * weight_of(b.m, top);
         b.m = top;
 #pragma unroll
         for (int e = N - 1; e >= 0; --e)
@@ -337,14 +351,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) choose_kernel
         }
     }
 
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+    best = join(best);
     if (lane == 0) warp_best[warp] = best;
     __syncthreads();
     if (warp == 0) {
-        best = lane < kWarps ? warp_best[lane] : Best{kLowest, 0.0f, kNone};
-#pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+        best = join(lane < kWarps ? warp_best[lane] : Best{kLowest, 0.0f, kNone});
     }
     if (parts > 1) {
         namespace cg = cooperative_groups;
@@ -353,9 +364,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) choose_kernel
         cluster_sync();
         if (part != 0) return;
         if (warp == 0) {
-            best = lane < parts ? cta_best[lane] : Best{kLowest, 0.0f, kNone};
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) best = merge(best, shfl_xor(best, o));
+            best = join(lane < parts ? cta_best[lane] : Best{kLowest, 0.0f, kNone});
         }
     }
     if (tid == 0) {
