@@ -11,7 +11,7 @@
 // values and next scores of one row tile after those of the other. Warps 13-15 look
 // over the values of the tiles that some rows do not see whole, before their product
 // (done by the loading warps it cost 6 to 12 % on every tile, in registers).
-// What bounds it: a step of 128 keys takes 4200 (dim 64) to 5600 cycles (dim 128) of
+// What bounds it: a step of 128 keys in f16 takes 4200 (dim 64) to 5600 cycles (dim 128) of
 // which the tensor core computes 1024 and 2048 and the exponentials take 2048. While
 // one row tile's exponentials run, the other's stores, barriers and products wait in
 // the same queue for some 100 cycles each, so neither unit is ever full: 8192 tokens

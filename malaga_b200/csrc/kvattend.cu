@@ -49,6 +49,7 @@ struct AttendArgs {
     bool overlap;    // the kernel for few rows runs beside the one for many
     uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
+    uint32_t span;   // few rows: a sequence is cut into one part each `span` keys
 };
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -135,6 +136,12 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 // by 2^8, so most blocks need one vote and no reduction across lanes. Warps
 // join in shared memory, the CTAs of a cluster (which cut the keys among them)
 // through distributed shared memory, in a fixed order.
+//
+// What bounds it: HBM with long f16 caches (6.3 TB/s at dim 128), the instructions a
+// key with 8-bit ones (8 sequences, 233,369 positions, 8 heads of 128, four rows
+// each: 112 us, 4.4 TB/s), latencies with short ones (one row of 33 positions, 16
+// heads of 64: 3.7 us; 64 sequences of 272 positions on average and 1024 at most, 16
+// heads of 64, 8 bits: 21 us, of which the longest sequence's loop is 12).
 
 template <int D, bool Q8>
 struct Frag {
@@ -490,7 +497,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
     __shared__ float row_scale[R], wm[kRowWarps][R], wl[kRowWarps][R], cm[R], cl[R], weight[16][R];
     __shared__ int row_limit[R];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
+    const uint32_t part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
     // beside the launch for many rows, which has seen the one before it end
     if (a.overlap) let_next_start();
@@ -506,6 +513,9 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         if (keeper) wait_for_previous();
         return;
     }
+    // a shorter sequence takes fewer of the cluster's CTAs; the others leave (its barriers count the threads that stay)
+    const uint32_t parts = min(gridDim.x, ((uint32_t)max(len, 1) + a.span - 1) / a.span);
+    if (part >= parts) return;
     uint8_t *ring = smem + warp * (RG::N * RG::STAGE);
     uint32_t put = 0, get = 0;  // next stage to fill and to read
     uint32_t have = 0;          // BLOCKS bits a stage: which of its blocks are in the cache
@@ -795,20 +805,26 @@ cudaError_t launch_rows(const AttendArgs &a, dim3 grid, cudaStream_t s) {
 }
 
 // Keys are cut over the CTAs of a cluster (at most 16) while all CTAs still run
-// at once and every warp keeps two blocks, and further while a CTA would have
-// more than 2048 keys: sequences of unlike lengths then even out.
+// at once and every warp keeps two blocks, and further, from 3 * 1024 positions on,
+// while a CTA would have more than 1024 keys: sequences of unlike lengths then even
+// out. A sequence that is shorter than the longest takes as few of the CTAs as keep
+// the longest's share of keys, 512 at most. Against cuts at 2048 for all: 32 sequences
+// of 200 to 6000 positions, 8 heads of 64, 8 bits 42 -> 30 us, 96 of 100 to 8000, dim
+// 128, 107 -> 100; twice as many cuts cost sequences of like lengths up to 20 %.
 template <int D, bool Q8, bool SPLIT, int NT>
-cudaError_t launch_rows(const AttendArgs &a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
+cudaError_t launch_rows(AttendArgs a, uint64_t rows, uint64_t most_len, cudaStream_t s) {
     constexpr int SMEM = Ring<D, Q8>::BYTES + Frag<D, Q8>::STATIC * NT, FIT = 227 * 1024 / SMEM;
     constexpr int SLOTS = 148 * (FIT < Frag<D, Q8>::ctas(NT) ? FIT : Frag<D, Q8>::ctas(NT));
     uint64_t tiles = (rows + 8 * NT - 1) / (8 * NT);
     if (tiles * a.kv.heads > 65535) tiles = 65535 / a.kv.heads;
     const uint64_t base = tiles * a.kv.heads * a.seq.seqs;
     uint64_t parts = base < SLOTS ? SLOTS / base : 1;
-    if (parts < most_len / 2048) parts = most_len / 2048;
+    if (most_len >= 3 * 1024 && parts < most_len / 1024) parts = most_len / 1024;
     if (parts > most_len / (kRowWarps * 32)) parts = most_len / (kRowWarps * 32);
     // sizes that pack into the GPU's clusters of 16 or 18 SMs
     parts = parts >= 16 ? 16 : parts >= 8 ? 8 : parts >= 4 ? 4 : parts < 1 ? 1 : parts;
+    a.span = (uint32_t)((most_len + parts - 1) / parts);
+    a.span = a.span < 1 ? 1 : a.span > 512 ? 512 : a.span;
     return launch_rows<D, Q8, SPLIT, NT>(a, dim3((unsigned)parts, (unsigned)(tiles * a.kv.heads), a.seq.seqs), s);
 }
 
@@ -909,7 +925,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
-                 false, 0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e};
+                 false, 0xffffffffu, (scale == 0.0f ? 1e-30f : scale) * kLog2e, 1};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;

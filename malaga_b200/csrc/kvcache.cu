@@ -1,6 +1,10 @@
 // Writing rows into a paged K/V cache, and reading them back.
 //
-// Both move each number once and compute next to nothing, so HBM bounds them.
+// Both move each number once, so HBM is their floor. Measured, K and V of 16 heads
+// of 128: writing 17,221 bf16 tokens as 8-bit codes takes 72 us (3.0 TB/s; the
+// exact quotients keep 70 % of the issue slots busy and bound it), reading 45,789
+// tokens of 8 heads back as f16 66 us (4.3 TB/s, waiting for loads). 64 tokens of 64
+// take 2.7 us a launch.
 // A CTA takes a run of the call's tokens: its threads first look up each
 // token's place (a search for its sequence, then the page table), then move the
 // rows of all heads, K and V. A row is spread over dim / 8 lanes of 8 numbers;
