@@ -129,9 +129,9 @@ struct Shared {
     uint32_t holes[4];  // bit i: keys 16 i .. 16 i + 15 of the tile have no page
     float m[256], l[256], weight[8][256];
     // Where some rows of the tile do not see a key, an infinity or NaN in its V is
-    // taken out (0 times it would reach them) and noted: rows that see key wild[d]
-    // get NaN in dim d. wild_any: whether there is one.
-    int wild[D], wild_any;
+    // taken out (0 times it would reach them) and noted: NaN (0), +inf (1) or -inf (2)
+    // is added to dim d of rows that see key wild[.][d]. wild_any: whether there is one.
+    int wild[3][D], wild_any;
     uint32_t tmem;
     int lost;  // a wait ran out: nothing more is computed, the rows become NaN
 };
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         sh.lost = 0;
         sh.wild_any = 0;
     }
-    if (tid < D) sh.wild[tid] = 0x7fffffff;
+    for (int u = tid; u < 3 * D; u += kThreads) (&sh.wild[0][0])[u] = 0x7fffffff;
     fence_before();
     __syncthreads();
     fence_after();
@@ -435,7 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     tmem_wait_load();
 #pragma unroll
                     for (int c = 0; c < 16; ++c)
-                        if (sh.wild[c0 + c] < lim) raw[c] = 0x7fffffffu;
+                        for (int k = 0; k < 3; ++k)
+                            if (sh.wild[k][c0 + c] < lim)
+                                raw[c] = __float_as_uint(__uint_as_float(raw[c]) + __uint_as_float(k == 0 ? 0x7fffffffu : k == 1 ? 0x7f800000u : 0xff800000u));
                     tmem_store16(o_at + c0, raw);
                 }
                 tmem_wait_store();
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 sh.l[row] = l;
             }
             asm volatile("barrier.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-            if (tid < D) sh.wild[tid] = 0x7fffffff;
+            for (int u = tid; u < 3 * D; u += kSoftWarps * 32) (&sh.wild[0][0])[u] = 0x7fffffff;
             if (tid == 0) sh.wild_any = 0;
             fence_before();
             meet(parts > 1);
@@ -802,8 +804,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                         for (int e = 0; e < 8; ++e) {
                             uint16_t *y = reinterpret_cast<uint16_t *>(tile + piece<D>(r, c)) + e;
                             if ((*y & 0x7c00) != 0x7c00) continue;
+                            atomicMin(&sh.wild[*y & 0x3ff ? 0 : 1 + (*y >> 15)][8 * c + e], (sp.first + j) * kKeys + r);
                             *y = 0;
-                            atomicMin(&sh.wild[8 * c + e], (sp.first + j) * kKeys + r);
                             sh.wild_any = 1;
                         }
                     }

@@ -367,6 +367,30 @@ def test_masked_values_never_reach_a_row(ops, fmt, new):
 
 
 @gpu_only
+@pytest.mark.parametrize("new", [9, 150, 300, 700])
+@pytest.mark.parametrize("dim", [16, 128])
+def test_infinite_values_keep_their_sign(ops, new, dim):
+    """A row that sees an infinite V gets that infinity in its dim, one that sees both signs NaN, the others neither."""
+    torch = _torch()
+    length = new + 37
+    c = Case(ops, "f16", 1, dim, 16, [new], [length])
+    for at, d, x in ((3, 9, math.inf), (length - 7, 2, math.inf), (length - 4, 2, -math.inf), (length - 4, 5, -math.inf)):
+        c.cache.v[c.tables[0][at // 16], 0, at % 16, d] = x
+        c.values[0][1][at, 0, d] = x
+    q = 0.1 * torch.randn(new, 1, dim, device="cuda").half()
+    with np.errstate(invalid="ignore"):
+        want, _ = attend_plain(q.cpu().double().numpy(), c.values, c.new, c.lens, dim ** -0.5, True, 2.0 ** -15, 2.0 ** -11, 2.0 ** -11)
+    got = c.cache.attend(c.seqs, q).cpu().double().numpy()
+    fin = np.isfinite(want)
+    assert np.isposinf(want[:, 0, 9]).all() and np.isneginf(want[-1, 0, 5]) and np.isnan(want[-1, 0, 2]) and np.isposinf(want[-6, 0, 2])
+    np.testing.assert_array_equal(got[~fin], want[~fin])
+    assert np.isfinite(got[fin]).all()
+    _, tol = attend_plain(q.cpu().double().numpy(), [[np.nan_to_num(x, posinf=0.0, neginf=0.0) for x in kv] for kv in c.values], c.new,
+                          c.lens, dim ** -0.5, True, 2.0 ** -15, 2.0 ** -11, 2.0 ** -11)
+    assert (np.abs(got[fin] - want[fin]) <= tol[fin]).all()
+
+
+@gpu_only
 @pytest.mark.parametrize("fmt", ["f16", "q8"])
 @pytest.mark.parametrize("new", [3, 100])
 def test_attend_holes_hints_and_scales(ops, fmt, new):
