@@ -896,10 +896,13 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
               (q8 ? 34.0 : 30.0) + (double)tiles_cost(a, most_new, most_len, parts) * (0.3 + D / 120.0);
     }
     if (few) return launch_rows<D>(a, q8, rows, most_len, s);
-    a.few = kFewRows;
+    // Sequences of unlike lengths: there may be some of few rows, which go to the other
+    // kernel. The host knows bounds, not lengths (the rows may be more than the sequences
+    // have, a bound too small), so without the second launch the tiles take them all.
+    const bool both = a.seq.tokens < most_new * a.seq.seqs;
+    a.few = both ? kFewRows : 0;
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
-    // sequences of unlike lengths: there may be some of few rows
-    if (e == cudaSuccess && a.seq.tokens < most_new * a.seq.seqs) {
+    if (e == cudaSuccess && both) {
         a.overlap = true;
         e = launch_rows<D>(a, q8, kFewRows, most_len, s);
     }

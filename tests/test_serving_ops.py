@@ -416,6 +416,55 @@ def test_attend_holes_hints_and_scales(ops, fmt, new):
 
 
 @gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+@pytest.mark.parametrize("new,lens,rows,bound", [
+    ([300, 1], [400, 90], 1024, 300),     # rows to spare behind the sequences'
+    ([300, 1], [400, 90], 602, 301),
+    ([40], [140], 512, 512),
+    ([1], [77], 512, 512),
+    ([2, 0, 64, 65], [5, 0, 90, 70], 2048, 512),
+    ([599, 1], [640, 50], 600, 300),      # a bound that is too small
+    ([700, 1, 7], [800, 500, 7], 708, 200),
+])
+def test_every_sequence_is_computed(ops, fmt, new, lens, rows, bound):
+    """Whatever the bound and the number of rows say of the sequences' lengths: no row of theirs keeps what out held."""
+    torch = _torch()
+    c = Case(ops, fmt, 2, 64, 16, new, lens, seed=rows)
+    seqs = ops.Seqs(*c.seqs.tensors, bound, max(lens))
+    spare = np.zeros((rows, 4, 64), bool)
+    spare[sum(new):] = True
+    for dt in (torch.float16, torch.bfloat16, torch.float32):
+        q = torch.randn(rows, 4, 64, device="cuda").to(dt)
+        check_attend(ops, c, dt, 2, seqs=seqs, q=q, out=torch.full_like(q, math.nan), skip=spare)
+
+
+@gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+def test_graph_replayed_over_other_lengths(ops, fmt):
+    """A step captured for up to 512 new tokens, replayed for the last chunk of a prompt and for single tokens."""
+    torch = _torch()
+    c = Case(ops, fmt, 2, 64, 16, [512, 512], [700, 600])
+    start, length = (x.clone() for x in c.seqs.tensors[1:])
+    seqs = ops.Seqs(c.seqs.tensors[0], start, length, 512, 700)
+    q = torch.randn(1024, 2, 64, device="cuda").half()
+    out = torch.empty_like(q)
+    c.cache.attend(seqs, q, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.cache.attend(seqs, q, out=out)
+    for new, lens in (([512, 512], [700, 600]), ([40, 512], [700, 600]), ([512, 1], [600, 600]), ([40, 1], [40, 555]), ([1, 1], [1, 600])):
+        start.copy_(torch.tensor([0, new[0], sum(new)], dtype=torch.int32))
+        length.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(math.nan)
+        graph.replay()
+        want, tol = attend_plain(q.cpu().double().numpy(), [[x[:n] for x in kv] for kv, n in zip(c.values, lens)], new, lens,
+                                 64 ** -0.5, True, 2.0 ** -15, 2.0 ** -11, 2.0 ** -11)
+        got = out.cpu().double().numpy()
+        assert (np.abs(got - want) <= tol)[: sum(new)].all()
+
+
+@gpu_only
 @pytest.mark.parametrize("new", [2, 130])
 def test_attend_strides_and_types(ops, new):
     torch = _torch()
