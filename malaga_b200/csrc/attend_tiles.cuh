@@ -26,7 +26,9 @@
 // them into K as it is unpacked was 4 % faster and made the error of f16
 // outputs 3.2e-4 -> 6.8e-4); V's scales, over the running exponent, multiply its
 // codes as they are unpacked, one rounding of the product to f16 (the scale
-// enters as a high and a low part).
+// enters as a high and a low part). In the tiles that some rows do not see whole
+// V's scales multiply P instead, over a row's own exponent: that of a key which a
+// row does not see must not move the row's numbers out of f16's range.
 #pragma once
 
 namespace tiles {
@@ -124,8 +126,8 @@ struct Shared {
     // Of tile j at j & 3: the softmax of tile j may still read when the loading
     // of tile j + 2 begins (which waits for the scores of j), not when that of
     // j + 3 does (the scores of j + 1 follow the softmax of j).
-    alignas(16) float k_scale[4][kKeys];
-    int v_exp[4];       // V of the tile is over 2^v_exp
+    alignas(16) float k_scale[4][kKeys], v_scale[4][kKeys];
+    int v_exp[4];       // V of the tile is over 2^v_exp, where all rows see all of it
     uint32_t holes[4];  // bit i: keys 16 i .. 16 i + 15 of the tile have no page
     float m[256], l[256], weight[8][256];
     // Where some rows of the tile do not see a key, an infinity or NaN in its V is
@@ -261,9 +263,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         cleaned += s.count - s.clean;
         ++turns;
     };
-    // values that some rows do not see go by way of the warps that look them over
+    // values that some rows do not see go by way of the warps that look them over (8-bit codes are finite)
     auto values_at = [&](const Span &s, int j) {
-        return j < s.clean ? &sh.v_full[(ks + j) & 1] : &sh.v_raw[(cleaned + j - s.clean) & 1];
+        return Q8 || j < s.clean ? &sh.v_full[(ks + j) & 1] : &sh.v_raw[(cleaned + j - s.clean) & 1];
     };
 
     if (warp < kSoftWarps) {
@@ -387,7 +389,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll
                 for (int c = 0; c < kKeys / 2; ++c) top[c & 3] = max3(top[c & 3], x[c].x, x[c].y);
                 const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale;
-                const int e = Q8 ? sh.v_exp[slot] : exp_v;
+                const bool folded = Q8 && j >= sp.clean;  // V's scales go into P
+                const float *vscale = sh.v_scale[slot];
+                int e = Q8 ? sh.v_exp[slot] : exp_v;
+                if (folded) {
+                    float most = 0.0f;
+#pragma unroll 4
+                    for (int key = 0; key < kKeys; key += 4) {
+                        const float4 d = *reinterpret_cast<const float4 *>(vscale + key);
+                        const float most4[4] = {fabsf(d.x), fabsf(d.y), fabsf(d.z), fabsf(d.w)};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (key0 + key + i < lim && !((holes >> (key >> 4)) & 1)) most = fmaxf(most, most4[i]);
+                    }
+                    e = max(exp_v, min(126, (__float_as_int(most) >> 23) - 126));
+                }
                 if (__any_sync(0xffffffffu, best > m + kSlack || e != exp_v)) {
                     const float now = fmaxf(m, best), w = m == kLowest ? 0.0f : exp2_of(m - now);
                     m = now;
@@ -418,6 +434,26 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_store();
+                if (folded) {  // in a pass of its own: within the loop above it cost 5 to 11 % on every tile, in registers
+                    const float over_e = __int_as_float((127 - e) << 23);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kKeys / 2; c0 += 16) {
+                        uint32_t p[16];
+                        tmem_load16(s_at + c0, p);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            const int key = 2 * (c0 + c);
+                            const float2 d = *reinterpret_cast<const float2 *>(vscale + key), y = unpack(p[c]);
+                            // 0 where the key is not seen, whatever its scale
+                            const bool hole = (holes >> (key >> 4)) & 1;
+                            p[c] = pack(key0 + key < lim && !hole ? y.x * (d.x * over_e) : 0.0f,
+                                        key0 + key + 1 < lim && !hole ? y.y * (d.y * over_e) : 0.0f);
+                        }
+                        tmem_store16(s_at + c0, p);
+                    }
+                    tmem_wait_store();
+                }
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cta(&sh.p_full[group]);
@@ -613,18 +649,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 };
                 // over the tile's 128 keys: the exponent that their largest scale stays below
                 auto exponent = [&](const float (&d)[kLoadWarps]) {
-                    float top = fabsf(d[0]);
+                    float top = 0.0f;  // NaN never is the larger
 #pragma unroll
-                    for (int w = 1; w < kLoadWarps; ++w) top = fmaxf(top, fabsf(d[w]));
+                    for (int w = 0; w < kLoadWarps; ++w) top = fmaxf(top, fabsf(d[w]));
                     return min(126, ((int)__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 126);
                 };
-                // the scale of the warp's key `lane` over 2^e, as a high and a low f16 part
-                auto own_scale = [&](const float (&d)[kLoadWarps], int e) {
+                // the scale of the warp's key `lane`
+                auto own_scale = [&](const float (&d)[kLoadWarps]) {
                     float x = d[0];
 #pragma unroll
                     for (int w = 1; w < kLoadWarps; ++w)
                         if (w == lw) x = d[w];
-                    x *= __int_as_float((127 - e) << 23);
+                    return x;
+                };
+                // as a high and a low f16 part
+                auto parts_of = [&](float x) {
                     const __half hi = __float2half_rn(x);
                     const __half2 both = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
                     return *reinterpret_cast<const uint32_t *>(&both);
@@ -662,11 +701,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     const uint32_t stage = (ks + j) & 1, turn = (ks + j) >> 1, slot = (ks + j) & 3;
                     fetch(vbase, vraw);
                     const uint32_t holes = __ballot_sync(0xffffffffu, pages >= a.kv.pages) & 0xff;
-                    exp_v = max(exp_v, exponent(vd));
-                    const uint32_t v_own = own_scale(vd, exp_v);
+                    const float own = own_scale(vd);
+                    const bool folded = j >= sp.clean;
+                    if (!folded) exp_v = max(exp_v, exponent(vd));
+                    const uint32_t v_own = parts_of(folded ? 1.0f : own * __int_as_float((127 - exp_v) << 23));
                     if (turn > 0) ok = wait(&sh.k_free[stage], turn - 1);
                     if (!ok) break;
                     sh.k_scale[slot][32 * lw + lane] = kd;
+                    sh.v_scale[slot][32 * lw + lane] = own;
                     if (lw == 0 && lane == 0) {
                         sh.v_exp[slot] = exp_v;
                         sh.holes[slot] = holes;
@@ -788,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 // values that some rows do not see: 0 times an infinity or NaN would reach them
                 const int me = tid - 32 * (kMmaWarp + 1);
                 bool ok = true;
-                for (int j = sp.clean; j < sp.count && ok; ++j) {
+                for (int j = Q8 ? sp.count : sp.clean; j < sp.count && ok; ++j) {
                     const uint32_t stage = (ks + j) & 1;
                     ok = wait(&sh.v_raw[(cleaned + j - sp.clean) & 1], (cleaned + j - sp.clean) >> 1);
                     if (!ok) break;

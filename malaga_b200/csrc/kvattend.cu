@@ -60,6 +60,10 @@ __device__ __forceinline__ float exp2_of(float x) {
 
 __device__ __forceinline__ float power_of_2(int e) { return e < -126 ? 0.0f : __int_as_float((e + 127) << 23); }
 
+// 1 / the power of two above d >= 0, kept between 2^-126 and 2^126; the inverse of such a number.
+__device__ __forceinline__ float over(float d) { return __int_as_float((253 - min(252, __float_as_int(d) >> 23)) << 23); }
+__device__ __forceinline__ float inverse(float power) { return __int_as_float((254 << 23) - __float_as_int(power)); }
+
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -272,7 +276,9 @@ struct Rows {
     int all;  // keys below are seen by every row
     float o[NT][F::STEPS][4];
     float m[NT][2], l[NT][2];
-    int exp_v;  // V's scales so far are below 2^exp_v
+    // 8-bit caches: of the V scales that the row has seen the largest is below 1 / back, a power of two. A row's
+    // own: a scale in a place that it does not see must not push its weights out of f16's range.
+    float back[NT][2];
     int k_at, v_at;  // where the lane's reads of a stage begin
 
     // have: bit i, block i of the stage is in the cache; key0: the stage's first key
@@ -350,16 +356,20 @@ struct Rows {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) past |= s[i][n][e] > m[n][e & 1] + kSlack;
-            if constexpr (Q8) d = fmaxf(d, fmaxf(fabsf(x[i].vs[0]), fabsf(x[i].vs[1])));
-        }
-        if constexpr (Q8) past |= (__float_as_int(d) >> 23) - 126 > exp_v;
-        if (__any_sync(0xffffffffu, past)) {
-            float f = 1.0f;
             if constexpr (Q8) {
-                const int e = max(exp_v, min(126, (__float_as_int(max_keys(d)) >> 23) - 126));
-                f = power_of_2(exp_v - e);
-                exp_v = e;
+                d = fmaxf(d, fmaxf(fabsf(x[i].vs[0]), fabsf(x[i].vs[1])));
+                if (!whole) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) past |= s[i][n][e] != kLowest && fabsf(x[i].vs[e >> 1]) * back[n][e & 1] >= 1.0f;
+                }
             }
+        }
+        // a whole block follows keys that all rows have seen, so the first row's back is that of all
+        if (Q8 && whole) past |= d * back[0][0] >= 1.0f;
+        if (__any_sync(0xffffffffu, past)) {
+            if constexpr (Q8) d = max_keys(d);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -371,14 +381,29 @@ struct Rows {
                     const float w = m[n][r] == kLowest ? 0.0f : exp2_of(m[n][r] - top);
                     m[n][r] = top;
                     l[n][r] *= w;
+                    float f = w;
+                    if constexpr (Q8) {
+                        float seen = d;
+                        if (!whole) {
+                            seen = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < B; ++i)
+#pragma unroll
+                                for (int u = 0; u < 2; ++u)
+                                    if (s[i][n][2 * u + r] != kLowest) seen = fmaxf(seen, fabsf(x[i].vs[u]));
+                            seen = max_keys(seen);
+                        }
+                        const float now = fminf(back[n][r], over(seen));
+                        f *= now * inverse(back[n][r]);
+                        back[n][r] = now;
+                    }
 #pragma unroll
                     for (int j = 0; j < F::STEPS; ++j) {
-                        o[n][j][r] *= w * f;
-                        o[n][j][2 + r] *= w * f;
+                        o[n][j][r] *= f;
+                        o[n][j][2 + r] *= f;
                     }
                 }
         }
-        const float back = Q8 ? __int_as_float((127 - exp_v) << 23) : 1.0f;
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             if (B > 1 && !((have >> i) & 1)) continue;
@@ -392,12 +417,14 @@ struct Rows {
                 for (int e = 0; e < 4; ++e) {
                     w[e] = exp2_of(s[i][n][e] - z[e & 1]);
                     l[n][e & 1] += w[e];
-                    if constexpr (Q8) w[e] *= x[i].vs[e >> 1] * back;
                 }
-                if (Q8 && !whole) {  // a masked key's scale may be NaN
+                if (Q8 && whole) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] *= x[i].vs[e >> 1] * back[0][0];
+                } else if (Q8) {  // a masked key's scale may be NaN
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (s[i][n][e] == kLowest) w[e] = 0.0f;
+                        w[e] = s[i][n][e] == kLowest ? 0.0f : w[e] * (x[i].vs[e >> 1] * back[n][e & 1]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -636,7 +663,6 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         }
         __syncthreads();
         Rows<D, Q8, SPLIT, NT> st;
-        st.exp_v = -126;
         st.k_at = F::byte(g, t * F::KB);
         st.v_at = F::byte(2 * t, g * F::VB);
         st.all = row_limit[0];  // what the rows past `live` see does not matter
@@ -663,6 +689,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                 st.limit[j][r] = row_limit[8 * j + 2 * t + r];
                 st.m[j][r] = kLowest;
                 st.l[j][r] = 0.0f;
+                st.back[j][r] = over(0.0f);
             }
 #pragma unroll
             for (int s = 0; s < F::STEPS; ++s)
@@ -701,7 +728,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                 float top = wm[0][row];
 #pragma unroll
                 for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, wm[w][row]);
-                const float f = st.m[j][r] == kLowest ? 0.0f : exp2_of(st.m[j][r] - top) * (Q8 ? power_of_2(st.exp_v) : 1.0f);
+                const float f = st.m[j][r] == kLowest ? 0.0f : exp2_of(st.m[j][r] - top) * (Q8 ? inverse(st.back[j][r]) : 1.0f);
 #pragma unroll
                 for (int s = 0; s < F::STEPS; ++s) {
                     so[warp][row][F::v_dim(g, 2 * s)] = st.o[j][s][r] * f;

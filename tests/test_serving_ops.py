@@ -367,6 +367,49 @@ def test_masked_values_never_reach_a_row(ops, fmt, new):
 
 
 @gpu_only
+@pytest.mark.parametrize("new,first", [(9, 5), (60, 20), (150, 30), (512, 400), (700, 130)])
+@pytest.mark.parametrize("dim", [32, 128])
+@pytest.mark.parametrize("size", [math.nan, math.inf, 2.0 ** 40])
+def test_scales_of_later_tokens_never_reach_a_row(ops, new, first, dim, size):
+    """However large V's scales are from new token `first` on, and where they are no numbers: the tokens before see none
+    of them, and later ones what the definition says of finite scales."""
+    torch = _torch()
+    length = new + 37
+    c = Case(ops, "q8", 1, dim, 16, [new], [length], seed=new)
+    for p in range(length - new + first, length):
+        page, at = c.tables[0][p // 16], p % 16
+        c.cache.v_scale[page, 0, at] *= size
+        with np.errstate(invalid="ignore"):
+            c.values[0][1][p] = c.cache.v[page, :, at].cpu().double().numpy() * c.cache.v_scale[page, :, at].cpu().double().numpy()[:, None]
+    later = np.zeros((new, 2, dim), bool)
+    later[first:] = not math.isfinite(size)
+    c.values = [[np.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) for x in kv] for kv in c.values]
+    for dt in (torch.float16, torch.bfloat16, torch.float32):
+        q = torch.randn(new, 2, dim, device="cuda").to(dt)
+        out = torch.empty(new, 2, dim, device="cuda")
+        got = check_attend(ops, c, dt, 2, q=q, out=out, skip=later)
+        assert np.isfinite(got[:first]).all()
+        if not math.isfinite(size):  # a code of 0 times an infinity is no number either
+            assert not np.isfinite(got[first:]).any()
+
+
+@gpu_only
+@pytest.mark.parametrize("new,first", [(512, 400), (1000, 390)])
+def test_scales_without_a_number_for_long(ops, new, first):
+    """Whole tiles of later tokens whose V scales are NaN: the tokens before keep their values."""
+    torch = _torch()
+    c = Case(ops, "q8", 1, 64, 128, [new], [new])
+    clean = [[x.copy() for x in kv] for kv in c.values]
+    for p in range(first, new):
+        c.cache.v_scale[c.tables[0][p // 128], 0, p % 128] = math.nan
+    later = np.zeros((new, 1, 64), bool)
+    later[first:] = True
+    q = torch.randn(new, 1, 64, device="cuda").half()
+    got = check_attend(ops, c, torch.float16, q=q, values=clean, skip=later)
+    assert np.isnan(got[first:]).all()
+
+
+@gpu_only
 @pytest.mark.parametrize("new", [9, 150, 300, 700])
 @pytest.mark.parametrize("dim", [16, 128])
 def test_infinite_values_keep_their_sign(ops, new, dim):
