@@ -461,8 +461,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (sp.count > 0 && ok) ok = wait(&sh.o_full, os);
             fence_after();
             if (!ok) l = __int_as_float(0x7fffffff);
-            const float back = Q8 ? power_of_2(exp_v) : 1.0f;
-            const bool has = count > 0;
+            // a row that sees nothing has at most 128 times 2^-126 a tile
+            const bool some = count > 0 && !(l < 1e-30f);
+            const float f = some ? (Q8 ? power_of_2(exp_v) : 1.0f) / l : 0.0f;
             if (sh.wild_any) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 16) {
@@ -479,8 +480,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                 tmem_wait_store();
             }
             if (parts == 1) {
-                const bool some = has && !(l < 1e-30f);  // a row that sees nothing has at most 128 times 2^-126 a tile
-                const float f = some ? back / l : 0.0f;
                 if (a.o_vec16) {
                     // through the warp's rows of Q, which no product reads any more, to whole rows of 16-bit numbers
                     constexpr int PIECES = D / 8;
@@ -536,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
                     tmem_wait_load();
 #pragma unroll
                     for (int c = 0; c < 16; c += 4) {
-                        float4 x = make_float4(__uint_as_float(raw[c]) * back, __uint_as_float(raw[c + 1]) * back,
-                                               __uint_as_float(raw[c + 2]) * back, __uint_as_float(raw[c + 3]) * back);
-                        if (!has) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        float4 x = make_float4(__uint_as_float(raw[c]) * f, __uint_as_float(raw[c + 1]) * f,
+                                               __uint_as_float(raw[c + 2]) * f, __uint_as_float(raw[c + 3]) * f);
+                        if (!some) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         reinterpret_cast<float4 *>(o)[((c0 + c) / 4 + row) % (D / 4)] = x;
                     }
                 }
@@ -553,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (parts > 1) {
                 namespace cg = cooperative_groups;
                 auto cluster = cg::this_cluster();
-                // the parts' weights of a row, over the row's sum
+                // the parts' weights of a row
                 if (row < sp.live) {
                     float its[8], sum = 0.0f, best = kLowest;
 #pragma unroll
@@ -564,11 +563,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         const float lc = c < (int)parts ? *cluster.map_shared_rank(&sh.l[row], c) : 0.0f;
-                        its[c] = its[c] == kLowest ? 0.0f : exp2_of(its[c] - best);
-                        sum += lc != lc ? lc : its[c] * lc;
+                        its[c] = lc != lc ? lc : its[c] == kLowest ? 0.0f : exp2_of(its[c] - best) * lc;
+                        sum += its[c];
                     }
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) sh.weight[c][row] = sum < 1e-30f ? 0.0f : sum != sum ? sum : its[c] / sum;
+                    for (int c = 0; c < 8; ++c) sh.weight[c][row] = sum < 1e-30f ? 0.0f : its[c] / sum;
                 }
                 asm volatile("barrier.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
                 const float4 *o = reinterpret_cast<const float4 *>(smem + SM::K);

@@ -264,6 +264,9 @@ __device__ __forceinline__ float sum_keys(float x) {
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+// A part's sum l of exponentials over its own maximum m, over `top`. Where it has seen nothing (-inf) l is 0, or NaN.
+__device__ __forceinline__ float weighed(float m, float l, float top) { return m == kLowest ? l : l * exp2_of(m - top); }
+
 // NT: tiles of 8 rows. State of a warp: per row (2t and 2t + 1 of each tile,
 // the same in all lanes of equal t) the near maximum m; l is this lane's share.
 template <int D, bool Q8, bool SPLIT, int NT>
@@ -725,22 +728,26 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
             for (int r = 0; r < 2; ++r) {
                 const int row = 8 * j + 2 * t + r;
                 if (row >= live) continue;
-                float top = wm[0][row];
+                float top = wm[0][row], sum = 0.0f;
 #pragma unroll
                 for (int w = 1; w < kRowWarps; ++w) top = fmaxf(top, wm[w][row]);
-                const float f = st.m[j][r] == kLowest ? 0.0f : exp2_of(st.m[j][r] - top) * (Q8 ? inverse(st.back[j][r]) : 1.0f);
+#pragma unroll
+                for (int w = 0; w < kRowWarps; ++w) sum += weighed(wm[w][row], wl[w][row], top);
+                // the CTA's sum first: over V's power the outputs alone could pass f32's range
+                const float f = st.m[j][r] == kLowest || sum == 0.0f ? 0.0f : exp2_of(st.m[j][r] - top) / sum;
+                const float unit = Q8 ? inverse(st.back[j][r]) : 1.0f;
 #pragma unroll
                 for (int s = 0; s < F::STEPS; ++s) {
-                    so[warp][row][F::v_dim(g, 2 * s)] = st.o[j][s][r] * f;
-                    so[warp][row][F::v_dim(g, 2 * s + 1)] = st.o[j][s][2 + r] * f;
+                    so[warp][row][F::v_dim(g, 2 * s)] = st.o[j][s][r] * f * unit;
+                    so[warp][row][F::v_dim(g, 2 * s + 1)] = st.o[j][s][2 + r] * f * unit;
                 }
             }
-        if (tid < live) {
+        if (parts > 1 && tid < live) {
             float top = kLowest, sum = 0.0f;
 #pragma unroll
             for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, wm[w][tid]);
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) sum += wm[w][tid] == kLowest ? wl[w][tid] : wl[w][tid] * exp2_of(wm[w][tid] - top);
+            for (int w = 0; w < kRowWarps; ++w) sum += weighed(wm[w][tid], wl[w][tid], top);
             cm[tid] = top;
             cl[tid] = sum;
         }
@@ -772,7 +779,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
         if (parts > 1) {
             for (int u = tid; u < live * (D / W); u += kRowThreads) reinterpret_cast<Numbers *>(&so[0][0][0])[u] = of_warps(u).all;
             cluster_sync();
-            // the CTAs' weights of a row, over the row's sum; where WIDE, all of their maxima and sums are
+            // the CTAs' weights of a row; where WIDE, all of their maxima and sums are
             // fetched at once, into the place of the second warp's outputs
             float(*part_m)[R] = reinterpret_cast<float(*)[R]>(&so[1][0][0]), (*part_l)[R] = part_m + 16;
             static_assert(!WIDE || D >= 32, "two times sixteen parts' numbers fit in a warp's outputs");
@@ -789,12 +796,11 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                 float top = kLowest, sum = 0.0f;
                 for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, m_of(c));
                 for (uint32_t c = 0; c < parts; ++c) {
-                    const float m = m_of(c), l = l_of(c);
-                    const float f = m == kLowest ? 0.0f : exp2_of(m - top);
-                    weight[c][tid] = f;
-                    sum += m == kLowest ? l : f * l;
+                    weight[c][tid] = weighed(m_of(c), l_of(c), top);
+                    sum += weight[c][tid];
                 }
-                row_scale[tid] = sum;
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                for (uint32_t c = 0; c < parts; ++c) weight[c][tid] *= f;
             }
             __syncthreads();
         }
@@ -808,11 +814,8 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
 #pragma unroll 4
                 for (uint32_t c = 0; c < parts; ++c) add(sum, weight[c][r], cluster.map_shared_rank(&so[0][0][0], c), u);
             }
-            const float l = parts == 1 ? cl[r] : row_scale[r];
             const int rr = r0 + r, i = rr / (int)a.group, h = rr - i * (int)a.group;
             const int64_t to = (t0 + i) * a.o_token + (int64_t)(head * a.group + h) * a.o_head + d;
-#pragma unroll
-            for (int e = 0; e < W; ++e) sum.at[e] = l == 0.0f ? 0.0f : sum.at[e] / l;
             if constexpr (W == 4) store4(a.out, to, a.o_type, a.o_vec, sum.at);
             else store1(a.out, (size_t)to, a.o_type, sum.at[0]);
         }

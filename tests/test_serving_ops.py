@@ -369,7 +369,7 @@ def test_masked_values_never_reach_a_row(ops, fmt, new):
 @gpu_only
 @pytest.mark.parametrize("new,first", [(9, 5), (60, 20), (150, 30), (512, 400), (700, 130)])
 @pytest.mark.parametrize("dim", [32, 128])
-@pytest.mark.parametrize("size", [math.nan, math.inf, 2.0 ** 40])
+@pytest.mark.parametrize("size", [math.nan, math.inf, 2.0 ** 40, 1e36])
 def test_scales_of_later_tokens_never_reach_a_row(ops, new, first, dim, size):
     """However large V's scales are from new token `first` on, and where they are no numbers: the tokens before see none
     of them, and later ones what the definition says of finite scales."""
@@ -391,6 +391,22 @@ def test_scales_of_later_tokens_never_reach_a_row(ops, new, first, dim, size):
         assert np.isfinite(got[:first]).all()
         if not math.isfinite(size):  # a code of 0 times an infinity is no number either
             assert not np.isfinite(got[first:]).any()
+
+
+@gpu_only
+@pytest.mark.parametrize("new,length", [(1, 40), (3, 9001), (20, 700), (150, 160), (300, 2100)])
+@pytest.mark.parametrize("size", [1e36, 1e-34])
+def test_values_near_the_ends_of_the_range(ops, new, length, size):
+    """Values of 1e37 and of 1e-34: the outputs are as large, the sums before the division by the weights' would not be."""
+    torch = _torch()
+    c = Case(ops, "q8", 2, 64, 64, [new], [length])
+    c.cache.v_scale *= size
+    v = [c.cache.v[c.tables[0][p // 64], :, p % 64].cpu().double().numpy()
+         * c.cache.v_scale[c.tables[0][p // 64], :, p % 64].cpu().double().numpy()[:, None] for p in range(length)]
+    c.values[0][1] = np.stack(v)
+    for dt in (torch.float16, torch.float32):
+        q = torch.randn(new, 4, 64, device="cuda").to(dt)
+        check_attend(ops, c, dt, 2, q=q, out=torch.empty(new, 4, 64, device="cuda"))
 
 
 @gpu_only
