@@ -621,14 +621,23 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
             if (Q8 || a.q_type != MGB_F16) {
 #pragma unroll
                 for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // the row's largest number to just below 2^14 (f16 q over f16 caches stays as it is), by 2^shift in two
+                // factors, since either may leave the range of f32 alone. Undone, a row below 2^-100 or so has lost bits
+                // of its scale, which leaves f32's normal numbers.
+                const int shift = m > 0.0f && m <= kHuge ? 140 - (__float_as_int(m) >> 23) : 0;
+                const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
+                const float f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
+                m = m * f1 * f2;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = x[e] * f1 * f2;
+                undo = undo * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
             }
             if constexpr (Q8) {
                 // q as whole numbers over the row's largest; a row with an infinity or NaN gets an infinite scale, and
                 // so scores of NaN
                 constexpr float kMost = SPLIT ? 127 * 16384 + 8191 : 127 * 128 + 63;
-                const bool tiny = m < 1e-30f;  // as good as zeros, whose scores are 0
-                const float inv = tiny ? 0.0f : kMost / m;
-                undo = tiny ? a.scale : a.scale * (m / kMost);
+                const float inv = m == 0.0f ? 0.0f : kMost / m;
+                undo *= m / kMost;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     int v = __float2int_rn(x[e] * inv);
@@ -642,21 +651,11 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
                     sd[DIGITS - 1][r][c * E + e] = (int8_t)(v - (mid << 7));
                 }
             } else {
-                // the row's largest number to just below 2^14 (f16 q stays as it is)
-                float f1 = 1.0f, f2 = 1.0f;
-                if (a.q_type != MGB_F16) {
-                    // 2^shift in two factors, since either may leave the range of f32 alone
-                    const int shift = m > 0.0f && m <= kHuge ? 140 - (__float_as_int(m) >> 23) : 0;
-                    const int s1 = max(-100, min(100, shift)), s2 = shift - s1;
-                    f1 = __int_as_float((127 + s1) << 23), f2 = __int_as_float((127 + s2) << 23);
-                    undo = a.scale * __int_as_float((127 - s1) << 23) * __int_as_float((127 - s2) << 23);
-                }
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float y = x[e] * f1 * f2;
-                    const __half hi = __float2half_rn(y);
+                    const __half hi = __float2half_rn(x[e]);
                     sq[0][r][c * E + e] = hi;
-                    if constexpr (SPLIT) sq[SPLIT][r][c * E + e] = __float2half_rn(y - __half2float(hi));
+                    if constexpr (SPLIT) sq[SPLIT][r][c * E + e] = __float2half_rn(x[e] - __half2float(hi));
                 }
             }
             if (c == 0) {

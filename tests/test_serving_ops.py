@@ -566,6 +566,21 @@ def test_attend_query_and_cache_ranges(ops, magnitude):
 
 
 @gpu_only
+@pytest.mark.parametrize("new", [3, 80])
+@pytest.mark.parametrize("magnitude", [1e-31, 4e-31])
+def test_tiny_queries_count(ops, new, magnitude):
+    """Queries below 1e-30 over keys as large as they are small."""
+    torch = _torch()
+    c = Case(ops, "q8", 1, 32, 16, [new], [new + 20])
+    c.cache.k_scale /= magnitude
+    c.values[0][0] = np.stack([c.cache.k[c.tables[0][p // 16], :, p % 16].cpu().double().numpy()
+                               * c.cache.k_scale[c.tables[0][p // 16], :, p % 16].cpu().double().numpy()[:, None] for p in range(new + 20)])
+    q = torch.randn(new, 1, 32, device="cuda") * magnitude
+    check_attend(ops, c, torch.float32, q=q)
+    check_attend(ops, c, torch.bfloat16, q=q.bfloat16())
+
+
+@gpu_only
 def test_cache_beyond_32_bit_offsets(ops):
     """Places whose numbers lie past 2^31 of a side."""
     torch = _torch()
