@@ -304,12 +304,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
 #pragma unroll
                     for (int u = 0; u < PER; ++u) raw[u] = ahead[u];
                     if (q < 3) fetch(q + 1, ahead);
-                    float mul = fabsf(a.scale);
-                    const float sign = copysignf(1.0f, a.scale);
+                    // the scale's sign goes into Q, and so does a scale of 0: the masked scores' -inf times it has to stay -inf
+                    float mul = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+                    const float sign = a.scale == 0.0f ? 0.0f : copysignf(1.0f, a.scale);
                     if (a.q_type == MGB_F16) {
-                        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+                        const __half2 s = __float2half2_rn(sign);
+                        auto signed2 = [&](uint32_t w) {
+                            const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&w), s);
+                            return *reinterpret_cast<const uint32_t *>(&x);
+                        };
 #pragma unroll
-                        for (int u = 0; u < PER; ++u) raw[u].x ^= flip, raw[u].y ^= flip, raw[u].z ^= flip, raw[u].w ^= flip;
+                        for (int u = 0; u < PER; ++u) raw[u] = make_uint4(signed2(raw[u].x), signed2(raw[u].y), signed2(raw[u].z), signed2(raw[u].w));
                     } else {
                         uint32_t top = 0;  // of the magnitudes' bits
 #pragma unroll

@@ -581,6 +581,21 @@ def test_tiny_queries_count(ops, new, magnitude):
 
 
 @gpu_only
+@pytest.mark.parametrize("new", [3, 300])
+@pytest.mark.parametrize("scale", [0.0, -0.0])
+def test_a_scale_of_zero(ops, new, scale):
+    """Every key that is seen counts alike, however large the products are."""
+    torch = _torch()
+    for fmt, size in (("q8", 1e12), ("f16", 1.0)):
+        c = Case(ops, fmt, 1, 32, 16, [new], [new + 20])
+        if fmt == "q8":
+            c.cache.k_scale *= size
+        for dt, top in ((torch.float32, 1e22), (torch.bfloat16, 1e22), (torch.float16, 1e4)):
+            q = (torch.randn(new, 1, 32, device="cuda") * (top if fmt == "q8" else 1.0)).to(dt)
+            check_attend(ops, c, dt, q=q, scale=scale)
+
+
+@gpu_only
 def test_cache_beyond_32_bit_offsets(ops):
     """Places whose numbers lie past 2^31 of a side."""
     torch = _torch()
