@@ -284,8 +284,25 @@ struct Rows {
     float back[NT][2];
     int k_at, v_at;  // where the lane's reads of a stage begin
 
-    // have: bit i, block i of the stage is in the cache; key0: the stage's first key
-    __device__ __forceinline__ void step(const uint8_t *stage, uint32_t have, int key0, int end, int g, int t) {
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                m[n][r] = kLowest;
+                l[n][r] = 0.0f;
+                back[n][r] = over(0.0f);
+            }
+#pragma unroll
+            for (int j = 0; j < F::STEPS; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
+        }
+    }
+
+    // have: bit i, block i of the stage is in the cache; key0: the stage's first key; careful: look for infinities in
+    // blocks that all rows see, too
+    __device__ __forceinline__ void step(const uint8_t *stage, uint32_t have, int key0, int end, int g, int t, bool careful) {
         constexpr int B = Ring<D, Q8>::BLOCKS;
         Block<D, Q8> x[B];
         float s[B][NT][4];  // key g: rows 2t, 2t + 1; key g + 8: the same
@@ -439,15 +456,13 @@ struct Rows {
                     }
                 }
             }
-            auto pair = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            // O += the weights' high or low part times V^T's part
+            auto part = [&](int low, int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
                 const uint32_t f[4] = {a0, a1, a2, a3};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma16(o[n][j], f, p[0][n][0], p[0][n][1]);
-                    if constexpr (SPLIT) mma16(o[n][j], f, p[SPLIT][n][0], p[SPLIT][n][1]);
-                }
+                for (int n = 0; n < NT; ++n) mma16(o[n][j], f, p[low][n][0], p[low][n][1]);
             };
-            auto products = [&] {
+            auto products = [&](auto pair) {  // pair(step, its part of V^T)
 #pragma unroll
                 for (int c = 0; c < F::VW; ++c) {
                     if constexpr (Q8) {
@@ -468,9 +483,10 @@ struct Rows {
             };
             if constexpr (!Q8) {
                 // 0 times an infinity or NaN would reach rows that do not see its key: such a block goes key by key,
-                // and every row keeps what it had where the key is masked
+                // and every row keeps what it had where the key is masked. The weights' low parts, which may be 0 or
+                // below it, only meet finite values.
                 bool wild = false;
-                if (!whole) {
+                if (!whole || (SPLIT && careful)) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -482,6 +498,16 @@ struct Rows {
                 }
                 if (wild) {
                     const Block<D, Q8> all_keys = x[i];
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+#pragma unroll
+                            for (int c = 0; c < F::VW; ++c) {
+                                if ((x[i].v[u][c] & 0x7c00u) == 0x7c00u) x[i].v[u][c] &= 0xffff0000u;
+                                if ((x[i].v[u][c] & 0x7c000000u) == 0x7c000000u) x[i].v[u][c] &= 0xffffu;
+                            }
+                        products([&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) { part(SPLIT, j, a0, a1, a2, a3); });
+                    }
 #pragma unroll 1
                     for (int key = 0; key < 16; ++key) {
                         float kept[NT][F::STEPS][4];
@@ -495,7 +521,7 @@ struct Rows {
                         for (int u = 0; u < 4; ++u)
 #pragma unroll
                             for (int c = 0; c < F::VW; ++c) x[i].v[u][c] = 2 * t + (u & 1) + 8 * (u >> 1) == key ? all_keys.v[u][c] : 0u;
-                        products();
+                        products([&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) { part(0, j, a0, a1, a2, a3); });
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -507,7 +533,10 @@ struct Rows {
                     continue;
                 }
             }
-            products();
+            products([&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                part(0, j, a0, a1, a2, a3);
+                if constexpr (SPLIT) part(SPLIT, j, a0, a1, a2, a3);
+            });
         }
     }
 };
@@ -689,24 +718,37 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT)) attend_row
             for (int r = 0; r < 2; ++r) {
                 st.scale[j][r] = row_scale[8 * j + 2 * t + r];
                 st.limit[j][r] = row_limit[8 * j + 2 * t + r];
-                st.m[j][r] = kLowest;
-                st.l[j][r] = 0.0f;
-                st.back[j][r] = over(0.0f);
             }
-#pragma unroll
-            for (int s = 0; s < F::STEPS; ++s)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) st.o[j][s][e] = 0.0f;
         }
 
-        for (int i = 0; i < mine; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(RG::N - 1) : "memory");
-            __syncwarp();
-            const uint32_t got = (have >> (get * RG::BLOCKS)) & ((1u << RG::BLOCKS) - 1);
-            if (got) st.step(ring + get * RG::STAGE, got, block_of(i) * 16, end, g, t);
-            __syncwarp();  // every lane has read the stage
-            issue(i + RG::N);
-            get = get + 1 == RG::N ? 0 : get + 1;
+        // f32 queries over f16 caches: the weights' low parts times an infinity in V are NaN where the row has that
+        // infinity. Looking for those in every block would cost a fifth of the instructions, so a warp whose
+        // outputs have a NaN takes its keys again, looking.
+        for (bool careful = false;; careful = true) {
+            st.clear();
+            for (int i = 0; i < mine; ++i) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(RG::N - 1) : "memory");
+                __syncwarp();
+                const uint32_t got = (have >> (get * RG::BLOCKS)) & ((1u << RG::BLOCKS) - 1);
+                if (got) st.step(ring + get * RG::STAGE, got, block_of(i) * 16, end, g, t, careful);
+                __syncwarp();  // every lane has read the stage
+                issue(i + RG::N);
+                get = get + 1 == RG::N ? 0 : get + 1;
+            }
+            if constexpr (SPLIT && !Q8) {
+                bool nan = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int s = 0; s < F::STEPS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) nan |= st.o[n][s][e] != st.o[n][s][e];
+                if (careful || !__any_sync(0xffffffffu, nan)) break;
+#pragma unroll
+                for (int i = 0; i < RG::N; ++i) issue(i);  // the ring is empty, what is left in flight are empty groups
+            } else {
+                break;
+            }
         }
 
         // the CTA's warps

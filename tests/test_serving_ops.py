@@ -450,6 +450,33 @@ def test_infinite_values_keep_their_sign(ops, new, dim):
 
 
 @gpu_only
+@pytest.mark.parametrize("new", [1, 9, 150, 300])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_infinite_values_keep_their_sign_for_wider_queries(ops, new, dim, dtype):
+    """As above where the weights have two parts, or q is scaled: infinities that all rows see, and that some do."""
+    torch = _torch()
+    dt, length = getattr(torch, dtype), new + 70
+    c = Case(ops, "f16", 1, dim, 16, [new], [length])
+    for at, d, x in ((3, 9, math.inf), (40, 11, -math.inf), (41, 12, math.inf), (50, 12, -math.inf), (length - 1, 5, -math.inf),
+                     (60, 13, math.nan)):
+        c.cache.v[c.tables[0][at // 16], 0, at % 16, d] = x
+        c.values[0][1][at, 0, d] = x
+    q = (0.1 * torch.randn(new, 2, dim, device="cuda")).to(dt)
+    single = dt == torch.float32
+    units = (2.0 ** -21, 2.0 ** -21, 2.0 ** -24) if single else (2.0 ** -15, 2.0 ** -11, 2.0 ** -24)
+    with np.errstate(invalid="ignore"):
+        want, _ = attend_plain(q.cpu().double().numpy(), c.values, c.new, c.lens, dim ** -0.5, True, *units)
+    got = c.cache.attend(c.seqs, q, out=torch.empty(new, 2, dim, device="cuda")).cpu().double().numpy()
+    fin = np.isfinite(want)
+    assert np.isposinf(want[..., 9]).all() and np.isneginf(want[..., 11]).all() and np.isnan(want[..., 12]).all() and np.isneginf(want[-1, :, 5]).all()
+    np.testing.assert_array_equal(got[~fin], want[~fin])
+    _, tol = attend_plain(q.cpu().double().numpy(), [[np.nan_to_num(x, posinf=0.0, neginf=0.0) for x in kv] for kv in c.values], c.new,
+                          c.lens, dim ** -0.5, True, *units)
+    assert (np.abs(got[fin] - want[fin]) <= tol[fin]).all()
+
+
+@gpu_only
 @pytest.mark.parametrize("fmt", ["f16", "q8"])
 @pytest.mark.parametrize("new", [3, 100])
 def test_attend_holes_hints_and_scales(ops, fmt, new):
