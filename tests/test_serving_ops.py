@@ -369,7 +369,7 @@ def test_masked_values_never_reach_a_row(ops, fmt, new):
 @gpu_only
 @pytest.mark.parametrize("new,first", [(9, 5), (60, 20), (150, 30), (512, 400), (700, 130)])
 @pytest.mark.parametrize("dim", [32, 128])
-@pytest.mark.parametrize("size", [math.nan, math.inf, 2.0 ** 40, 1e36])
+@pytest.mark.parametrize("size", [math.nan, math.inf, 2.0 ** 8, 2.0 ** 12, 2.0 ** 16, 2.0 ** 40, 1e36])
 def test_scales_of_later_tokens_never_reach_a_row(ops, new, first, dim, size):
     """However large V's scales are from new token `first` on, and where they are no numbers: the tokens before see none
     of them, and later ones what the definition says of finite scales."""
