@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
             else hi = mid;
         }
         int64_t row = -1;
-        const int start = a.seq.q_start[lo], stop = a.seq.q_start[lo + 1];
+        const int start = hi ? a.seq.q_start[lo] : 0, stop = hi ? a.seq.q_start[lo + 1] : 0;  // hi: there are sequences
         if (token >= start && token < stop) {
             const long long pos = (long long)a.seq.kv_len[lo] - (stop - token);
             if (pos >= 0 && (pos >> a.kv.page_log2) < a.seq.table_stride) {
@@ -232,7 +232,7 @@ mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, co
     if (!bad && (k->tokens != v->tokens)) bad = "K and V differ in their tokens";
     if (!bad && (k->heads != kv->heads || v->heads != kv->heads)) bad = "the rows' heads are not the cache's";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
-    if (seqs->seqs == 0 || k->tokens == 0) return MGB_OK;
+    if (k->tokens == 0 || (WRITE && seqs->seqs == 0)) return MGB_OK;  // a read without sequences is of zeros
     MoveArgs a{view(*kv), view(*seqs, k->tokens),
                {{k->data, k->token_stride, k->head_stride, static_cast<uint8_t *>(kv->k), kv->k_scale},
                 {v->data, v->token_stride, v->head_stride, static_cast<uint8_t *>(kv->v), kv->v_scale}},

@@ -132,7 +132,7 @@ inline const char *check_kv(const mgb_kv *kv) {
 }
 
 inline const char *check_seqs(const mgb_kv_seqs *s) {
-    if (!s || !s->table || !s->q_start || !s->kv_len) return "null sequence pointer";
+    if (!s || (s->seqs && (!s->q_start || !s->kv_len || (s->table_stride && !s->table)))) return "null sequence pointer";
     if (s->seqs > 65535) return "more than 65535 sequences";
     return nullptr;
 }

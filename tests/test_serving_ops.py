@@ -274,6 +274,28 @@ def test_places_that_do_not_exist(ops):
                 assert torch.equal(c.cache.k[page].view(torch.int8), before[page].view(torch.int8))
 
 
+@gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+def test_no_sequences(ops, fmt):
+    """A call without sequences writes nothing and reads zeros, whether or not there are rows."""
+    torch = _torch()
+    cache = ops.PagedKV.empty(3, 2, 16, 32, fmt)
+    cache.k.fill_(5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for seqs in (ops.Seqs.of([], [], []), ops.Seqs(torch.zeros(0, 4, **i32), torch.zeros(1, **i32), torch.zeros(0, **i32))):
+        out = tuple(torch.full((7, 2, 32), 3.0, device="cuda") for _ in range(2))
+        cache.read(seqs, out=out)
+        assert (out[0] == 0).all() and (out[1] == 0).all()
+        cache.write(seqs, *(torch.ones(7, 2, 32, device="cuda") for _ in range(2)))
+        assert (cache.k == 5).all() and (cache.v == 0).all()
+        assert cache.read(ops.Seqs(*seqs.tensors, tokens=0))[0].shape == (0, 2, 32)
+    # sequences without any room: positions that do not exist
+    seqs = ops.Seqs(torch.zeros(2, 0, **i32), torch.tensor([0, 3, 4], **i32), torch.tensor([5, 1], **i32), tokens=4)
+    cache.write(seqs, *(torch.ones(4, 2, 32, device="cuda") for _ in range(2)))
+    assert (cache.k == 5).all() and all((x == 0).all() for x in cache.read(seqs))
+    assert (cache.attend(seqs, torch.randn(4, 4, 32, device="cuda")) == 0).all()
+
+
 # ---------------------------------------------------------------------------
 # Attention
 
