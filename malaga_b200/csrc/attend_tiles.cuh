@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
     begin();
+    zero_outside(a, b);
     int n;
     const int t0 = a.seq.first(b, n);
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows

@@ -252,6 +252,38 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
+// Zeros into rows [from, to) of the call, by the CTAs of one sequence (all of them, in whatever shape of block). A
+// call of its own: inlined into the kernels it moved their registers.
+__device__ __noinline__ void zero_rows(void *out, int type, bool vec, long long o_token, long long o_head, uint32_t q_heads, uint32_t quads, int from, int to) {
+    const size_t ctas = (size_t)gridDim.x * gridDim.y, cta = blockIdx.x + (size_t)gridDim.x * blockIdx.y;
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (size_t u = cta * blockDim.x + threadIdx.x; u < (size_t)(to - from) * q_heads * quads; u += ctas * blockDim.x) {
+        const size_t r = u / quads;
+        store4(out, (from + (long long)(r / q_heads)) * o_token + (long long)(r % q_heads) * o_head + 4 * (long long)(u % quads), type, vec, zero);
+    }
+}
+__device__ __forceinline__ void zero_rows(const AttendArgs &a, int from, int to) {
+    zero_rows(a.out, a.o_type, a.o_vec, a.o_token, a.o_head, a.kv.heads * a.group, a.kv.dim / 4, from, to);
+}
+
+// Rows before the first sequence's and behind the last one's see nothing: zeros.
+__device__ __forceinline__ void zero_outside(const AttendArgs &a, uint32_t b) {
+    const int tokens = (int)a.seq.tokens;
+    if (b == 0) {
+        const int first = min(tokens, a.seq.q_start[0]);
+        if (first > 0) zero_rows(a, 0, first);
+    }
+    if (b + 1 == a.seq.seqs) {
+        const int stop = max(0, a.seq.q_start[a.seq.seqs]);
+        if (stop < tokens) zero_rows(a, stop, tokens);
+    }
+}
+
+__global__ void __launch_bounds__(256) attend_nothing_kernel(const AttendArgs a) {
+    begin();
+    zero_rows(a, 0, (int)a.seq.tokens);
+}
+
 // Over the eight lanes that share t (the keys of a block).
 __device__ __forceinline__ float max_keys(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -560,8 +592,12 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
     const uint32_t part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
     // beside the launch for many rows, which has seen the one before it end
-    if (a.overlap) let_next_start();
-    else begin();
+    if (a.overlap) {
+        let_next_start();
+    } else {
+        begin();
+        zero_outside(a, b);
+    }
     int n;
     const int t0 = a.seq.first(b, n);
     const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
@@ -1009,7 +1045,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (!bad && (q->heads == 0 || q->heads % kv->heads)) bad = "query heads are not a multiple of the cache's";
     if (!bad && (uint64_t)q->tokens * q->heads > 0x7fffffffu) bad = "more than 2^31 - 1 query rows";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
-    if (seqs->seqs == 0 || q->tokens == 0) return MGB_OK;
+    if (q->tokens == 0) return MGB_OK;
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
@@ -1018,6 +1054,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
     cudaError_t e;
+    if (seqs->seqs == 0) return op_launch_status(op_launch(attend_nothing_kernel, dim3(148), 256, 0, 1, a, s), op);
     switch (kv->dim) {
         case 16: e = launch<16>(a, q8, most_new, most_len, s); break;
         case 32: e = launch<32>(a, q8, most_new, most_len, s); break;

@@ -178,7 +178,8 @@ class PagedKV:
         """Attention of the new tokens' queries q [tokens, query heads, dim] over their sequences:
         softmax(scale * q k) v, scale 1 / sqrt(dim) unless given. Query head h reads cache head
         h // (query heads / heads). causal: a token sees the positions up to its own, else all of its
-        sequence. A token that sees nothing gets zeros. Returns out (q's type and shape unless given)."""
+        sequence. A token that sees nothing gets zeros, and so does a row of no sequence. Returns out (q's
+        type and shape unless given)."""
         self._check(seqs)
         cq = _rows(q, "q", self.index, self.dim)
         if out is None:

@@ -547,6 +547,31 @@ def test_every_sequence_is_computed(ops, fmt, new, lens, rows, bound):
 
 
 @gpu_only
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("new,before,after,bound", [
+    ([1, 3], 0, 5, 3), ([1, 3], 2, 0, 3), ([300], 7, 213, 300), ([300, 40, 1], 1, 700, 300), ([300, 2], 0, 900, 300), ([0, 0], 0, 9, 0), ([], 0, 40, 0)])
+def test_rows_of_no_sequence_are_zeros(ops, dtype, new, before, after, bound):
+    """Rows before the first sequence's and behind the last one's, whichever kernel runs; places between rows stay."""
+    torch = _torch()
+    dt = getattr(torch, dtype)
+    c = Case(ops, "q8", 2, 32, 16, new, [n + 50 for n in new])
+    table, start, length = c.seqs.tensors
+    seqs = ops.Seqs(table, start + before, length, bound, max([n + 50 for n in new], default=0))
+    tokens = before + sum(new) + after
+    q = torch.randn(tokens, 6, 32, device="cuda").to(dt)
+    for wide in (32, 33):  # rows that allow wide stores, and that do not
+        out = torch.full((tokens, 6, wide + 8), math.nan, device="cuda", dtype=dt)
+        c.cache.attend(seqs, q, out=out[..., :32])
+        got = out[..., :32].float()
+        assert (got[:before] == 0).all() and (got[before + sum(new):] == 0).all() and torch.isnan(out[..., 32:]).all()
+        mine = slice(before, before + sum(new))
+        want, tol = attend_plain(q[mine].cpu().double().numpy(), c.values, c.new, c.lens, 32 ** -0.5, True,
+                                 *((2.0 ** -21,) * 2 if dt == torch.float32 else (2.0 ** -15, 2.0 ** -11)), UNIT[dtype])
+        assert (np.abs(got[mine].cpu().double().numpy() - want) <= tol + 1e-30).all()
+    assert (c.cache.attend(seqs, q)[before + sum(new):] == 0).all()
+
+
+@gpu_only
 @pytest.mark.parametrize("fmt", ["f16", "q8"])
 def test_graph_replayed_over_other_lengths(ops, fmt):
     """A step captured for up to 512 new tokens, replayed for the last chunk of a prompt and for single tokens."""
