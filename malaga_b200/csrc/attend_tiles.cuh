@@ -201,11 +201,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
     begin();
     zero_outside(a, b);
-    int n;
-    const int t0 = a.seq.first(b, n);
+    int n, stand;
+    const int t0 = a.seq.first(b, n, stand);
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
     if ((uint32_t)rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
-    const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;
+    const int len = a.seq.length(b, a.kv.page_log2);
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     auto limit = [&](int i) { return a.causal ? max(0, min(len, stand + i + 1)) : len; };
 

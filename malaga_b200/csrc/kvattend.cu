@@ -598,9 +598,9 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
         begin();
         zero_outside(a, b);
     }
-    int n;
-    const int t0 = a.seq.first(b, n);
-    const int len = a.seq.length(b, a.kv.page_log2), stand = a.seq.kv_len[b] - n;  // position of the first new token
+    int n, stand;  // position of the first new token
+    const int t0 = a.seq.first(b, n, stand);
+    const int len = a.seq.length(b, a.kv.page_log2);
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
     // then one CTA sees to it that this kernel does not end first

@@ -547,6 +547,25 @@ def test_every_sequence_is_computed(ops, fmt, new, lens, rows, bound):
 
 
 @gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+@pytest.mark.parametrize("new,rows", [([3, 4], 5), ([20, 30], 35), ([300, 300], 450), ([300, 5], 302)])
+def test_more_new_tokens_than_rows(ops, fmt, new, rows):
+    """A token whose row is not one of the call's still has its position: the others see what they saw with it, as in
+    the write and the read."""
+    torch = _torch()
+    c = Case(ops, fmt, 2, 32, 16, new, [n + 9 for n in new])
+    for dt in (torch.float16, torch.float32):
+        q = torch.randn(sum(new), 4, 32, device="cuda").to(dt)
+        want, tol = attend_plain(q.cpu().double().numpy(), c.values, c.new, c.lens, 32 ** -0.5, True,
+                                 *((2.0 ** -21,) * 2 if dt == torch.float32 else (2.0 ** -15, 2.0 ** -11)), UNIT[str(dt).split(".")[1]])
+        got = c.cache.attend(c.seqs, q[:rows]).cpu().double().numpy()
+        assert (np.abs(got - want[:rows]) <= tol[:rows] + 1e-30).all()
+    for got, want in zip(c.cache.read(c.seqs, out=tuple(torch.empty(rows, 2, 32, device="cuda") for _ in range(2))),
+                         c.cache.read(c.seqs, torch.float32)):
+        assert torch.equal(got, want[:rows])
+
+
+@gpu_only
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("new,before,after,bound", [
     ([1, 3], 0, 5, 3), ([1, 3], 2, 0, 3), ([300], 7, 213, 300), ([300, 40, 1], 1, 700, 300), ([300, 2], 0, 900, 300), ([0, 0], 0, 9, 0), ([], 0, 40, 0)])
