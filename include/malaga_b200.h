@@ -262,7 +262,8 @@ MGB_API mgb_status mgb_kv_read(const mgb_kv *kv, const mgb_kv_seqs *seqs, const 
  * token t and query head h (a multiple of the cache's heads; query head h reads
  * cache head h / (q heads / cache heads)). causal: a token sees the positions up
  * to its own; otherwise all kv_len[b]. A token that sees no position gets zeros, and
- * so do rows before the first sequence's and behind the last one's.
+ * so do rows before the first sequence's and behind the last one's (a call without
+ * sequences does nothing).
  * q and out may have different types and strides, and are f32, f16 or bf16;
  * sums, maxima and outputs are held in f32 and rounded once. scale: of the
  * scores, commonly 1 / sqrt(dim). */

@@ -279,11 +279,6 @@ __device__ __forceinline__ void zero_outside(const AttendArgs &a, uint32_t b) {
     }
 }
 
-__global__ void __launch_bounds__(256) attend_nothing_kernel(const AttendArgs a) {
-    begin();
-    zero_rows(a, 0, (int)a.seq.tokens);
-}
-
 // Over the eight lanes that share t (the keys of a block).
 __device__ __forceinline__ float max_keys(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -1045,7 +1040,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (!bad && (q->heads == 0 || q->heads % kv->heads)) bad = "query heads are not a multiple of the cache's";
     if (!bad && (uint64_t)q->tokens * q->heads > 0x7fffffffu) bad = "more than 2^31 - 1 query rows";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
-    if (q->tokens == 0) return MGB_OK;
+    if (seqs->seqs == 0 || q->tokens == 0) return MGB_OK;
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
@@ -1054,7 +1049,6 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;
     cudaError_t e;
-    if (seqs->seqs == 0) return op_launch_status(op_launch(attend_nothing_kernel, dim3(148), 256, 0, 1, a, s), op);
     switch (kv->dim) {
         case 16: e = launch<16>(a, q8, most_new, most_len, s); break;
         case 32: e = launch<32>(a, q8, most_new, most_len, s); break;

@@ -91,7 +91,7 @@ class Seqs:
         n, device = table.size(0), table.device
         self.tensors = (table, q_start, kv_len)  # kept alive
         self.device, self.index = device, table.get_device()
-        self.tokens = tokens
+        self.tokens, self.empty = tokens, n == 0
         self._c = _lib.KvSeqs(_cuda(table, "table", torch.int32), _cuda(q_start, "q_start", torch.int32, (n + 1,), device),
                               _cuda(kv_len, "kv_len", torch.int32, (n,), device), n, table.size(1),
                               max_new or 0, max_len or 0)
@@ -190,6 +190,8 @@ class PagedKV:
             co = _rows(out, "out", self.index, self.dim)
         _call(self.index, self._lib.mgb_kv_attend, self._ref, seqs._ref, ctypes.byref(cq), ctypes.byref(co),
               self._scale if scale is None else scale, causal)
+        if seqs.empty:  # a call that does nothing
+            out.zero_()
         return out
 
 
