@@ -270,6 +270,12 @@ MGB_API mgb_status mgb_kv_read(const mgb_kv *kv, const mgb_kv_seqs *seqs, const 
 MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *q, const mgb_rows *out,
                                  float scale, int causal, void *stream);
 
+/* Waits for the work of `stream` and tells whether an attention on this device
+ * gave up a wait inside its kernel since the last call (after 0.5 s; none is known
+ * that does): MGB_ERR_CUDA then, and some of the rows that such a call wrote are
+ * NaN. Not for streams that are being captured. */
+MGB_API mgb_status mgb_kv_status(void *stream);
+
 /* Rules on `rows` rows of logits x (NULL / 0 members are rules that are absent).
  * With c the number of times that a token stands among the first
  * history_len[r] ids of history[r], in this order:

@@ -75,6 +75,7 @@ SIGNATURES = {
     "mgb_kv_write": (_i, [_vp, _vp, _vp, _vp, _vp]),
     "mgb_kv_read": (_i, [_vp, _vp, _vp, _vp, _vp]),
     "mgb_kv_attend": (_i, [_vp, _vp, _vp, _vp, ctypes.c_float, _i, _vp]),
+    "mgb_kv_status": (_i, [_vp]),
     "mgb_logits_choose": (_i, [_vp, _i, ctypes.c_int64, _u32, _u32, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp]),
 }
 

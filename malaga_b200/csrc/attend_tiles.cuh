@@ -138,7 +138,7 @@ struct Shared {
     // is added to dim d of rows that see key wild[.][d]. wild_any: whether there is one.
     int wild[3][D], wild_any;
     uint32_t tmem;
-    int lost;  // a wait ran out: nothing more is computed, the rows become NaN
+    int lost;  // a wait ran out: nothing more is computed, the rows become NaN, and the device's word says so
 };
 
 // Changes the warpgroup's registers a thread from the launch's 128 to N: .inc and
@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     if (tid == 0) {
         mbar_init(&sh.q_full, kSoftWarps);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], kLoadWarps);
+            // the test hook has the first CTA wait for an arrival too many
+            mbar_init(&sh.k_full[i], kLoadWarps + (a.withhold == i && (part | blockIdx.y | b) == 0));
             mbar_init(&sh.v_full[i], kLoadWarps);
             mbar_init(&sh.v_raw[i], kLoadWarps);
             mbar_init(&sh.k_free[i], 2);
@@ -884,8 +885,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
             if (parts > 1) meet(true);
             next_tile(sp);
         }
+        if (tid == kMmaWarp * 32 && *reinterpret_cast<volatile int *>(&sh.lost)) g_wait_lost = 1;
         if (warp == kMmaWarp) {
             fence_after();
+            __syncwarp();
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         }
     }

@@ -25,6 +25,7 @@
 //    are exact.
 #include <cooperative_groups.h>
 
+#include <cstdlib>
 #include <type_traits>
 
 #include "numerics.cuh"
@@ -50,7 +51,11 @@ struct AttendArgs {
     uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
     uint32_t span;   // few rows: a sequence is cut into one part each `span` keys
+    int withhold;    // test hook: the stage of keys that never fills in the tiles' first CTA, or -1
 };
+
+// Set by a kernel in which a wait ran out, until mgb_kv_status reads it.
+__device__ uint32_t g_wait_lost;
 
 __device__ __forceinline__ float exp2_of(float x) {
     float y;
@@ -1028,6 +1033,22 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
 }  // namespace
 }  // namespace mgb
 
+extern "C" MGB_API mgb_status mgb_kv_status(void *stream) {
+    using namespace mgb;
+    static const char *op = "mgb_kv_status";
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint32_t lost = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&lost, g_wait_lost, sizeof lost, 0, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess && lost) {
+        const uint32_t none = 0;
+        e = cudaMemcpyToSymbolAsync(g_wait_lost, &none, sizeof none, 0, cudaMemcpyHostToDevice, s);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+        if (e == cudaSuccess) return op_fail(MGB_ERR_CUDA, op, "a wait of the attention ran out of time: rows of NaN in its output");
+    }
+    return op_launch_status(e, op);
+}
+
 extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *q,
                                             const mgb_rows *out, float scale, int causal, void *stream) {
     using namespace mgb;
@@ -1041,10 +1062,13 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (!bad && (uint64_t)q->tokens * q->heads > 0x7fffffffu) bad = "more than 2^31 - 1 query rows";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);
     if (seqs->seqs == 0 || q->tokens == 0) return MGB_OK;
+    // Failure-path test hook, read once: a stage of keys (0 or 1) that never fills, so that a wait runs out. Off
+    // unless the variable is set.
+    static const int withhold = getenv("MGB_TEST_WITHHOLD_KEYS") ? atoi(getenv("MGB_TEST_WITHHOLD_KEYS")) : -1;
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
-                 false, 0xffffffffu, scale * kLog2e, 1};
+                 false, 0xffffffffu, scale * kLog2e, 1, withhold};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;

@@ -2,7 +2,8 @@
 //
 // Every wait on an mbarrier is bounded by %globaltimer: after kWaitNs of device
 // time the waiter gives up, the kernel records a flag in the engine's device
-// error word and stops, and the host turns the flag into MGB_ERR_CUDA.
+// error word (the attention over paged caches: in a word of the device that
+// mgb_kv_status reads) and stops, and the host turns the flag into MGB_ERR_CUDA.
 #pragma once
 #include <stdint.h>
 

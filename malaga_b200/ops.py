@@ -4,6 +4,7 @@
       .write     the new tokens' K and V rows into their pages, quantised as they are written
       .read      the last positions of every sequence back out of the pages
       .attend    attention of new tokens over their sequences' pages
+      .check     waits, and raises if an attention gave up inside its kernel
     Seqs         the sequences of a call: page tables, new tokens, lengths
     LogitRules   repetition / frequency / presence penalties, biases and grammar masks
       .choose    the rules on logits, the greedy choice and its log-probability
@@ -193,6 +194,11 @@ class PagedKV:
         if seqs.empty:  # a call that does nothing
             out.zero_()
         return out
+
+    def check(self) -> None:
+        """Waits for the current stream's work and raises MgbError if an attention on this GPU gave up a wait
+        inside its kernel since the last check: some rows that it wrote are NaN then."""
+        _call(self.index, self._lib.mgb_kv_status)
 
 
 class LogitRules:

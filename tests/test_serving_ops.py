@@ -746,6 +746,54 @@ def test_streams_graphs_and_repeats(ops):
             assert torch.equal(a, b)
 
 
+GAVE_UP = """
+import sys
+import torch
+from malaga_b200 import _lib, ops
+
+fmt, parts = sys.argv[1], int(sys.argv[2])
+new, length = (300, 2100) if parts > 1 else (1100, 1100)
+pages = -(-length // 16)
+cache = ops.PagedKV.empty(2 * pages, 4 if parts > 1 else 16, 16, 64, fmt)
+seqs = ops.Seqs.of([list(range(pages)), list(range(pages, 2 * pages))], [new, new], [length, length])
+q = torch.randn(2 * new, cache.heads, 64, device="cuda").half()
+out = cache.attend(seqs, q)
+try:
+    cache.check()
+    raise SystemExit("no error")
+except _lib.MgbError as e:
+    assert e.code == _lib.MGB_ERR_CUDA and "ran out of time" in str(e), e
+cache.check()  # told once
+lost = out.isnan().flatten(1).any(1)
+# the first CTA has rows of the first sequence's first head alone; the caches hold zeros, and so do the other rows
+assert lost[:new].any() and not lost[new:].any() and not out[:, 1:].isnan().any() and (out[:, 1:] == 0).all()
+assert (torch.arange(1000, device="cuda").sum() == 499500).item()
+"""
+
+
+@gpu_only
+@pytest.mark.parametrize("fmt", ["f16", "q8"])
+@pytest.mark.parametrize("parts,stage", [(1, 0), (1, 1), (8, 1)])
+def test_a_wait_that_runs_out_is_told(ops, fmt, parts, stage):
+    """One CTA waits for an arrival of keys that never comes and gives up: the kernel ends, its rows are NaN,
+    mgb_kv_status says so once, and the device goes on. In a process of its own, since the hook is read once."""
+    import os
+    import subprocess
+    import sys
+
+    env = dict(os.environ, MGB_TEST_WITHHOLD_KEYS=str(stage))
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", GAVE_UP, fmt, str(parts)], env=env, cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@gpu_only
+def test_status_is_good(ops):
+    c = Case(ops, "q8", 2, 64, 16, [300, 1], [400, 50])
+    c.cache.attend(c.seqs, _torch().randn(301, 2, 64, device="cuda").half())
+    c.cache.check()
+
+
 # ---------------------------------------------------------------------------
 # Logits
 
