@@ -199,7 +199,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t parts = gridDim.x, part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
-    begin();
+    wait_for_previous();
+    if (a.turn && (part | blockIdx.y | b) == 0) {
+        if (tid == 0) give_turn(a.turn);
+        __syncthreads();
+    }
+    let_next_start();
     zero_outside(a, b);
     int n, stand;
     const int t0 = a.seq.first(b, n, stand);

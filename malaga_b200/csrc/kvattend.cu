@@ -48,6 +48,7 @@ struct AttendArgs {
     bool o_vec, q_vec16, o_vec16;  // rows that allow accesses of four numbers, of eight 16-bit ones
     uint32_t group;  // query heads of a cache head
     bool overlap;    // the kernel for few rows runs beside the one for many
+    uint32_t turn;   // the number of a call that launches both, else 0
     uint32_t few;    // sequences with at most this many rows a cache head go to the kernel for few rows
     float scale;     // times log2(e)
     uint32_t span;   // few rows: a sequence is cut into one part each `span` keys
@@ -56,6 +57,24 @@ struct AttendArgs {
 
 // Set by a kernel in which a wait ran out, until mgb_kv_status reads it.
 __device__ uint32_t g_wait_lost;
+
+// A call with both kernels: the second starts when every CTA of the first has, which
+// is after all work before the call has ended. That the second sees that work's
+// writes takes more than that: the first CTA of the tiles, for which they are visible,
+// releases the call's number here, and whoever acquires it sees them, too. A CTA that
+// does not find it (calls of several streams share the places) waits for the tiles.
+// The last CTA to stay takes the number away, so that a replayed graph starts anew.
+constexpr uint32_t kTurns = 256;
+__device__ uint32_t g_turn[kTurns];
+
+__device__ __forceinline__ void give_turn(uint32_t turn) {
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(&g_turn[turn % kTurns]), "r"(turn) : "memory");
+}
+__device__ __forceinline__ void take_turn(uint32_t turn) {
+    uint32_t got;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(got) : "l"(&g_turn[turn % kTurns]) : "memory");
+    if (got != turn) wait_for_previous();
+}
 
 __device__ __forceinline__ float exp2_of(float x) {
     float y;
@@ -591,8 +610,8 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t part = blockIdx.x, heads = a.kv.heads;
     const uint32_t head = blockIdx.y % heads, b = blockIdx.z;
-    // beside the launch for many rows, which has seen the one before it end
-    if (a.overlap) {
+    if (a.overlap) {  // beside the launch for many rows
+        take_turn(a.turn);
         let_next_start();
     } else {
         begin();
@@ -605,8 +624,13 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
     // then one CTA sees to it that this kernel does not end first
     const bool keeper = a.overlap && blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && b == gridDim.z - 1;
+    auto keep = [&] {
+        if (!keeper) return;
+        wait_for_previous();
+        if (tid == 0) atomicCAS(&g_turn[a.turn % kTurns], a.turn, 0u);
+    };
     if ((uint32_t)rows > a.few) {
-        if (keeper) wait_for_previous();
+        keep();
         return;
     }
     // a shorter sequence takes fewer of the cluster's CTAs; the others leave (its barriers count the threads that stay)
@@ -913,7 +937,7 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
         if (parts > 1) cluster_sync();
         else __syncthreads();
     }
-    if (keeper) wait_for_previous();
+    keep();
 }
 
 template <int D, bool Q8, bool SPLIT, int NT>
@@ -1022,6 +1046,8 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
     // have, a bound too small), so without the second launch the tiles take them all.
     const bool both = a.seq.tokens < most_new * a.seq.seqs;
     a.few = both ? kFewRows : 0;
+    static std::atomic<uint32_t> calls{0};
+    while (both && !a.turn) a.turn = ++calls;
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
     if (e == cudaSuccess && both) {
         a.overlap = true;
@@ -1068,7 +1094,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     AttendArgs a{view(*kv), view(*seqs, q->tokens), q->data, out->data, q->token_stride, q->head_stride,
                  out->token_stride, out->head_stride, q->type, out->type, causal != 0, rows_vec(*out), rows_vec16(*q), rows_vec16(*out),
                  q->heads / kv->heads,
-                 false, 0xffffffffu, scale * kLog2e, 1, withhold};
+                 false, 0, 0xffffffffu, scale * kLog2e, 1, withhold};
     const uint64_t most_new = bound_new(*seqs, q->tokens), most_len = bound_len(*seqs, kv->page);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool q8 = kv->format == MGB_KV_Q8;

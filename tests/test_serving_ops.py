@@ -794,6 +794,68 @@ def test_status_is_good(ops):
     c.cache.check()
 
 
+@gpu_only
+def test_mixed_calls_read_what_was_just_written(ops):
+    """Both kernels of a call of unlike sequences start from what the kernel right before it wrote (queries, lengths,
+    page tables, the cache), on two streams at once and in a replayed graph."""
+    torch = _torch()
+    c = Case(ops, "f16", 4, 64, 16, [300, 1, 7, 20], [900, 700, 400, 333])
+    steps = 24
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(steps, 328, 4, 64, device="cuda", generator=gen).half()
+    k = torch.randn(steps, 328, 4, 64, device="cuda", generator=gen).half()
+    less = torch.randint(0, 90, (steps, 4), device="cuda", generator=gen, dtype=torch.int32)
+
+    class Side:
+        def __init__(self):
+            self.cache = ops.PagedKV(c.cache.k.clone(), c.cache.v.clone())
+            self.table, self.start, self.length = (x.clone() for x in c.seqs.tensors)
+            self.seqs = ops.Seqs(self.table, self.start, self.length, 300, 900)
+            self.q, self.k, self.out = torch.zeros_like(q[0]), torch.zeros_like(k[0]), torch.zeros_like(q[0])
+
+        def step(self, i, settle):
+            """i: the step's number on the device, [1]."""
+            pages = c.seqs.tensors[0].shape[1]
+            self.cache.write(self.seqs, self.k, self.k)
+            torch.index_select(k, 0, i, out=self.k[None])
+            self.length.copy_((c.seqs.tensors[2][None] - less[i])[0])
+            self.table[1, : pages // 2].copy_(c.seqs.tensors[0][1][: pages // 2].roll(3))
+            torch.index_select(q, 0, i, out=self.q[None])
+            if settle:
+                torch.cuda.synchronize()
+            self.cache.attend(self.seqs, self.q, out=self.out)
+            return self.out
+
+    numbers = torch.arange(steps, device="cuda")
+    side, want = Side(), []
+    for i in range(steps):
+        want.append(side.step(numbers[i: i + 1], True).clone())
+        torch.cuda.synchronize()
+    streams, sides, got = [torch.cuda.Stream() for _ in range(2)], [Side(), Side()], [[], []]
+    torch.cuda.synchronize()
+    for i in range(steps):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[s].append(sides[s].step(numbers[i: i + 1], False).clone())
+    torch.cuda.synchronize()
+    for s in range(2):
+        for a, b in zip(got[s], want):
+            assert torch.equal(a, b)
+    side, at = Side(), torch.zeros(1, dtype=torch.int64, device="cuda")
+    fresh = [x.clone() for x in (side.cache.k, side.cache.v, side.k, side.length, side.table)]
+    side.step(at, False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.step(at, False)
+    for x, y in zip((side.cache.k, side.cache.v, side.k, side.length, side.table), fresh):
+        x.copy_(y)
+    for i in range(steps):
+        at.fill_(i)
+        graph.replay()
+        assert torch.equal(side.out, want[i])
+
+
 # ---------------------------------------------------------------------------
 # Logits
 
