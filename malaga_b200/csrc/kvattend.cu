@@ -1083,6 +1083,7 @@ extern "C" MGB_API mgb_status mgb_kv_attend(const mgb_kv *kv, const mgb_kv_seqs 
     if (!bad) bad = check_seqs(seqs);
     if (!bad) bad = check_rows(q);
     if (!bad) bad = check_rows(out);
+    if (!bad) bad = check_out(out);
     if (!bad && (q->tokens != out->tokens || q->heads != out->heads)) bad = "q and out differ in shape";
     if (!bad && (q->heads == 0 || q->heads % kv->heads)) bad = "query heads are not a multiple of the cache's";
     if (!bad && (uint64_t)q->tokens * q->heads > 0x7fffffffu) bad = "more than 2^31 - 1 query rows";

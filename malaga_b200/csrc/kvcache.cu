@@ -229,6 +229,8 @@ mgb_status move(const mgb_kv *kv, const mgb_kv_seqs *seqs, const mgb_rows *k, co
     if (!bad) bad = check_seqs(seqs);
     if (!bad) bad = check_rows(k);
     if (!bad) bad = check_rows(v);
+    if (!bad && !WRITE) bad = check_out(k);
+    if (!bad && !WRITE) bad = check_out(v);
     if (!bad && (k->tokens != v->tokens)) bad = "K and V differ in their tokens";
     if (!bad && (k->heads != kv->heads || v->heads != kv->heads)) bad = "the rows' heads are not the cache's";
     if (bad) return op_fail(MGB_ERR_INVALID, op, bad);

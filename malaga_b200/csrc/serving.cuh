@@ -149,6 +149,12 @@ inline const char *check_rows(const mgb_rows *r) {
     return nullptr;
 }
 
+// Rows that are written: none of them is another's place.
+inline const char *check_out(const mgb_rows *r) {
+    if ((r->tokens > 1 && r->token_stride == 0) || (r->heads > 1 && r->head_stride == 0)) return "rows that are written overlap";
+    return nullptr;
+}
+
 inline KvView view(const mgb_kv &kv) {
     return KvView{kv.k, kv.v, kv.k_scale, kv.v_scale, kv.pages, kv.heads, log2_of(kv.page), kv.dim};
 }

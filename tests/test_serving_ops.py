@@ -1077,6 +1077,32 @@ def test_library_refuses_more():
     assert choose(16, 0, 8, 0, 8, None, None, None, None, 0, None) == _lib.MGB_OK
 
 
+def test_library_refuses_rows_written_twice():
+    """A broadcast tensor as an output, whose result would be whichever store came last; as an input it is welcome."""
+    lib = _lib.load(build_if_missing=True)
+    ref = ctypes.byref
+    kv, seqs, good = _kv(), _seqs(), _rows(tokens=3)
+    for bad in (_rows(tokens=3, token_stride=0), _rows(tokens=3, head_stride=0)):
+        for call in (lambda: lib.mgb_kv_read(ref(kv), ref(seqs), ref(good), ref(bad), None),
+                     lambda: lib.mgb_kv_read(ref(kv), ref(seqs), ref(bad), ref(good), None),
+                     lambda: lib.mgb_kv_attend(ref(kv), ref(seqs), ref(good), ref(bad), 1.0, 1, None)):
+            assert call() == _lib.MGB_ERR_INVALID
+            assert "overlap" in lib.mgb_last_error().decode()
+
+
+@gpu_only
+def test_broadcast_rows_as_inputs(ops):
+    torch = _torch()
+    c = Case(ops, "f16", 2, 32, 16, [5], [9])
+    one = torch.randn(1, 1, 32, device="cuda").half()
+    c.cache.write(c.seqs, one.expand(5, 2, 32), one.expand(5, 2, 32))
+    assert torch.equal(c.cache.read(c.seqs)[0], one.expand(5, 2, 32))
+    q = one.expand(5, 2, 32)
+    assert torch.equal(c.cache.attend(c.seqs, q), c.cache.attend(c.seqs, q.contiguous()))
+    single = torch.empty(1, 2, 32, device="cuda")[:, :, :].expand(1, 2, 32)
+    assert c.cache.attend(ops.Seqs.of(c.tables, [1], c.lens), q[:1], out=single) is single
+
+
 @gpu_only
 def test_python_refuses(ops):
     torch = _torch()
