@@ -205,9 +205,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tiles_kernel(const AttendA
         __syncthreads();
     }
     let_next_start();
-    zero_outside(a, b);
-    int n, stand;
-    const int t0 = a.seq.first(b, n, stand);
+    int n, stand, start, stop;
+    const int t0 = a.seq.first(b, n, stand, start, stop);
+    zero_outside(a, b, start, stop);
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
     if ((uint32_t)rows <= a.few) return;  // left to the kernel for few rows; the whole cluster leaves
     const int len = a.seq.length(b, a.kv.page_log2);

@@ -290,17 +290,11 @@ __device__ __forceinline__ void zero_rows(const AttendArgs &a, int from, int to)
     zero_rows(a.out, a.o_type, a.o_vec, a.o_token, a.o_head, a.kv.heads * a.group, a.kv.dim / 4, from, to);
 }
 
-// Rows before the first sequence's and behind the last one's see nothing: zeros.
-__device__ __forceinline__ void zero_outside(const AttendArgs &a, uint32_t b) {
+// Rows before the first sequence's and behind the last one's see nothing: zeros. start, stop: sequence b's.
+__device__ __forceinline__ void zero_outside(const AttendArgs &a, uint32_t b, int start, int stop) {
     const int tokens = (int)a.seq.tokens;
-    if (b == 0) {
-        const int first = min(tokens, a.seq.q_start[0]);
-        if (first > 0) zero_rows(a, 0, first);
-    }
-    if (b + 1 == a.seq.seqs) {
-        const int stop = max(0, a.seq.q_start[a.seq.seqs]);
-        if (stop < tokens) zero_rows(a, stop, tokens);
-    }
+    if (b == 0 && start > 0) zero_rows(a, 0, min(tokens, start));
+    if (b + 1 == a.seq.seqs && stop < tokens) zero_rows(a, max(0, stop), tokens);
 }
 
 // Over the eight lanes that share t (the keys of a block).
@@ -615,13 +609,13 @@ __global__ void __launch_bounds__(kRowThreads, Frag<D, Q8>::ctas(NT) + (D == 16 
         let_next_start();
     } else {
         begin();
-        zero_outside(a, b);
     }
-    int n, stand;  // position of the first new token
-    const int t0 = a.seq.first(b, n, stand);
+    int n, stand, start, after;  // stand: position of the first new token
+    const int t0 = a.seq.first(b, n, stand, start, after);
     const int len = a.seq.length(b, a.kv.page_log2);
     const int32_t *table = a.seq.table + (size_t)b * a.seq.table_stride;
     const int rows = n * (int)a.group;  // the call has fewer than 2^31 query rows
+    if (!a.overlap) zero_outside(a, b, start, after);
     // then one CTA sees to it that this kernel does not end first
     const bool keeper = a.overlap && blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && b == gridDim.z - 1;
     auto keep = [&] {

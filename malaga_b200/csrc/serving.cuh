@@ -98,10 +98,11 @@ struct SeqView {
     const int32_t *table, *q_start, *kv_len;
     uint32_t seqs, table_stride, tokens;
     // First row and number of the new tokens of sequence b, kept inside the
-    // call's rows, and the first one's position; positions of the sequence, kept
-    // inside its table.
-    __device__ __forceinline__ int first(uint32_t b, int &n, int &position) const {
-        const int t0 = max(0, q_start[b]), t1 = q_start[b + 1];
+    // call's rows, and the first one's position; `start` and `stop`, q_start as it
+    // stands. Positions of the sequence, kept inside its table.
+    __device__ __forceinline__ int first(uint32_t b, int &n, int &position, int &start, int &stop) const {
+        start = q_start[b], stop = q_start[b + 1];
+        const int t0 = max(0, start), t1 = stop;
         n = max(0, min((int)tokens, t1) - t0);
         // the last token's is kv_len - 1, whether or not its row is one of the call's
         position = (int)max(-0x7fffffffll, min(0x7fffffffll, (long long)kv_len[b] - ((long long)t1 - t0)));
