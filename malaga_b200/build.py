@@ -32,8 +32,9 @@ NVCC_FLAGS = [
 # Compiled in one piece: with --split-compile the same source got one of several
 # register assignments from build to build, which moved the attention kernels by up
 # to 15 % and the logit rules from 29 to 33 us (34.5 in one piece; one row 6.9 us
-# against 7.0 to 7.8). Level 3: most attention instances spill least and run fastest
-# (8192 tokens over 16384 keys of dim 128 in f16: 1.16 ms, 1.29 without).
+# against 7.0 to 7.8). Level 3: the attention's tiles spill least and run fastest (8192
+# tokens over 16384 keys of dim 128 in f16: 1.05 ms, 1.20 without; few rows take 1 to 3 %
+# longer with it).
 SOURCE_FLAGS = {"kvcache.cu": [], "kvattend.cu": ["-Xptxas=--register-usage-level=3"], "logits.cu": []}
 ENGINE_SOURCES = ["engine.cu", "noalloc.cu", "kvcache.cu", "kvattend.cu", "logits.cu"]
 OBJ_DIR = os.path.join(HERE, "_build")

@@ -12,11 +12,12 @@
 // over the values of the tiles that some rows do not see whole, before their product
 // (done by the loading warps it cost 6 to 12 % on every tile, in registers).
 // What bounds it: a step of 128 keys in f16 takes 4200 (dim 64) to 5600 cycles (dim 128) of
-// which the tensor core computes 1024 and 2048 and the exponentials take 2048. While
-// one row tile's exponentials run, the other's stores, barriers and products wait in
-// the same queue for some 100 cycles each, so neither unit is ever full: 8192 tokens
-// over 16384 positions of 16 heads of dim 128, causal, take 1.16 ms in f16 (710
-// TFLOP/s) and 1.23 ms in 8 bits, of dim 64 0.77 and 0.95 ms.
+// which the tensor core computes 1024 and 2048 and the exponentials take 2048. No unit
+// is full (4099 tokens over 20,011 positions, 8 bits: tensor pipe 32 % of the cycles,
+// exponentials 25 %, issue slots 44 %); warps wait for scores, tensor memory and
+// barriers, one row tile's chain of scores, softmax and product only partly under the
+// other's. 8192 tokens over 16384 positions of 16 heads of dim 128, causal, take 1.05
+// ms in f16 (790 TFLOP/s) and 1.22 ms in 8 bits, of dim 64 0.77 and 0.99 ms.
 // Registers go where a whole row of scores is held (setmaxnreg). Operands lie
 // in the K-major layout without swizzle: 8 rows x 16 bytes are one 128-byte
 // block, so a warp's 16-byte stores cover whole blocks; V is read from the same

@@ -167,9 +167,9 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
 //
 // What bounds it: HBM with long f16 caches (6.3 TB/s at dim 128), the instructions a
 // key with 8-bit ones (8 sequences, 233,369 positions, 8 heads of 128, four rows
-// each: 112 us, 4.4 TB/s), latencies with short ones (one row of 33 positions, 16
-// heads of 64: 3.7 us; 64 sequences of 272 positions on average and 1024 at most, 16
-// heads of 64, 8 bits: 21 us, of which the longest sequence's loop is 12).
+// each: 116 us, 4.2 TB/s), latencies with short ones (one row of 33 positions, 16
+// heads of 64: 4.1 us; 64 sequences of 272 positions on average and 1024 at most, 16
+// heads of 64, 8 bits: 22 us, of which the longest sequence's loop is 12).
 
 template <int D, bool Q8>
 struct Frag {
@@ -1021,7 +1021,8 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
 // (100 to 250 new tokens, 1500 to 16,000 positions, 8 and 16 heads, 1 to 16
 // sequences) put as: it takes 6 us and 0.3 + dim / 95 us (8 bits: 0.6 + dim / 105)
 // for every 28,500 pairs of a 16-row tile and a key, the tiles 30 us (8 bits: 34)
-// and 0.3 + dim / 120 us for each of tiles_cost's key tiles. Over 4000 positions,
+// and 0.3 + dim / 120 us for each of tiles_cost's key tiles (dim 32 follows from the
+// others; causal calls have as little as half of these pairs, others all). Over 4000 positions,
 // 16 heads of 64, f16: 100 rows 22 against 32 us, 200 rows 30 against 40; 100 rows
 // over 1500 in 16 sequences 98 against 63.
 template <int D>

@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(kThreads) kv_move_kernel(const MoveArgs a) {
     }
 }
 
-// As many tokens a CTA as leave two CTAs an SM (148 SMs) on either side, so that
-// all run at once and look their places up once.
+// Few tokens: as many a CTA as leave two CTAs an SM (148 SMs) on either side, so that
+// all run at once. From 296 * kMaxTokens on kMaxTokens a CTA, and more CTAs.
 template <int DIM, bool Q8, bool WRITE>
 cudaError_t launch(MoveArgs a, int sides, int type, bool vec, cudaStream_t s) {
     const uint32_t n = a.seq.tokens / (2 * 148);

@@ -180,7 +180,8 @@ class PagedKV:
         softmax(scale * q k) v, scale 1 / sqrt(dim) unless given. Query head h reads cache head
         h // (query heads / heads). causal: a token sees the positions up to its own, else all of its
         sequence. A token that sees nothing gets zeros, and so does a row of no sequence. Returns out (q's
-        type and shape unless given)."""
+        type and shape unless given). Sums are held in f32; with float16 or bfloat16 q each key's weight counts
+        to 2^-11 of itself, with float32 q to 2^-21."""
         self._check(seqs)
         cq = _rows(q, "q", self.index, self.dim)
         if out is None:
