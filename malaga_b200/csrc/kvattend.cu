@@ -1015,6 +1015,14 @@ cudaError_t launch_tiles(const AttendArgs &a, uint64_t most_new, uint64_t most_l
                      tiles::Smem<D>::ASKED, parts, a, s);
 }
 
+// Numbers of calls with both kernels, of all dims alike; never 0.
+uint32_t next_turn() {
+    static std::atomic<uint32_t> calls{0};
+    uint32_t turn = ++calls;
+    while (!turn) turn = ++calls;
+    return turn;
+}
+
 // Which kernel. f32 queries, whose two f16 parts only the kernel for few rows
 // takes, and calls of at most kFewRows rows a cache head go there. So do calls of
 // at most 256 rows where it is faster, which measurements at dims 16, 64 and 128
@@ -1041,8 +1049,7 @@ cudaError_t launch(AttendArgs a, bool q8, uint64_t most_new, uint64_t most_len, 
     // have, a bound too small), so without the second launch the tiles take them all.
     const bool both = a.seq.tokens < most_new * a.seq.seqs;
     a.few = both ? kFewRows : 0;
-    static std::atomic<uint32_t> calls{0};
-    while (both && !a.turn) a.turn = ++calls;
+    if (both) a.turn = next_turn();
     cudaError_t e = q8 ? launch_tiles<D, true>(a, most_new, most_len, s) : launch_tiles<D, false>(a, most_new, most_len, s);
     if (e == cudaSuccess && both) {
         a.overlap = true;
