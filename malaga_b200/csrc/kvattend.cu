@@ -427,7 +427,7 @@ struct Rows {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) past |= s[i][n][e] != kLowest && fabsf(x[i].vs[e >> 1]) * back[n][e & 1] >= 1.0f;
+                        for (int e = 0; e < 4; ++e) past |= key0 + 16 * i + g + 8 * (e >> 1) < limit[n][e & 1] && fabsf(x[i].vs[e >> 1]) * back[n][e & 1] >= 1.0f;
                 }
             }
         }
@@ -455,7 +455,7 @@ struct Rows {
                             for (int i = 0; i < B; ++i)
 #pragma unroll
                                 for (int u = 0; u < 2; ++u)
-                                    if (s[i][n][2 * u + r] != kLowest) seen = fmaxf(seen, fabsf(x[i].vs[u]));
+                                    if (key0 + 16 * i + g + 8 * u < limit[n][r]) seen = fmaxf(seen, fabsf(x[i].vs[u]));
                             seen = max_keys(seen);
                         }
                         const float now = fminf(back[n][r], over(seen));

@@ -416,6 +416,31 @@ def test_scales_of_later_tokens_never_reach_a_row(ops, new, first, dim, size):
 
 
 @gpu_only
+def test_a_score_below_all_numbers_beside_a_hole(ops):
+    """Two rows of a tile, of which one's score of a key is -inf, where V's scale is large and the page behind is missing:
+    the other row's later keys keep their weight."""
+    torch = _torch()
+    c = Case(ops, "q8", 1, 32, 16, [1], [700], stale=0.0)
+    page, at = c.tables[0][0], 3
+    c.cache.k[page, 0, at] = 100
+    c.cache.k_scale[page, 0, at] = 1e25
+    c.cache.v_scale[page, 0, at] *= 2.0 ** 40
+    table = c.seqs.tensors[0].clone()
+    table[0, 1] = c.cache.pages
+    seqs = ops.Seqs(table, *c.seqs.tensors[1:], 1, 700)
+    q = torch.empty(1, 2, 32, device="cuda")
+    q[0, 0], q[0, 1] = -1e20, -5e-28
+    c.values[0][0][at, 0] = 100 * float(c.cache.k_scale[page, 0, at])
+    c.values[0][1][at, 0] *= 2.0 ** 40
+    short = [[np.delete(x, range(16, 32), 0) for x in c.values[0]]]
+    for dt in (torch.float32, torch.bfloat16):
+        units = (2.0 ** -21, 2.0 ** -21, 2.0 ** -24) if dt == torch.float32 else (2.0 ** -15, 2.0 ** -11, 2.0 ** -24)
+        want, tol = attend_plain(q.to(dt).cpu().double().numpy(), short, [1], [684], 32 ** -0.5, True, *units)
+        got = c.cache.attend(seqs, q.to(dt), out=torch.empty_like(q)).cpu().double().numpy()
+        assert (np.abs(got - want) <= tol)[0, 1].all(), (np.abs(got - want) / tol)[0, 1].max()
+
+
+@gpu_only
 @pytest.mark.parametrize("new,length", [(1, 40), (3, 9001), (20, 700), (150, 160), (300, 2100)])
 @pytest.mark.parametrize("size", [1e36, 1e-34])
 def test_values_near_the_ends_of_the_range(ops, new, length, size):
